@@ -326,6 +326,63 @@ int lq_zrmsnorm_fwd(const void* x, const float* scale, int dtype, int64_t rows, 
 int lq_zrmsnorm_bwd(const void* dy, const void* x, const float* scale, const float* rstd, int dtype,
                     int64_t rows, int64_t h, void* dx, void* stream);
 
+/* The seam between two sub-blocks in one pass (crates/loractl-core/src/mmdit.rs:857-869 with the norms of
+ * :282-330; the reference runs it as broadcast tensor ops): the norm behind a sub-block, its gate and
+ * residual scale, and the modulated norm before the next sub-block,
+ *
+ *     u = y                 or, with post_weight,  y * rsqrt(mean(y^2) + eps) * (1 + post_weight)
+ *     r = alpha * x + gate * u                     (r = x when y is NULL; alpha is then not applied)
+ *     z = (r - mu) * rsqrt(mean((r - mu)^2) + eps) * (1 + weight) * (1 + scale) + shift
+ *
+ * mu = mean(r) when `layer` is non-zero, else 0.  x, y, r, z have element type `dtype` (LQ_F32 or LQ_BF16);
+ * rows are `h` contiguous elements (1 <= h <= 16384), x and y with any sample and token stride (in
+ * elements), r and z contiguous [samples, tokens, h].  gate, shift, scale: [samples, h] with a sample stride
+ * (0 broadcasts one vector over the samples), all f32 (`mod_f32` = 1) or all bf16 (0).  weight, post_weight:
+ * f32 [h], may be NULL.  Arithmetic is f32; z is formed from the unrounded r.  Rows and vectors that all start on 16 bytes
+ * (h a multiple of 8) take 16-byte accesses, others single elements.
+ * rstd, mean (layer), post_rstd (post_weight): f32 [samples * tokens], written by the forward when rstd is
+ * not NULL and read by the backward.  r may be NULL. */
+typedef struct lq_residual_norm_args {
+    const void* x;
+    const void* y;
+    const void* gate;
+    const void* shift;
+    const void* scale;
+    const float* weight;
+    const float* post_weight;
+    void* r;
+    void* z;
+    float* mean;
+    float* rstd;
+    float* post_rstd;
+    int64_t x_sample, x_token, y_sample, y_token;
+    int64_t gate_sample, shift_sample, scale_sample;
+    int64_t samples, tokens, h;
+    int32_t dtype, mod_f32, layer;
+    float alpha, eps;
+} lq_residual_norm_args;
+/* Gradients of the same call.  dr, dz: the outputs' gradients (`dtype`, any sample and token stride; NULL = zero).
+ * dx, dy: contiguous, `dtype`.  dgate, dshift, dscale: contiguous [samples, h] in the type of the modulation vectors;
+ * dweight, dpost_weight: f32 [h], summed over the samples.  Each may be NULL.  The token sums go through `ws`
+ * (lq_residual_norm_workspace_bytes() bytes on the current device, 16-byte aligned; not needed when none is asked for)
+ * in a fixed order: two runs are bit-identical. */
+typedef struct lq_residual_norm_grads {
+    const void* dr;
+    const void* dz;
+    int64_t dr_sample, dr_token, dz_sample, dz_token;
+    void* dx;
+    void* dy;
+    void* dgate;
+    void* dshift;
+    void* dscale;
+    float* dweight;
+    float* dpost_weight;
+} lq_residual_norm_grads;
+size_t lq_residual_norm_workspace_bytes(int64_t samples, int64_t tokens, int64_t h);
+int lq_residual_norm_fwd(const lq_residual_norm_args* args, void* stream);
+int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_norm_grads* grads, void* ws,
+                         size_t ws_bytes, void* stream);
+
 /* ---- diagnostics -------------------------------------------------------------- */
 
 /* Device-side waits in the kernels are bounded; one that gives up records a code in a

@@ -13,7 +13,7 @@ from .fp8 import e4m3fn_lut, fp8_quantize, weight_from_fp8
 from .config import BackendKind, ComputeConfig, Precision, validate_b200
 from .optim import AdamW, DynamicLossScale, FlatAdapters, nonfinite_flag
 from .block_ckpt import checkpointed_step
-from . import dp, export, loader
+from . import block_ops, dp, export, loader
 from .export import export_adapters, import_adapters
 from .loader import load_quant_module
 
@@ -23,6 +23,6 @@ __all__ = [
     "LoraDelta", "LoraLinear", "init_factors", "LoraAdapters", "LoraConfig", "LoraSite", "TargetSpec",
     "build_adapters", "BaseLinear", "QuantLinear", "site", "e4m3fn_lut", "fp8_quantize", "weight_from_fp8",
     "BackendKind", "ComputeConfig", "Precision", "validate_b200",
-    "AdamW", "DynamicLossScale", "FlatAdapters", "nonfinite_flag", "checkpointed_step", "dp",
+    "AdamW", "DynamicLossScale", "FlatAdapters", "nonfinite_flag", "checkpointed_step", "block_ops", "dp",
     "export", "loader", "export_adapters", "import_adapters", "load_quant_module",
 ]

@@ -37,6 +37,22 @@ class MirrorJob(C.Structure):
                 ("mirror", C.c_void_p)]
 
 
+class ResidualNormArgs(C.Structure):
+    """`lq_residual_norm_args` of include/loractl_b200.h."""
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "y", "gate", "shift", "scale", "weight", "post_weight", "r", "z", "mean", "rstd",
+                                           "post_rstd")]
+                + [(n, C.c_int64) for n in ("x_sample", "x_token", "y_sample", "y_token", "gate_sample", "shift_sample",
+                                            "scale_sample", "samples", "tokens", "h")]
+                + [(n, C.c_int32) for n in ("dtype", "mod_f32", "layer")] + [("alpha", C.c_float), ("eps", C.c_float)])
+
+
+class ResidualNormGrads(C.Structure):
+    """`lq_residual_norm_grads` of include/loractl_b200.h."""
+    _fields_ = ([("dr", C.c_void_p), ("dz", C.c_void_p)]
+                + [(n, C.c_int64) for n in ("dr_sample", "dr_token", "dz_sample", "dz_token")]
+                + [(n, C.c_void_p) for n in ("dx", "dy", "dgate", "dshift", "dscale", "dweight", "dpost_weight")])
+
+
 class WeightInfo(C.Structure):
     _fields_ = [
         ("d_out", C.c_int64), ("d_in", C.c_int64), ("scheme", C.c_int32), ("group", C.c_int32),
@@ -86,6 +102,9 @@ SIGNATURES = {
     "lq_sigmoid_gate_fwd": (_I, [_P, _P, _I, _I64, _P, _P]),
     "lq_sigmoid_gate_bwd": (_I, [_P, _P, _P, _I, _I64, _P, _P, _P]),
     "lq_gate_residual_bwd": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, C.c_size_t, _P]),
+    "lq_residual_norm_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "lq_residual_norm_fwd": (_I, [C.POINTER(ResidualNormArgs), _P]),
+    "lq_residual_norm_bwd": (_I, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads), _P, _SZ, _P]),
     "lq_check_device_status": (_I, [_P]),
     "lq_selftest_bounded_wait": (_I, [C.c_uint, _P]),
     "lq_kernel_launch_count": (C.c_uint64, []),

@@ -5,6 +5,8 @@
     swiglu(gate, up)                      = silu(gate) * up           (mmdit.rs:695-708)
     sigmoid_gate(x, gate)                 = x * sigmoid(gate)         (mmdit.rs:659-664)
     zrmsnorm(x, scale)                    = x / sqrt(mean(x^2) + 1e-5) * (scale + 1)   (mmdit.rs:282-330)
+    modulated_zrmsnorm(x, w, shift, scale) = zrmsnorm(x, w) * (1 + scale) + shift
+    gated_residual_norm(x, gate, y, ..)   = r = a x + gate * post(y) and the modulated norm of r, in one pass
 
 the pattern of crates/loractl-core/src/mmdit.rs:857-869 (`(prescale + 1) * prenorm(x) + preshift`,
 `x + pregate * attn(..)`, ...).  `x`, `y` are `[b, tokens, h]`; `shift`, `scale`, `gate` are
@@ -15,9 +17,11 @@ CUDA tensors only (f32 or bf16): like every other op of this package there is no
 """
 from __future__ import annotations
 
-from typing import Dict, Tuple
+import ctypes as C
+from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .quant import _dtype_code, _require_cuda, _stream_ptr
@@ -203,3 +207,141 @@ class _ZRmsNorm(torch.autograd.Function):
 def zrmsnorm(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """ZRmsNorm over the last axis with a frozen `scale` (no gradient flows to it), one kernel each way."""
     return _ZRmsNorm.apply(x, scale)
+
+
+# ---- the seam between two sub-blocks --------------------------------------------------------------
+
+
+def _rows(v: torch.Tensor) -> torch.Tensor:
+    """`v` itself when its rows are contiguous (any sample and token stride), a copy otherwise."""
+    return v if v.stride(-1) == 1 or v.shape[-1] == 1 else v.contiguous()
+
+
+def _strides(v: torch.Tensor) -> Tuple[int, int]:
+    return v.stride(0), v.stride(1)
+
+
+def _vectors(b: int, h: int, **vectors: torch.Tensor):
+    """The modulation vectors as `[b, h]` views of one type: theirs when they agree on f32 or bf16, else f32."""
+    for name, v in vectors.items():
+        if v.numel() != b * h or v.shape[0] != b or v.shape[-1] != h:
+            raise ValueError(f"{name} must be [b = {b}, h = {h}] or [b, 1, h], got {list(v.shape)}")
+        if v.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"unsupported {name} dtype {v.dtype}: f32 or bf16")
+    kinds = {v.dtype for v in vectors.values()}
+    dtype = kinds.pop() if len(kinds) == 1 else torch.float32
+    out = {}
+    for name, v in vectors.items():
+        v = v.to(dtype).reshape(b, h)
+        out[name] = v if v.stride(1) == 1 or h == 1 else v.contiguous()
+    return out, dtype
+
+
+def _norm_weight(w: Optional[torch.Tensor], h: int, name: str) -> Optional[torch.Tensor]:
+    if w is None:
+        return None
+    if w.numel() != h:
+        raise ValueError(f"{name} must hold {h} values, got {list(w.shape)}")
+    return w.detach().to(torch.float32).reshape(h).contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, y, shift, scale, weight, post_weight, layer, alpha, eps):
+        _require_cuda(x, "x")
+        b, t, h = _dims(x)
+        dtype = _dtype_code(x)
+        if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
+            raise ValueError(f"x and y must agree in shape and dtype, got {list(x.shape)} {x.dtype} / {list(y.shape)} {y.dtype}")
+        named = {"shift": shift, "scale": scale} if y is None else {"gate": gate, "shift": shift, "scale": scale}
+        for name, v in {**named, "y": y, "weight": weight, "post_weight": post_weight}.items():
+            if v is not None and v.device != x.device:
+                raise RuntimeError(f"{name} is on {v.device}, x on {x.device}")
+        mods, mod_dtype = _vectors(b, h, **named)
+        w, pw = _norm_weight(weight, h, "weight"), _norm_weight(post_weight, h, "post_weight")
+        xr, yr = _rows(x), None if y is None else _rows(y)
+        z = torch.empty((b, t, h), dtype=x.dtype, device=x.device)
+        r = torch.empty_like(z) if y is not None else None
+        args = L.ResidualNormArgs(x=_ptr(xr), y=_ptr(yr), shift=_ptr(mods["shift"]), scale=_ptr(mods["scale"]), weight=_ptr(w),
+                                  post_weight=_ptr(pw), r=_ptr(r), z=_ptr(z), samples=b, tokens=t, h=h, dtype=dtype,
+                                  mod_f32=int(mod_dtype == torch.float32), layer=int(layer), alpha=alpha, eps=eps)
+        args.x_sample, args.x_token = _strides(xr)
+        args.shift_sample, args.scale_sample = mods["shift"].stride(0), mods["scale"].stride(0)
+        if yr is not None:
+            args.y_sample, args.y_token = _strides(yr)
+            args.gate, args.gate_sample = _ptr(mods["gate"]), mods["gate"].stride(0)
+        stats = None
+        if any(ctx.needs_input_grad):
+            stats = torch.empty((3, b * t), dtype=torch.float32, device=x.device)
+            args.mean, args.rstd, args.post_rstd = (stats[i].data_ptr() for i in range(3))
+        with torch.cuda.device(x.device):
+            L.check(L.lib().lq_residual_norm_fwd(C.byref(args), _stream_ptr(x.device)))
+        ctx.args = args  # the addresses are those of the saved tensors below, except r and z, which the backward does not read
+        ctx.mod_dtype = mod_dtype
+        ctx.like = [None if v is None else (v.shape, v.dtype) for v in (gate, shift, scale, weight, post_weight)]
+        ctx.save_for_backward(xr, yr, mods.get("gate"), mods["shift"], mods["scale"], w, pw, stats)
+        ctx.set_materialize_grads(False)
+        return z if r is None else (r, z)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *douts):
+        dr, dz = douts if len(douts) == 2 else (None, douts[0])
+        if dr is None and dz is None:
+            return (None,) * 10
+        xr, yr, gate, shift, scale, w, pw, stats = ctx.saved_tensors
+        b, t, h = xr.shape
+        dev, args = xr.device, ctx.args
+        need = ctx.needs_input_grad
+        new = lambda wanted, dtype, *shape: torch.empty(shape, dtype=dtype, device=dev) if wanted else None
+        dx, dy = new(need[0], xr.dtype, b, t, h), new(need[2], xr.dtype, b, t, h)
+        dgate, dshift, dscale = (new(need[i], ctx.mod_dtype, b, h) for i in (1, 3, 4))
+        dw, dpw = new(need[5], torch.float32, h), new(need[6], torch.float32, h)
+        g = L.ResidualNormGrads(dx=_ptr(dx), dy=_ptr(dy), dgate=_ptr(dgate), dshift=_ptr(dshift), dscale=_ptr(dscale),
+                                dweight=_ptr(dw), dpost_weight=_ptr(dpw))
+        if dr is not None:
+            dr = _rows(dr)
+            g.dr, (g.dr_sample, g.dr_token) = _ptr(dr), _strides(dr)
+        if dz is not None:
+            dz = _rows(dz)
+            g.dz, (g.dz_sample, g.dz_token) = _ptr(dz), _strides(dz)
+        with torch.cuda.device(dev):
+            ws = None
+            if any(v is not None for v in (dgate, dshift, dscale, dw, dpw)):
+                # of this call alone: from the pool of the current stream, or of the graph being captured
+                ws = torch.empty(L.lib().lq_residual_norm_workspace_bytes(b, t, h), dtype=torch.uint8, device=dev)
+            L.check(L.lib().lq_residual_norm_bwd(C.byref(args), C.byref(g), _ptr(ws), 0 if ws is None else ws.numel(),
+                                                 _stream_ptr(dev)))
+        back = [None if v is None else v.to(like[1]).reshape(like[0])
+                for v, like in zip((dgate, dshift, dscale, dw, dpw), ctx.like)]
+        return dx, back[0], dy, back[1], back[2], back[3], back[4], None, None, None
+
+
+def modulated_zrmsnorm(x: torch.Tensor, weight: Optional[torch.Tensor], shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """`zrmsnorm(x, weight) * (1 + scale) + shift` (mmdit.rs:857-862 before a sub-block), one kernel each way; `weight`
+    `[h]` or None.  Gradients flow to every argument that asks for one, the norm's weight among them."""
+    return _ResidualNorm.apply(x, None, None, shift, scale, weight, None, False, 1.0, ZRMS_EPS)
+
+
+def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
+                        norm: str = "zrms", weight: Optional[torch.Tensor] = None,
+                        post_weight: Optional[torch.Tensor] = None, residual_scale: float = 1.0
+                        ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The end of one sub-block and the start of the next in one pass; returns `(r, z)`:
+
+        r = residual_scale * x + gate * y          (y * rsqrt(mean(y^2) + eps) * (1 + post_weight) with a post_weight)
+        z = norm(r) * (1 + weight) * (1 + scale) + shift
+
+    `x`, `y`: `[b, tokens, h]`, f32 or bf16 alike, rows contiguous, samples and tokens at any stride; `gate`, `shift`,
+    `scale`: `[b, 1, h]` or `[b, h]` (slices of one modulation tensor are read in place; expand over `b` to share a
+    vector); `weight`, `post_weight`: `[h]` or None; h <= 16384.  `norm`: "zrms" (mmdit.rs:282-330) or "layer".
+    Arithmetic is f32, `z` comes from the unrounded `r`, each output is rounded once; one kernel forward, one plus a
+    fixed-order sum over tokens backward, gradients to every tensor argument that asks for one."""
+    if norm not in ("zrms", "layer"):
+        raise ValueError(f"norm must be zrms or layer, got {norm!r}")
+    eps = ZRMS_EPS if norm == "zrms" else LN_EPS
+    return _ResidualNorm.apply(x, gate, y, shift, scale, weight, post_weight, norm == "layer", float(residual_scale), eps)
