@@ -279,6 +279,27 @@ int lq_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_
                   float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
                   float grad_scale, const int* skip_flag, void* stream);
 
+/* lq_adamw_step with one more factor on the gradients that is read on the device: g = grad_scale * *clip_coef *
+ * grads[i] (the coefficient of lq_grad_norm), so that clipping costs no pass over the gradients. */
+int lq_adamw_step_clipped(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n,
+                          float lr, float beta1, float beta2, float eps, float weight_decay, int64_t step,
+                          float grad_scale, const float* clip_coef, const int* skip_flag, void* stream);
+
+/* The 2-norm of `n_tensors` gradient tensors taken as one vector, and clipping by it (the reference clips nothing;
+ * it stands beside the finite check of crates/loractl-core/src/diffusion_trainer.rs:1708-1725, which it includes):
+ *     norm = |grad_scale| * sqrt(sum of g^2)         coef = min(1, max_norm / (norm + 1e-6))
+ *     outs[i] = grads[i] * (grad_scale * coef)       when outs is not NULL
+ * Host arrays of n_tensors: device addresses, element counts, element types (LQ_F32 or LQ_BF16, the same for a
+ * gradient and its output); tensors are contiguous and aligned to their element.  outs[i] == grads[i] scales in
+ * place; outputs overlap neither each other nor another tensor.  Sums are f64 in a fixed order.  `norm`, `coef` (f32)
+ * and `nonfinite` (int: 1 if some gradient is NaN or Inf, else 0) are device scalars and may be NULL; max_norm is read
+ * for coef and outs only.  The arrays are read before the call returns; nothing is copied to the device.
+ * `ws`: lq_grad_norm_workspace_bytes() bytes on the current device, 8-byte aligned. */
+size_t lq_grad_norm_workspace_bytes(int n_tensors);
+int lq_grad_norm(const void* const* grads, void* const* outs, const int64_t* counts, const int32_t* dtypes,
+                 int n_tensors, float grad_scale, float max_norm, float* norm, float* coef, int* nonfinite,
+                 void* ws, size_t ws_bytes, void* stream);
+
 /* ---- element-wise companions of the linears inside a DiT block ------------------ */
 
 /* crates/loractl-core/src/mmdit.rs:857-869: the block's `(scale + 1) * norm(x) + shift` prologues

@@ -11,7 +11,7 @@ from .adapters import LoraAdapters, LoraConfig, LoraSite, TargetSpec, build_adap
 from .linear import BaseLinear, QuantLinear, site
 from .fp8 import e4m3fn_lut, fp8_quantize, weight_from_fp8
 from .config import BackendKind, ComputeConfig, Precision, validate_b200
-from .optim import AdamW, DynamicLossScale, FlatAdapters, nonfinite_flag
+from .optim import AdamW, DynamicLossScale, FlatAdapters, clip_grad_norm, global_grad_norm, nonfinite_flag
 from .block_ckpt import checkpointed_step
 from . import block_ops, dp, export, loader
 from .export import export_adapters, import_adapters
@@ -23,6 +23,6 @@ __all__ = [
     "LoraDelta", "LoraLinear", "init_factors", "LoraAdapters", "LoraConfig", "LoraSite", "TargetSpec",
     "build_adapters", "BaseLinear", "QuantLinear", "site", "e4m3fn_lut", "fp8_quantize", "weight_from_fp8",
     "BackendKind", "ComputeConfig", "Precision", "validate_b200",
-    "AdamW", "DynamicLossScale", "FlatAdapters", "nonfinite_flag", "checkpointed_step", "block_ops", "dp",
+    "AdamW", "DynamicLossScale", "FlatAdapters", "clip_grad_norm", "global_grad_norm", "nonfinite_flag", "checkpointed_step", "block_ops", "dp",
     "export", "loader", "export_adapters", "import_adapters", "load_quant_module",
 ]

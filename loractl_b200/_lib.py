@@ -91,6 +91,9 @@ SIGNATURES = {
     "lq_weight_prepare_fp8_backward": (_I, [_P, _P]),
     "lq_grad_nonfinite_flag": (_I, [_P, _I64, _P, _P]),
     "lq_adamw_step": (_I, [_P, _P, _P, _P, _I64, _F, _F, _F, _F, _F, _I64, _F, _P, _P]),
+    "lq_adamw_step_clipped": (_I, [_P, _P, _P, _P, _I64, _F, _F, _F, _F, _F, _I64, _F, _P, _P, _P]),
+    "lq_grad_norm_workspace_bytes": (_SZ, [_I]),
+    "lq_grad_norm": (_I, [_P, _P, _P, _P, _I, _F, _F, _P, _P, _P, _P, _SZ, _P]),
     "lq_block_ops_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64]),
     "lq_ln_modulate_fwd": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, C.c_float, _P, _P, _P, _P]),
     "lq_ln_modulate_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, _P, C.c_size_t, _P]),

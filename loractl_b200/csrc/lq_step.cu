@@ -34,8 +34,10 @@ __global__ void __launch_bounds__(256) nonfinite_kernel(const float* __restrict_
 __global__ void __launch_bounds__(256) adamw_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                     float* __restrict__ m, float* __restrict__ v, int64_t n, float lr,
                                                     float b1, float b2, float eps, float wd, float bc1, float bc2,
-                                                    float grad_scale, const int* __restrict__ skip_flag) {
+                                                    float grad_scale, const float* __restrict__ clip_coef,
+                                                    const int* __restrict__ skip_flag) {
     if (skip_flag && *skip_flag != 0) return;  // non-finite gradients somewhere: skip the whole update
+    if (clip_coef) grad_scale *= *clip_coef;
     int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     int64_t stride = (int64_t)gridDim.x * blockDim.x;
     for (; i < n; i += stride) {
@@ -84,9 +86,9 @@ int lq_grad_nonfinite_flag(const float* grads, int64_t n, int* flag, void* strea
  * correction); `grad_scale` multiplies the gradients first (1/world for the data-parallel mean);
  * `skip_flag` (device int, may be NULL) non-zero turns the whole call into a no-op — the skip
  * branch of the dynamic loss scale, decided on the device. */
-int lq_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float lr,
-                  float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
-                  const int* skip_flag, void* stream) {
+int lq_adamw_step_clipped(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float lr,
+                          float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
+                          const float* clip_coef, const int* skip_flag, void* stream) {
     try {
         LQ_CHECK_ARG(n >= 0 && (n == 0 || (params && grads && exp_avg && exp_avg_sq)), "NULL argument");
         LQ_CHECK_ARG(step >= 1, "step is the 1-based update count");
@@ -98,7 +100,8 @@ int lq_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_
             if (blocks > 148 * 8) blocks = 148 * 8;
             LqProf prof(LQ_K_PREP, st);
             adamw_kernel<<<(unsigned)blocks, 256, 0, st>>>(params, grads, exp_avg, exp_avg_sq, n, lr, beta1, beta2,
-                                                          eps, weight_decay, bc1, bc2, grad_scale, skip_flag);
+                                                          eps, weight_decay, bc1, bc2, grad_scale, clip_coef,
+                                                          skip_flag);
             LQ_CUDA(cudaGetLastError());
         }
         lq_set_last_error("");
@@ -107,6 +110,13 @@ int lq_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_
         lq_set_last_error(e.what());
         return e.status;
     }
+}
+
+int lq_adamw_step(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, int64_t n, float lr,
+                  float beta1, float beta2, float eps, float weight_decay, int64_t step, float grad_scale,
+                  const int* skip_flag, void* stream) {
+    return lq_adamw_step_clipped(params, grads, exp_avg, exp_avg_sq, n, lr, beta1, beta2, eps, weight_decay, step,
+                                 grad_scale, nullptr, skip_flag, stream);
 }
 
 }  // extern "C"

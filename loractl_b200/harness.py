@@ -392,11 +392,13 @@ class Trainer:
     """One rank of the data-parallel LoRA trainer over a `BlockStack`."""
 
     def __init__(self, stack: BlockStack, lr: float = 1e-4, weight_decay: float = 1e-4, group=None,
-                 grad_checkpointing: bool = True, graphs: bool = False, reduce_every: int = 1):
+                 grad_checkpointing: bool = True, graphs: bool = False, reduce_every: int = 1,
+                 max_grad_norm: Optional[float] = None):
         """`graphs`: run the checkpointed sweep as CUDA graphs (`GraphedSweep`), captured at the first
         step of each batch shape.  `reduce_every`: blocks per gradient all-reduce of the reverse sweep
         (1 = one slice per block, started as soon as that block's backward is enqueued; the number of
-        blocks = one all-reduce of the whole bucket after the sweep)."""
+        blocks = one all-reduce of the whole bucket after the sweep).  `max_grad_norm`: clip the reduced, unscaled
+        gradients to this 2-norm over all adapters; `grad_norm` then holds the last step's norm (a device scalar)."""
         self.stack, self.lr, self.group = stack, lr, group
         self.optim = AdamW(stack.flat, weight_decay=weight_decay)
         self.scaler = DynamicLossScale(initial=1.0)  # bf16/f32 gradients do not need the f16 head-room
@@ -405,6 +407,9 @@ class Trainer:
             raise ValueError("graphs=True captures the block-checkpointed sweep: it needs grad_checkpointing")
         self.graphs = graphs
         self.reduce_every = max(int(reduce_every), 1)
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"max_grad_norm must be >= 0, got {max_grad_norm}")
+        self.max_grad_norm, self.grad_norm = max_grad_norm, None
         self._sweeps = {}
         self.steps_done = 0
 
@@ -462,11 +467,16 @@ class Trainer:
         scale = reducer.finish()
         torch.cuda.nvtx.range_pop()
         torch.cuda.nvtx.range_push("lq.optimizer")
-        nonfinite_flag(flat.grads, flat.flag)
+        clip_coef = None
+        if self.max_grad_norm is None:
+            nonfinite_flag(flat.grads, flat.flag)
+        else:  # the same pass over the bucket gives the flag, the norm and the factor
+            self.grad_norm, clip_coef = flat.clip_coefficient(self.max_grad_norm, scale / self.scaler.loss_scale)
         dp.reduce_flag(flat.flag, self.group)
         # the optimizer reads the flag on the device and skips itself; the host reads it only to
         # advance the loss-scale state (where the reference reads its |g| sum back)
-        self.optim.step(self.lr, grad_scale=scale / self.scaler.loss_scale, skip_flag=flat.flag)
+        self.optim.step(self.lr, grad_scale=scale / self.scaler.loss_scale, skip_flag=flat.flag,
+                        clip_coef=clip_coef)
         flat.refresh_mirrors()  # the factors changed: all bf16 operand mirrors in one batched launch
         torch.cuda.nvtx.range_pop()
         if self.graphs:

@@ -8,8 +8,10 @@ views, NCCL all-reduces the one buffer, the finite check is one kernel and AdamW
 """
 from __future__ import annotations
 
-from typing import List, Optional
+from array import array
+from typing import List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -102,6 +104,13 @@ class FlatAdapters:
         for d, key in stale:
             d._mirror_key = key
 
+    def clip_coefficient(self, max_norm: float, grad_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """One read of the gradient bucket: its 2-norm times `grad_scale`, the factor that brings that norm down to
+        `max_norm` (for `AdamW.step`), both as f32 device scalars, and the finite check into `flag`."""
+        norm, coef = torch.empty((2,), dtype=torch.float32, device=self.grads.device)
+        _grad_norm([self.grads], None, grad_scale, max_norm, norm, coef, self.flag)
+        return norm, coef
+
     def grad_views(self, index: int):
         """(dA view, dB view) of delta `index` — pass them to `lq_linear_bwd` as outputs."""
         a, b = self._params[2 * index], self._params[2 * index + 1]
@@ -139,6 +148,106 @@ def nonfinite_flag(grads: torch.Tensor, flag: torch.Tensor) -> None:
         L.check(L.lib().lq_grad_nonfinite_flag(grads.data_ptr(), grads.numel(), flag.data_ptr(), _stream(grads)))
 
 
+_CODES = {torch.float32: L.LQ_F32, torch.bfloat16: L.LQ_BF16}
+
+
+def _spans(tensors: Sequence[torch.Tensor]):
+    start = np.fromiter((t.data_ptr() for t in tensors), np.int64, len(tensors))
+    return start, start + np.fromiter((t.numel() * t.element_size() for t in tensors), np.int64, len(tensors))
+
+
+def _check_outputs(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor]) -> None:
+    """Outputs may be the gradients themselves, one for one, and share no byte with anything else."""
+    lo, hi = _spans(outs)
+    full = hi > lo
+    order = np.argsort(lo[full], kind="stable")
+    if (lo[full][order][1:] < hi[full][order][:-1]).any():
+        raise ValueError("the clipped tensors overlap one another (the same tensor twice?)")
+    if outs is grads:
+        return
+    glo, ghi = _spans(grads)
+    starts, ends = np.sort(glo[ghi > glo]), np.sort(ghi[ghi > glo])
+    # gradients that begin before an output ends, less those that end before it begins: its own alone may be one
+    met = np.searchsorted(starts, hi, side="left") - np.searchsorted(ends, lo, side="right")
+    if (met[full] > (lo == glo)[full]).any():
+        raise ValueError("an output overlaps a gradient tensor other than its own")
+
+
+def _grad_norm(grads: Sequence[torch.Tensor], outs: Optional[Sequence[torch.Tensor]], grad_scale: float, max_norm: float,
+               norm: Optional[torch.Tensor], coef: Optional[torch.Tensor], flag: Optional[torch.Tensor]) -> None:
+    dev, n = grads[0].device, len(grads)
+    table = array("q", [t.data_ptr() for t in grads])
+    table.extend([t.data_ptr() for t in outs] if outs is not None else ())
+    counts = array("q", [t.numel() for t in grads])
+    kinds = array("i", [_CODES[t.dtype] for t in grads])
+    at = table.buffer_info()[0]
+    with torch.cuda.device(dev):
+        lib = L.lib()
+        ws = torch.empty(lib.lq_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        L.check(lib.lq_grad_norm(at, at + 8 * n if outs is not None else None, counts.buffer_info()[0], kinds.buffer_info()[0], n,
+                                 grad_scale, max_norm, norm.data_ptr() if norm is not None else None,
+                                 coef.data_ptr() if coef is not None else None, flag.data_ptr() if flag is not None else None,
+                                 ws.data_ptr(), ws.numel(), _stream(ws)))
+
+
+def _gradients(grads) -> List[torch.Tensor]:
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise ValueError("no gradient tensors")
+    if not grads[0].is_cuda:
+        raise RuntimeError("gradients must live on a CUDA device: the b200 backend has no CPU path")
+    index = grads[0].get_device()
+    for t in grads:
+        if t.get_device() != index:
+            raise RuntimeError(f"gradients must live on one CUDA device, got {grads[0].device} and {t.device}")
+        if t.dtype not in _CODES:
+            raise TypeError(f"unsupported gradient dtype {t.dtype}: f32 or bf16")
+    return grads
+
+
+def global_grad_norm(grads: Sequence[torch.Tensor], grad_scale: float = 1.0) -> torch.Tensor:
+    """The 2-norm of all `grads` (f32 and bf16 tensors of any shape on one device) taken as one vector, times
+    `|grad_scale|`, as an f32 device scalar: two launches for up to 128 tensors, no host synchronisation.  Squares and
+    sums are 64-bit; the norm is NaN or Inf exactly when some gradient is."""
+    grads = [t if t.is_contiguous() else t.contiguous() for t in _gradients(grads)]
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _grad_norm(grads, None, float(grad_scale), 0.0, norm, None, None)
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
+                   grad_scale: float = 1.0) -> torch.Tensor:
+    """Scales every gradient by `grad_scale * min(1, max_norm / (norm + 1e-6))`, where `norm` is their
+    `global_grad_norm` (with `grad_scale`), and returns that norm: two launches for up to 128 tensors, no host
+    synchronisation.  `grads` are scaled in place (they must be contiguous and must not overlap), or written to `out`:
+    contiguous tensors of the same shapes and types that overlap nothing but their own gradient.  A norm that is not
+    finite gives what the formula gives: zeros and NaN for Inf, NaN for NaN."""
+    grads = _gradients(grads)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    if out is None:
+        outs = grads
+        if not all(t.is_contiguous() for t in grads):
+            raise ValueError("gradients that are clipped in place must be contiguous")
+    else:
+        outs = _gradients(out)
+        if len(outs) != len(grads) or any(o.shape != t.shape or o.dtype != t.dtype for o, t in zip(outs, grads)):
+            raise ValueError("out must hold one tensor of the same shape and type for each gradient")
+        if outs[0].get_device() != grads[0].get_device():
+            raise RuntimeError(f"gradients must live on one CUDA device, got {grads[0].device} and {outs[0].device}")
+        if not all(t.is_contiguous() for t in outs):
+            raise ValueError("out tensors must be contiguous")
+    _check_outputs(grads, outs)
+    if outs is not grads:
+        grads = [t if t.is_contiguous() else t.contiguous() for t in grads]
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _grad_norm(grads, outs, float(grad_scale), float(max_norm), norm, None, None)
+    for t in outs:
+        torch.autograd.graph.increment_version(t)
+    return norm
+
+
 class AdamW:
     """burn `AdamWConfig::new().with_weight_decay(wd)` (diffusion_trainer.rs:1564-1566) over a
     `FlatAdapters`: defaults beta1 0.9, beta2 0.999, epsilon 1e-5 (burn-optim 0.21), decoupled
@@ -150,15 +259,17 @@ class AdamW:
         self.steps = 0
 
     def step(self, lr: float, grad_scale: float = 1.0, skip_flag: Optional[torch.Tensor] = None,
-             count: bool = True) -> None:
+             count: bool = True, clip_coef: Optional[torch.Tensor] = None) -> None:
+        """`clip_coef`: a device scalar that multiplies the gradients too (`FlatAdapters.clip_coefficient`)."""
         f = self.flat
         if not f.params.is_cuda:
             raise RuntimeError("the b200 backend has no CPU path")
         if count:
             self.steps += 1
         with torch.cuda.device(f.params.device):
-            L.check(L.lib().lq_adamw_step(
+            L.check(L.lib().lq_adamw_step_clipped(
                 f.params.data_ptr(), f.grads.data_ptr(), f.exp_avg.data_ptr(), f.exp_avg_sq.data_ptr(), f.numel,
                 float(lr), self.beta1, self.beta2, self.eps, float(self.weight_decay), max(self.steps, 1),
-                float(grad_scale), skip_flag.data_ptr() if skip_flag is not None else None, _stream(f.params)))
+                float(grad_scale), clip_coef.data_ptr() if clip_coef is not None else None,
+                skip_flag.data_ptr() if skip_flag is not None else None, _stream(f.params)))
         f.param_epoch[0] += 1  # the kernel wrote through raw pointers: bf16 operand mirrors are stale
