@@ -261,6 +261,43 @@ int lq_linear_fwd_grouped(const lq_group_site* sites, int n_sites, const void* X
  * step loop allocation-free.  No counterpart in the reference. */
 int lq_weight_prepare_fp8_backward(const lq_weight_t* w, void* stream);
 
+/* ---- microscaled 4-bit floating point (MXFP4) -------------------------------------- */
+
+/* A second 4-bit format beside LQ_INT4 (crates/loractl-core/src/quant.rs:61-67): e2m1 elements (0, .5, 1, 1.5, 2, 3, 4, 6
+ * and their negatives), one e8m0 scale (a power of two) per 32 elements along a row, no zero point.  The tensor cores
+ * multiply it as it is stored (tcgen05 kind::mxf4), so a product needs no dequantised copy of either operand; in
+ * exchange activations are quantised too.
+ *
+ *   scale  2^e, e = floor(log2(max |v| of the block)) - 2, in [-127, 125]; zeros: -127; a block with an Inf or a NaN gets the
+ *          NaN scale and stands for 32 NaNs
+ *   code   v / 2^e to nearest, ties to the even code, saturated at 6 (the division is exact)
+ *
+ * A tensor is [rows, k] with k a multiple of 32: `codes`, rows * k / 2 bytes, row-major, two elements a byte, the even one
+ * in the low nibble; `scales`, lq_mx4_scale_bytes(rows, k) bytes: tiles of 128 rows x 4 scales (512 bytes; row r, scale s at
+ * (r % 32) * 16 + (r / 32 % 4) * 4 + s), tile (r / 128, s / 4) at (r / 128) * k_tiles + s / 4, k_tiles = 2 * ceil(k / 256).
+ * Both 16-byte aligned, caller-owned. */
+size_t lq_mx4_scale_bytes(int64_t rows, int64_t k);
+
+/* x: [rows, k], `dtype` LQ_F32 or LQ_BF16, `ld` elements between rows. */
+int lq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, void* codes, void* scales, void* stream);
+
+/* out: [rows, k] contiguous, 16-byte aligned; exact in f32 and in bf16. */
+int lq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, void* out, int out_dtype, void* stream);
+
+/* Y[n, m] = X[n, k] . W[m, k]^T + bias[m] (f32, may be NULL), both operands microscaled, f32 accumulation, y contiguous
+ * LQ_F32 or LQ_BF16 (rounded once).  `ws`: lq_mx4_matmul_workspace_bytes() bytes on the current device (may be 0),
+ * 16-byte aligned; calls that can overlap need one each. */
+size_t lq_mx4_matmul_workspace_bytes(int64_t n, int64_t m, int64_t k);
+int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales,
+                  int64_t m, int64_t k, const float* bias, void* y, int y_dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* dX[n, k] = dY[n, m] . W[m, k]: the gradient through the frozen weight (that of crates/loractl-core/src/
+ * quant.rs:221-235), with the quantisation of x taken as the identity.  dy, dx contiguous, 16-byte aligned, LQ_BF16
+ * (W is exact in bf16) or LQ_F32 (f32 arithmetic).  `ws`: lq_mx4_matmul_dx_workspace_bytes() bytes, 256-byte aligned. */
+size_t lq_mx4_matmul_dx_workspace_bytes(int64_t n, int64_t m, int64_t k, int dtype);
+int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
+                     int64_t k, void* dx, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- step glue on the flat LoRA buffers ---------------------------------------- */
 
 /* crates/loractl-core/src/diffusion_trainer.rs:1708-1725 (the finite check over every adapter

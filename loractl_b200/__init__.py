@@ -9,6 +9,7 @@ from .quant import (QUANT_BLOCK, Quant, QuantWeight, check_device_status, dequan
 from .lora import LoraDelta, LoraLinear, init_factors
 from .adapters import LoraAdapters, LoraConfig, LoraSite, TargetSpec, build_adapters
 from .linear import BaseLinear, QuantLinear, site
+from .mx4 import Mx4Linear, Mx4Tensor, mx4_matmul_dx, mx4_matmul_t, mx4_quantize
 from .fp8 import e4m3fn_lut, fp8_quantize, weight_from_fp8
 from .config import BackendKind, ComputeConfig, Precision, validate_b200
 from .optim import AdamW, DynamicLossScale, FlatAdapters, clip_grad_norm, global_grad_norm, nonfinite_flag
@@ -22,6 +23,7 @@ __all__ = [
     "quant_value", "quantize_linear_weight", "quantize_linear_weight_chunked",
     "LoraDelta", "LoraLinear", "init_factors", "LoraAdapters", "LoraConfig", "LoraSite", "TargetSpec",
     "build_adapters", "BaseLinear", "QuantLinear", "site", "e4m3fn_lut", "fp8_quantize", "weight_from_fp8",
+    "Mx4Linear", "Mx4Tensor", "mx4_matmul_dx", "mx4_matmul_t", "mx4_quantize",
     "BackendKind", "ComputeConfig", "Precision", "validate_b200",
     "AdamW", "DynamicLossScale", "FlatAdapters", "clip_grad_norm", "global_grad_norm", "nonfinite_flag", "checkpointed_step", "block_ops", "dp",
     "export", "loader", "export_adapters", "import_adapters", "load_quant_module",

@@ -89,6 +89,13 @@ SIGNATURES = {
     "lq_linear_grouped_workspace_bytes": (_SZ, [C.POINTER(GroupSite), _I, _I64, _I]),
     "lq_linear_fwd_grouped": (_I, [C.POINTER(GroupSite), _I, _P, _I64, _I, _P, _SZ, _P]),
     "lq_weight_prepare_fp8_backward": (_I, [_P, _P]),
+    "lq_mx4_scale_bytes": (_SZ, [_I64, _I64]),
+    "lq_mx4_quantize": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
+    "lq_mx4_dequantize": (_I, [_P, _P, _I64, _I64, _P, _I, _P]),
+    "lq_mx4_matmul_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "lq_mx4_matmul": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I, _P, _SZ, _P]),
+    "lq_mx4_matmul_dx_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
+    "lq_mx4_matmul_dx": (_I, [_P, _I, _I64, _P, _P, _I64, _I64, _P, _P, _SZ, _P]),
     "lq_grad_nonfinite_flag": (_I, [_P, _I64, _P, _P]),
     "lq_adamw_step": (_I, [_P, _P, _P, _P, _I64, _F, _F, _F, _F, _F, _I64, _F, _P, _P]),
     "lq_adamw_step_clipped": (_I, [_P, _P, _P, _P, _I64, _F, _F, _F, _F, _F, _I64, _F, _P, _P, _P]),

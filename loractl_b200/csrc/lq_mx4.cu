@@ -1,0 +1,613 @@
+// Microscaled 4-bit floating point (MXFP4: e2m1 elements, one e8m0 scale per 32 along a row): quantisation,
+// the product of two such tensors on the block-scaled tensor cores, and the backward through a frozen weight.
+//
+// A block of 32 values v has the scale 2^e, e = floor(log2(max |v|)) - 2 (2 is e2m1's largest exponent),
+// clamped to [-127, 125], and the elements are v / 2^e rounded to nearest even among 0, .5, 1, 1.5, 2, 3, 4, 6 and
+// saturated at 6.  Scaling by a power of two is exact, so an element is rounded once.  A block of zeros has e = -127;
+// a block with an Inf or a NaN has the NaN scale (0xFF) and stands for 32 NaNs.
+//
+// Storage of [rows, k], k a multiple of 32:
+//   codes   row-major, two elements a byte, the even one in the low nibble: what a TMA tile and the MMA read
+//   scales  tiles of 128 rows x 4 scales (128 elements of k), 512 bytes each: row r, scale s at byte
+//           (r % 32) * 16 + (r / 32) * 4 + s, which is what one 32-lane x 128-bit copy to tensor memory wants;
+//           tile (rt, kt) at (rt * k_tiles + kt) * 512 with k_tiles even (a k-block of the product is 256
+//           elements = two tiles) and, above 128 rows, an even number of row tiles (its pair of SMs loads 256 rows).
+//           Scales of padding are 0 (2^-127, never NaN: they meet zero codes).
+//
+// The product Y[n, m] = sum_k X[n, k] W[m, k] (+ bias) multiplies codes and scales where they lie: nothing is
+// dequantised (tcgen05.mma kind::mxf4.block_scale, f32 accumulators).
+#include <algorithm>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "lq_internal.cuh"
+#include "lq_prof.cuh"
+#include "lq_tc.cuh"
+#include "lq_umma.cuh"
+
+namespace {
+
+using namespace umma;
+
+constexpr int kTile = 512;  // bytes of one scale tile
+
+__host__ __device__ inline int64_t row_tiles(int64_t rows) { return rows <= 128 ? 1 : 2 * ((rows + 255) / 256); }
+__host__ __device__ inline int64_t k_tiles(int64_t k) { return 2 * ((k + 255) / 256); }
+
+// ---- quantise / dequantise ------------------------------------------------------------------------
+
+// Eight f32 to eight e2m1 codes, element i in nibble i.
+__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8]) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+__device__ __forceinline__ void unpack_e2m1(uint32_t w, float (&v)[8]) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(w));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*(const __half2*)&h[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    const uint32_t bits = byte == 0 ? 0x00400000u : (byte == 255 ? 0x7FC00000u : byte << 23);
+    return __uint_as_float(bits);
+}
+
+__device__ __forceinline__ void load8(const float* p, bool vec, float (&v)[8]) {
+    if (vec) {
+        const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[i];
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vec, float (&v)[8]) {
+    if (vec) {
+        const uint4 u = *(const uint4*)p;
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
+    }
+}
+
+// One warp per (row, 256 elements): a lane holds 8 elements, 4 lanes a block, so that loads and code stores are
+// whole lines.  HBM-bound; the padding rows of the last scale tile are items too and get zero scales.
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t k, int64_t ld, int vec,
+                                                           int64_t pad_rows, uint32_t* __restrict__ codes,
+                                                           uint8_t* __restrict__ scales) {
+    const int64_t kb = (k + 255) / 256;
+    const int64_t items = pad_rows * kb;
+    const int lane = threadIdx.x & 31;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
+        const int64_t row = it / kb, b = it - row * kb;
+        const int64_t col = b * 256 + lane * 8;
+        const bool in = row < rows && col < k;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (in) load8(x + row * ld + col, vec, v);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the exponent field f stands for 2^(f - 127): e = f - 129, stored as e + 127; subnormals fall to the lowest
+        uint32_t byte = (uint32_t)max((int)(top >> 23) - 2, 0);
+        const bool bad = top >= 0x7F800000u;
+        if (bad) byte = 255;
+        const float inv = __uint_as_float((254u - (bad ? 252u : byte)) << 23);
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= inv;
+        if (!bad) w = pack_e2m1(v);
+        if (in) codes[(row * k + col) >> 3] = w;
+        // the four scales of 128 elements as one word, from the lanes 0, 4, 8, 12 of each half-warp
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xffffffffu, byte, (lane & 16) + 4 * i) << (8 * i);
+        if ((lane & 15) == 0) {
+            const int64_t tile = (row >> 7) * (2 * kb) + 2 * b + (lane >> 4);
+            const int r = (int)(row & 127);
+            *(uint32_t*)(scales + tile * kTile + (r & 31) * 16 + (r >> 5) * 4) = word;
+        }
+    }
+}
+
+// out[row, col .. col + 7] = code * scale, 8 elements a thread; exact in f32 and in bf16.
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                             int64_t rows, int64_t k, T* __restrict__ out) {
+    const int64_t n = rows * (k / 8), kt = k_tiles(k);
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = i / (k / 8), col = (i - row * (k / 8)) * 8;
+        const int r = (int)(row & 127);
+        const int64_t tile = (row >> 7) * kt + (col >> 7);
+        const float s = scale_value(scales[tile * kTile + (r & 31) * 16 + (r >> 5) * 4 + ((col >> 5) & 3)]);
+        float v[8];
+        unpack_e2m1(codes[i], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= s;
+        if (sizeof(T) == 4) {
+            ((float4*)out)[2 * i] = make_float4(v[0], v[1], v[2], v[3]);
+            ((float4*)out)[2 * i + 1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                w[e] = *(const uint32_t*)&h;
+            }
+            ((uint4*)out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// ---- the product ------------------------------------------------------------------------------------
+
+// tcgen05.mma kind::mxf4, block scale of 32 elements: K = 64 per instruction, two scales per row.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// One scale tile (512 bytes of shared memory, 32 rows of 16) to 4 columns of all four lane quarters.
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Shared-memory descriptor of a scale tile: no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// Instruction descriptor of kind::mxf4: [4,6) which scale pair of B's column word, [7,10) and [10,12) e2m1 = 1,
+// [17,23) N >> 3, [23] scales are e8m0, [24,29) M >> 4, [29,31) which scale pair of A's.
+__host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t M, uint32_t N, uint32_t pair) {
+    return (2 * pair << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24) | (2 * pair << 29);
+}
+
+struct ProductParams {
+    const uint8_t* w_scales;
+    const uint8_t* x_scales;
+    int m, n, kb;             // d_out, tokens, k-blocks of 256
+    int w_tiles, x_tiles;     // 128 weight rows; BN tokens, which is 128 (a whole scale tile) when there are several
+    int splits;
+    float* part;              // [splits][n][m] f32 when splits > 1
+    const float* bias;
+    void* y;
+    int y_f32;
+    int* status;
+};
+
+constexpr int kThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+
+template <int BN>
+struct CfgT {
+    static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN * 128, S_BYTES = 2 * kTile;
+    static constexpr uint32_t STAGE = A_BYTES + B_BYTES + 2 * S_BYTES;
+    static constexpr int STAGES = (200 * 1024) / STAGE < 10 ? (200 * 1024) / STAGE : 10;
+    static constexpr uint32_t TMEM = 512;
+    static constexpr uint32_t SCALE_COL = 2 * BN;  // behind the two accumulators: 16 columns per stage
+    static_assert(2 * BN + 16 * STAGES <= 512, "tensor memory");
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 256;
+};
+
+// Few tokens (or few weight rows): the weight is the 128-row operand and BN tokens are the columns, so that a
+// narrow batch wastes no tensor rows, and the reduction is cut into `splits` ranges so that every SM streams
+// weights.  D's lane is a weight row, so a store of one token writes 32 consecutive outputs.
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_constant__ CUtensorMap tmW,
+                                                                 const __grid_constant__ CUtensorMap tmX, ProductParams p) {
+    using C = CfgT<BN>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem_a = smem;
+    uint8_t* smem_b = smem_a + (size_t)STAGES * C::A_BYTES;
+    uint8_t* smem_s = smem_b + (size_t)STAGES * C::B_BYTES;  // per stage: W's two scale tiles, then X's
+    uint64_t* bars = (uint64_t*)(smem_s + (size_t)STAGES * 2 * C::S_BYTES);
+    uint64_t* full = bars;
+    uint64_t* empty = bars + STAGES;
+    uint64_t* tfull = bars + 2 * STAGES;
+    uint64_t* tempty = bars + 2 * STAGES + 2;
+    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 4);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(smem_u32(&tfull[a]), 1);
+            mbar_init(smem_u32(&tempty[a]), 128);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmW);
+        prefetch_tmap(&tmX);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), C::TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int items = p.w_tiles * p.x_tiles * p.splits;
+    auto range = [&](int item, int& wt, int& xt, int& z, int& k0, int& k1) {
+        z = item % p.splits;
+        wt = item / p.splits % p.w_tiles;
+        xt = item / p.splits / p.w_tiles;
+        k0 = (int)((long long)p.kb * z / p.splits);
+        k1 = (int)((long long)p.kb * (z + 1) / p.splits);
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            const int kt = 2 * p.kb;
+            for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+                int wt, xt, z, k0, k1;
+                range(item, wt, xt, z, k0, k1);
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 71)) { ok = false; break; }
+                    const uint32_t bar = smem_u32(&full[s]);
+                    uint8_t* sc = smem_s + (size_t)s * 2 * C::S_BYTES;
+                    mbar_expect_tx(bar, C::STAGE);
+                    tma_load_2d(smem_u32(smem_a + (size_t)s * C::A_BYTES), &tmW, bar, kb * 128, wt * 128);
+                    tma_load_2d(smem_u32(smem_b + (size_t)s * C::B_BYTES), &tmX, bar, kb * 128, xt * BN);
+                    bulk_load(smem_u32(sc), p.w_scales + ((int64_t)wt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
+                    bulk_load(smem_u32(sc + C::S_BYTES), p.x_scales + ((int64_t)xt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok)
+                for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the block ends
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t d_hi = desc_hi(1024);
+            int s = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+                int wt, xt, z, k0, k1;
+                range(item, wt, xt, z, k0, k1);
+                if (!mbar_wait(smem_u32(&tempty[acc]), acc_phase ^ 1u, abort_flag, p.status, 72)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(acc * BN);
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 73)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t sc = smem_u32(smem_s + (size_t)s * 2 * C::S_BYTES);
+                    const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 16, sfb = sfa + 8;
+                    cp_scales(sfa, scale_desc(sc));
+                    cp_scales(sfa + 4, scale_desc(sc + kTile));
+                    cp_scales(sfb, scale_desc(sc + 2 * kTile));
+                    cp_scales(sfb + 4, scale_desc(sc + 3 * kTile));
+                    const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
+                    const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)  // 64 elements = 32 bytes; scale pair k & 1 of tile k / 2
+                        mma_mxf4(d, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi), idesc_mxf4(128, BN, k & 1),
+                                 sfa + 4 * (k >> 1), sfb + 4 * (k >> 1), (kb > k0 || k > 0) ? 1u : 0u);
+                    mma_commit(smem_u32(&empty[s]));
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                mma_commit(smem_u32(&tfull[acc]));
+                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            int wt, xt, z, k0, k1;
+            range(item, wt, xt, z, k0, k1);
+            if (!mbar_wait(smem_u32(&tfull[acc]), acc_phase, abort_flag, p.status, 74)) break;
+            tc_fence_after();
+            const int row = wt * 128 + quarter * 32 + lane;
+            const float bias = (p.splits == 1 && p.bias && row < p.m) ? p.bias[row] : 0.f;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                uint32_t r[16];
+                tmem_ld_x16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN + c), r);
+                tmem_ld_wait();
+                if (row < p.m)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int tok = xt * BN + c + j;
+                        if (tok >= p.n) break;
+                        const float v = __uint_as_float(r[j]);
+                        const int64_t o = (int64_t)tok * p.m + row;
+                        if (p.splits > 1) p.part[(int64_t)z * p.n * p.m + o] = v;
+                        else if (p.y_f32) ((float*)p.y)[o] = v + bias;
+                        else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(v + bias);
+                    }
+            }
+            tc_fence_before();
+            mbar_arrive(smem_u32(&tempty[acc]));
+            if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM);
+    }
+}
+
+// y = sum of the splits in order + bias.
+__global__ void __launch_bounds__(256) mx4_join_kernel(ProductParams p) {
+    const int64_t n = (int64_t)p.n * p.m;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        float v = 0.f;
+        for (int z = 0; z < p.splits; ++z) v += p.part[z * n + i];
+        if (p.bias) v += p.bias[i % p.m];
+        if (p.y_f32) ((float*)p.y)[i] = v;
+        else ((__nv_bfloat16*)p.y)[i] = __float2bfloat16(v);
+    }
+}
+
+// [n, m] bf16 with a row stride of `ld` elements, for the tensor maps' 16-byte rows.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __nv_bfloat16* __restrict__ in, int64_t n, int64_t m, int64_t ld,
+                                                       __nv_bfloat16* __restrict__ out) {
+    const int64_t total = n * ld;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / ld, c = i - r * ld;
+        out[i] = c < m ? in[r * m + c] : __float2bfloat16(0.f);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+template <typename F>
+int guarded_call(F&& f) {
+    try {
+        f();
+        lq_set_last_error("");
+        return LQ_OK;
+    } catch (const LqError& e) {
+        lq_set_last_error(e.what());
+        return e.status;
+    } catch (const std::exception& e) {
+        lq_set_last_error(e.what());
+        return LQ_ERR_INVALID;
+    }
+}
+
+int current_device() {
+    int dev = 0;
+    LQ_CUDA(cudaGetDevice(&dev));
+    return dev;
+}
+inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+inline unsigned grid_of(int64_t items, int sms, int per_sm) {
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, (int64_t)sms * per_sm));
+}
+
+void check_dims(int64_t rows, int64_t k) {
+    LQ_CHECK_ARG(rows >= 0 && rows < (int64_t)1 << 31, "row count out of range");
+    LQ_CHECK_ARG(k >= 32 && k % 32 == 0 && k < (int64_t)1 << 31, "the block axis must be a positive multiple of 32");
+}
+void check_tensor(const void* codes, const void* scales) {
+    LQ_CHECK_ARG(codes && scales, "NULL argument");
+    LQ_CHECK_ARG(al16(codes) && al16(scales), "codes and scales must be 16-byte aligned");
+}
+
+int bn_of(int64_t n) { return n <= 16 ? 16 : (n <= 32 ? 32 : (n <= 64 ? 64 : 128)); }
+
+// Ranges of the reduction: as many as fill the SMs when the tiles alone do not, each of at least two k-blocks.
+int splits_of(int64_t tiles, int64_t kb, int sms) {
+    if (tiles >= sms) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / tiles, kb / 2), 16));
+}
+
+size_t product_ws(int64_t n, int64_t m, int64_t k, int sms) {
+    const int bn = bn_of(n);
+    const int64_t tiles = ((m + 127) / 128) * ((n + bn - 1) / bn);
+    const int s = splits_of(tiles, (k + 255) / 256, sms);
+    return s > 1 ? (size_t)s * n * m * sizeof(float) : 0;
+}
+
+template <int BN>
+void launch_stream(ProductParams p, const void* w_codes, const void* x_codes, int64_t k, int sms, cudaStream_t st) {
+    using C = CfgT<BN>;
+    const CUtensorMap tw = lq_tc_make_map_u8(w_codes, k / 2, p.m, k / 2, 128);
+    const CUtensorMap tx = lq_tc_make_map_u8(x_codes, k / 2, p.n, k / 2, BN);
+    LQ_CUDA(cudaFuncSetAttribute(mx4_stream_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    const int64_t items = (int64_t)p.w_tiles * p.x_tiles * p.splits;
+    LQ_CHECK_ARG(items < (int64_t)1 << 31, "too many tiles");
+    {
+        LqProf prof(LQ_K_GEMM_MAIN, st);
+        mx4_stream_kernel<BN><<<grid_of(items, sms, 1), kThreads, C::SMEM, st>>>(tw, tx, p);
+        LQ_CUDA(cudaGetLastError());
+    }
+    if (p.splits > 1) {
+        LqProf prof(LQ_K_REDUCE, st);
+        mx4_join_kernel<<<grid_of(((int64_t)p.n * p.m + 255) / 256, sms, 8), 256, 0, st>>>(p);
+        LQ_CUDA(cudaGetLastError());
+    }
+}
+
+size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+}  // namespace
+
+extern "C" {
+
+size_t lq_mx4_scale_bytes(int64_t rows, int64_t k) {
+    if (rows < 1 || k < 32) return 0;
+    return (size_t)row_tiles(rows) * k_tiles(k) * kTile;
+}
+
+int lq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, void* codes, void* scales, void* stream) {
+    return guarded_call([&] {
+        LQ_CHECK_ARG(dtype == LQ_F32 || dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
+        check_dims(rows, k);
+        if (rows == 0) return;
+        LQ_CHECK_ARG(x != nullptr, "NULL argument");
+        check_tensor(codes, scales);
+        LQ_CHECK_ARG(ld >= k || rows == 1, "rows overlap: the row stride is below their length");
+        cudaStream_t st = (cudaStream_t)stream;
+        const int64_t pad = row_tiles(rows) * 128;
+        const unsigned grid = grid_of((pad * ((k + 255) / 256) + 7) / 8, lq_tc_sm_count(current_device()), 16);
+        const int vec = al16(x) && (ld * (dtype == LQ_F32 ? 4 : 2)) % 16 == 0;
+        LqProf prof(LQ_K_QUANT, st);
+        if (dtype == LQ_F32)
+            mx4_quantize_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, k, ld, vec, pad, (uint32_t*)codes, (uint8_t*)scales);
+        else
+            mx4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, k, ld, vec, pad, (uint32_t*)codes,
+                                                                     (uint8_t*)scales);
+        LQ_CUDA(cudaGetLastError());
+    });
+}
+
+int lq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, void* out, int out_dtype, void* stream) {
+    return guarded_call([&] {
+        LQ_CHECK_ARG(out_dtype == LQ_F32 || out_dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
+        check_dims(rows, k);
+        if (rows == 0) return;
+        check_tensor(codes, scales);
+        LQ_CHECK_ARG(out && al16(out), "the output must be 16-byte aligned");
+        cudaStream_t st = (cudaStream_t)stream;
+        const unsigned grid = grid_of((rows * (k / 8) + 255) / 256, lq_tc_sm_count(current_device()), 16);
+        LqProf prof(LQ_K_DEQUANT, st);
+        if (out_dtype == LQ_F32)
+            mx4_dequantize_kernel<float><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, k, (float*)out);
+        else
+            mx4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, k,
+                                                                       (__nv_bfloat16*)out);
+        LQ_CUDA(cudaGetLastError());
+    });
+}
+
+size_t lq_mx4_matmul_workspace_bytes(int64_t n, int64_t m, int64_t k) {
+    if (n < 1 || m < 1 || k < 32) return 0;
+    size_t b = 0;
+    if (guarded_call([&] { b = product_ws(n, m, k, lq_tc_sm_count(current_device())); }) != LQ_OK) return 0;
+    return b;
+}
+
+int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
+                  int64_t k, const float* bias, void* y, int y_dtype, void* ws, size_t ws_bytes, void* stream) {
+    return guarded_call([&] {
+        LQ_CHECK_ARG(y_dtype == LQ_F32 || y_dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
+        check_dims(n, k);
+        check_dims(m, k);
+        if (n == 0 || m == 0) return;
+        check_tensor(x_codes, x_scales);
+        check_tensor(w_codes, w_scales);
+        LQ_CHECK_ARG(y != nullptr, "NULL argument");
+        cudaStream_t st = (cudaStream_t)stream;
+        const int dev = current_device(), sms = lq_tc_sm_count(dev);
+        if (ws_bytes < product_ws(n, m, k, sms) || (product_ws(n, m, k, sms) && !ws))
+            throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled product");
+        LQ_CHECK_ARG(al16(ws), "the workspace must be 16-byte aligned");
+        const int bn = bn_of(n);
+        ProductParams p;
+        p.w_scales = (const uint8_t*)w_scales;
+        p.x_scales = (const uint8_t*)x_scales;
+        p.m = (int)m;
+        p.n = (int)n;
+        p.kb = (int)((k + 255) / 256);
+        p.w_tiles = (int)((m + 127) / 128);
+        p.x_tiles = (int)((n + bn - 1) / bn);
+        p.splits = splits_of((int64_t)p.w_tiles * p.x_tiles, p.kb, sms);
+        p.part = (float*)ws;
+        p.bias = bias;
+        p.y = y;
+        p.y_f32 = y_dtype == LQ_F32;
+        p.status = lq_tc_status_word(dev);
+        if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, sms, st);
+        else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, sms, st);
+        else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, sms, st);
+        else launch_stream<128>(p, w_codes, x_codes, k, sms, st);
+    });
+}
+
+size_t lq_mx4_matmul_dx_workspace_bytes(int64_t n, int64_t m, int64_t k, int dtype) {
+    if (n < 1 || m < 1 || k < 32) return 0;
+    const size_t w = (size_t)m * k * (dtype == LQ_F32 ? 4 : 2);
+    return al256(w) + (dtype == LQ_BF16 && m % 8 ? (size_t)n * ((m + 7) / 8 * 8) * 2 : 0);
+}
+
+int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k, void* dx,
+                     void* ws, size_t ws_bytes, void* stream) {
+    return guarded_call([&] {
+        LQ_CHECK_ARG(dtype == LQ_F32 || dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
+        check_dims(n, k);
+        check_dims(m, k);
+        if (n == 0) return;
+        LQ_CHECK_ARG(dx && al16(dx), "dx must be 16-byte aligned");
+        cudaStream_t st = (cudaStream_t)stream;
+        if (m == 0) {
+            LQ_CUDA(cudaMemsetAsync(dx, 0, (size_t)n * k * (dtype == LQ_F32 ? 4 : 2), st));
+            return;
+        }
+        LQ_CHECK_ARG(dy != nullptr, "NULL argument");
+        check_tensor(w_codes, w_scales);
+        LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
+        if (ws_bytes < lq_mx4_matmul_dx_workspace_bytes(n, m, k, dtype))
+            throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled backward");
+        if (lq_mx4_dequantize(w_codes, w_scales, m, k, ws, dtype, stream) != LQ_OK) throw LqError(LQ_ERR_CUDA, lq_last_error());
+        if (dtype == LQ_F32) {
+            LqSimtArgs a{};
+            a.A = dy, a.a_dtype = LQ_F32, a.sa_i = m, a.sa_k = 1;
+            a.b_mode = 0, a.Bp = ws, a.b_dtype = LQ_F32, a.sb_k = k, a.sb_j = 1;
+            a.C = dx, a.c_dtype = LQ_F32, a.ldc = k;
+            a.I = n, a.J = k, a.Kred = m, a.alpha = 1.f, a.beta = 0;
+            lq_launch_simt_gemm(a, st);
+            return;
+        }
+        const void* src = dy;
+        const int64_t ld = (m + 7) / 8 * 8;
+        if (ld != m || !al16(dy)) {
+            LQ_CHECK_ARG(ld != m, "dy must be 16-byte aligned");
+            __nv_bfloat16* padded = (__nv_bfloat16*)((uint8_t*)ws + al256((size_t)m * k * 2));
+            LqProf prof(LQ_K_PREP, st);
+            pad_rows_kernel<<<grid_of((n * ld + 255) / 256, lq_tc_sm_count(current_device()), 16), 256, 0, st>>>(
+                (const __nv_bfloat16*)dy, n, m, ld, padded);
+            LQ_CUDA(cudaGetLastError());
+            src = padded;
+        }
+        lq_tc_gemm_nn(src, ld, ws, k, dx, n, k, m, st);
+    });
+}
+
+}  // extern "C"

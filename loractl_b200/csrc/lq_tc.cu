@@ -1956,6 +1956,17 @@ void lq_tc_gemm_bf16(const void* A, int a_mn, int64_t lda, const void* B, int b_
     throw LqError(LQ_ERR_UNSUPPORTED, "gemm: this (block_n, operand major) combination is not built");
 }
 
+void lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t Mg, int64_t Ng, int64_t Kg,
+                   cudaStream_t st) {
+    int dev;
+    LQ_CUDA(cudaGetDevice(&dev));
+    const Operand a{A, false, lda}, b{B, true, ldb};
+    if (pair_enabled() && Mg >= 256 && Ng > 192 && dev_ctx(dev).sm_count >= 2)
+        launch_gemm_pair<256, false, true>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, Mg, Ng, nullptr, st);
+    else
+        launch_gemm<128, false, true, __nv_bfloat16>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, 0, Mg, Ng, 1, nullptr, st);
+}
+
 // =========================================================================================
 // Split contraction for callers that must not allocate device memory
 // =========================================================================================
