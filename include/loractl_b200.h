@@ -291,6 +291,13 @@ size_t lq_mx4_matmul_workspace_bytes(int64_t n, int64_t m, int64_t k);
 int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales,
                   int64_t m, int64_t k, const float* bias, void* y, int y_dtype, void* ws, size_t ws_bytes, void* stream);
 
+/* lq_mx4_quantize of x [n, k] (`ldx` elements between rows) and lq_mx4_matmul in one call, Y in x's type: the product's first
+ * weight tiles are fetched while x is quantised.  `ws`: lq_mx4_linear_workspace_bytes() bytes on the current device,
+ * 256-byte aligned. */
+size_t lq_mx4_linear_workspace_bytes(int64_t n, int64_t m, int64_t k);
+int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* w_codes, const void* w_scales, int64_t m,
+                  int64_t k, const float* bias, void* y, void* ws, size_t ws_bytes, void* stream);
+
 /* dX[n, k] = dY[n, m] . W[m, k]: the gradient through the frozen weight (that of crates/loractl-core/src/
  * quant.rs:221-235), with the quantisation of x taken as the identity.  dy, dx contiguous, 16-byte aligned, LQ_BF16
  * (W is exact in bf16) or LQ_F32 (f32 arithmetic).  `ws`: lq_mx4_matmul_dx_workspace_bytes() bytes, 256-byte aligned. */

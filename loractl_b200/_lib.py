@@ -94,6 +94,8 @@ SIGNATURES = {
     "lq_mx4_dequantize": (_I, [_P, _P, _I64, _I64, _P, _I, _P]),
     "lq_mx4_matmul_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "lq_mx4_matmul": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I, _P, _SZ, _P]),
+    "lq_mx4_linear_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "lq_mx4_linear": (_I, [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
     "lq_mx4_matmul_dx_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "lq_mx4_matmul_dx": (_I, [_P, _I, _I64, _P, _P, _I64, _I64, _P, _P, _SZ, _P]),
     "lq_grad_nonfinite_flag": (_I, [_P, _I64, _P, _P]),
@@ -113,8 +115,8 @@ SIGNATURES = {
     "lq_sigmoid_gate_bwd": (_I, [_P, _P, _P, _I, _I64, _P, _P, _P]),
     "lq_gate_residual_bwd": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _P, _P, _P, C.c_size_t, _P]),
     "lq_residual_norm_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
-    "lq_residual_norm_fwd": (_I, [C.POINTER(ResidualNormArgs), _P]),
-    "lq_residual_norm_bwd": (_I, [C.POINTER(ResidualNormArgs), C.POINTER(ResidualNormGrads), _P, _SZ, _P]),
+    "lq_residual_norm_fwd": (_I, [_P, _P]),
+    "lq_residual_norm_bwd": (_I, [_P, _P, _P, _SZ, _P]),
     "lq_check_device_status": (_I, [_P]),
     "lq_selftest_bounded_wait": (_I, [C.c_uint, _P]),
     "lq_kernel_launch_count": (C.c_uint64, []),

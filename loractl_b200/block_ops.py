@@ -17,14 +17,15 @@ CUDA tensors only (f32 or bf16): like every other op of this package there is no
 """
 from __future__ import annotations
 
-import ctypes as C
+import functools
+import struct
 from typing import Dict, Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .quant import _dtype_code, _require_cuda, _stream_ptr
+from .quant import _dtype_code, _on_device, _raw_stream, _require_cuda, _stream_ptr
 
 LN_EPS = 1e-5  # torch.nn.functional.layer_norm's default, which the harness block used before
 
@@ -211,30 +212,32 @@ def zrmsnorm(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 
 # ---- the seam between two sub-blocks --------------------------------------------------------------
 
+# `lq_residual_norm_args` and `lq_residual_norm_grads` as one pack each: setting thirty ctypes fields takes longer
+# than the kernel of a short call
+_ARGS = struct.Struct("@12P10q3i2f0P")
+_GRADS = struct.Struct("@2P4q7P")
+
+
+@functools.lru_cache(maxsize=256)
+def _residual_norm_ws(index: int, b: int, t: int, h: int) -> int:
+    return L.lib().lq_residual_norm_workspace_bytes(b, t, h)
+
 
 def _rows(v: torch.Tensor) -> torch.Tensor:
     """`v` itself when its rows are contiguous (any sample and token stride), a copy otherwise."""
     return v if v.stride(-1) == 1 or v.shape[-1] == 1 else v.contiguous()
 
 
-def _strides(v: torch.Tensor) -> Tuple[int, int]:
-    return v.stride(0), v.stride(1)
-
-
-def _vectors(b: int, h: int, **vectors: torch.Tensor):
-    """The modulation vectors as `[b, h]` views of one type: theirs when they agree on f32 or bf16, else f32."""
-    for name, v in vectors.items():
-        if v.numel() != b * h or v.shape[0] != b or v.shape[-1] != h:
-            raise ValueError(f"{name} must be [b = {b}, h = {h}] or [b, 1, h], got {list(v.shape)}")
-        if v.dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError(f"unsupported {name} dtype {v.dtype}: f32 or bf16")
-    kinds = {v.dtype for v in vectors.values()}
-    dtype = kinds.pop() if len(kinds) == 1 else torch.float32
-    out = {}
-    for name, v in vectors.items():
-        v = v.to(dtype).reshape(b, h)
-        out[name] = v if v.stride(1) == 1 or h == 1 else v.contiguous()
-    return out, dtype
+def _vector(v: torch.Tensor, b: int, h: int, dtype: torch.dtype, name: str) -> torch.Tensor:
+    """A modulation vector as a `[b, h]` view (a copy where its type differs or its rows are not contiguous)."""
+    shape = v.shape
+    if shape[-1] != h or shape[0] != b or v.numel() != b * h:
+        raise ValueError(f"{name} must be [b = {b}, h = {h}] or [b, 1, h], got {list(shape)}")
+    if v.dtype != dtype:
+        v = v.to(dtype)
+    if len(shape) != 2:
+        v = v.reshape(b, h)
+    return v if v.stride(1) == 1 or h == 1 else v.contiguous()
 
 
 def _norm_weight(w: Optional[torch.Tensor], h: int, name: str) -> Optional[torch.Tensor]:
@@ -242,50 +245,60 @@ def _norm_weight(w: Optional[torch.Tensor], h: int, name: str) -> Optional[torch
         return None
     if w.numel() != h:
         raise ValueError(f"{name} must hold {h} values, got {list(w.shape)}")
-    return w.detach().to(torch.float32).reshape(h).contiguous()
+    if w.dtype != torch.float32 or w.dim() != 1:
+        w = w.to(torch.float32).reshape(h)
+    return w if w.stride(0) == 1 else w.contiguous()
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _residual_norm(x, gate, y, shift, scale, weight, post_weight, layer, alpha, eps, want_stats):
+    """The checks and the forward launch; returns (outputs, what the backward needs)."""
+    _require_cuda(x, "x")
+    b, t, h = _dims(x)
+    dtype, device = _dtype_code(x), x.device
+    if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
+        raise ValueError(f"x and y must agree in shape and dtype, got {list(x.shape)} {x.dtype} / {list(y.shape)} {y.dtype}")
+    index = x.get_device()
+    for name, v in (("gate", gate), ("y", y), ("shift", shift), ("scale", scale), ("weight", weight), ("post_weight", post_weight)):
+        if v is not None and v.get_device() != index:
+            raise RuntimeError(f"{name} is on {v.device}, x on {device}")
+    # one type for the modulation vectors: theirs when they agree on f32 or bf16, else f32
+    kinds = {v.dtype for v in (gate, shift, scale) if v is not None}
+    if not kinds <= {torch.float32, torch.bfloat16}:
+        raise TypeError(f"unsupported dtype of gate, shift or scale {sorted(map(str, kinds))}: f32 or bf16")
+    mod_dtype = shift.dtype if len(kinds) == 1 else torch.float32
+    gate = None if y is None else _vector(gate, b, h, mod_dtype, "gate")
+    shift, scale = _vector(shift, b, h, mod_dtype, "shift"), _vector(scale, b, h, mod_dtype, "scale")
+    w, pw = _norm_weight(weight, h, "weight"), _norm_weight(post_weight, h, "post_weight")
+    x = _rows(x)
+    z = torch.empty((b, t, h), dtype=x.dtype, device=device)
+    r, yp, ys, gp, gs, rp = None, 0, (0, 0, 0), 0, 0, 0
+    if y is not None:
+        y = _rows(y)
+        r = torch.empty_like(z)
+        yp, ys, gp, gs, rp = y.data_ptr(), y.stride(), gate.data_ptr(), gate.stride(0), r.data_ptr()
+    stats, sp = None, (0, 0, 0)
+    if want_stats:
+        stats = torch.empty((3, b * t), dtype=torch.float32, device=device)
+        p = stats.data_ptr()
+        sp = (p, p + 4 * b * t, p + 8 * b * t)
+    xs = x.stride()
+    args = _ARGS.pack(x.data_ptr(), yp, gp, shift.data_ptr(), scale.data_ptr(), 0 if w is None else w.data_ptr(),
+                      0 if pw is None else pw.data_ptr(), rp, z.data_ptr(), *sp, xs[0], xs[1], ys[0], ys[1], gs, shift.stride(0),
+                      scale.stride(0), b, t, h, dtype, mod_dtype == torch.float32, layer, alpha, eps)
+    with _on_device(index):
+        L.check(L.lib().lq_residual_norm_fwd(args, _raw_stream(index)))
+    return (z,) if r is None else (r, z), (args, mod_dtype, (x, y, gate, shift, scale, w, pw, stats))
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate, y, shift, scale, weight, post_weight, layer, alpha, eps):
-        _require_cuda(x, "x")
-        b, t, h = _dims(x)
-        dtype = _dtype_code(x)
-        if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
-            raise ValueError(f"x and y must agree in shape and dtype, got {list(x.shape)} {x.dtype} / {list(y.shape)} {y.dtype}")
-        named = {"shift": shift, "scale": scale} if y is None else {"gate": gate, "shift": shift, "scale": scale}
-        for name, v in {**named, "y": y, "weight": weight, "post_weight": post_weight}.items():
-            if v is not None and v.device != x.device:
-                raise RuntimeError(f"{name} is on {v.device}, x on {x.device}")
-        mods, mod_dtype = _vectors(b, h, **named)
-        w, pw = _norm_weight(weight, h, "weight"), _norm_weight(post_weight, h, "post_weight")
-        xr, yr = _rows(x), None if y is None else _rows(y)
-        z = torch.empty((b, t, h), dtype=x.dtype, device=x.device)
-        r = torch.empty_like(z) if y is not None else None
-        args = L.ResidualNormArgs(x=_ptr(xr), y=_ptr(yr), shift=_ptr(mods["shift"]), scale=_ptr(mods["scale"]), weight=_ptr(w),
-                                  post_weight=_ptr(pw), r=_ptr(r), z=_ptr(z), samples=b, tokens=t, h=h, dtype=dtype,
-                                  mod_f32=int(mod_dtype == torch.float32), layer=int(layer), alpha=alpha, eps=eps)
-        args.x_sample, args.x_token = _strides(xr)
-        args.shift_sample, args.scale_sample = mods["shift"].stride(0), mods["scale"].stride(0)
-        if yr is not None:
-            args.y_sample, args.y_token = _strides(yr)
-            args.gate, args.gate_sample = _ptr(mods["gate"]), mods["gate"].stride(0)
-        stats = None
-        if any(ctx.needs_input_grad):
-            stats = torch.empty((3, b * t), dtype=torch.float32, device=x.device)
-            args.mean, args.rstd, args.post_rstd = (stats[i].data_ptr() for i in range(3))
-        with torch.cuda.device(x.device):
-            L.check(L.lib().lq_residual_norm_fwd(C.byref(args), _stream_ptr(x.device)))
-        ctx.args = args  # the addresses are those of the saved tensors below, except r and z, which the backward does not read
-        ctx.mod_dtype = mod_dtype
-        ctx.like = [None if v is None else (v.shape, v.dtype) for v in (gate, shift, scale, weight, post_weight)]
-        ctx.save_for_backward(xr, yr, mods.get("gate"), mods["shift"], mods["scale"], w, pw, stats)
+    def forward(ctx, *inputs):
+        outs, (ctx.args, ctx.mod_dtype, saved) = _residual_norm(*inputs, True)
+        # the addresses in `args` are those of the saved tensors; r and z among them are not read by the backward
+        ctx.save_for_backward(*saved)
+        ctx.like = [None if v is None else (v.shape, v.dtype) for v in (inputs[1], *inputs[3:7])]
         ctx.set_materialize_grads(False)
-        return z if r is None else (r, z)
+        return outs if len(outs) == 2 else outs[0]
 
     @staticmethod
     @once_differentiable
@@ -293,38 +306,53 @@ class _ResidualNorm(torch.autograd.Function):
         dr, dz = douts if len(douts) == 2 else (None, douts[0])
         if dr is None and dz is None:
             return (None,) * 10
-        xr, yr, gate, shift, scale, w, pw, stats = ctx.saved_tensors
-        b, t, h = xr.shape
-        dev, args = xr.device, ctx.args
-        need = ctx.needs_input_grad
-        new = lambda wanted, dtype, *shape: torch.empty(shape, dtype=dtype, device=dev) if wanted else None
-        dx, dy = new(need[0], xr.dtype, b, t, h), new(need[2], xr.dtype, b, t, h)
-        dgate, dshift, dscale = (new(need[i], ctx.mod_dtype, b, h) for i in (1, 3, 4))
-        dw, dpw = new(need[5], torch.float32, h), new(need[6], torch.float32, h)
-        g = L.ResidualNormGrads(dx=_ptr(dx), dy=_ptr(dy), dgate=_ptr(dgate), dshift=_ptr(dshift), dscale=_ptr(dscale),
-                                dweight=_ptr(dw), dpost_weight=_ptr(dpw))
+        x = ctx.saved_tensors[0]  # the others only have to live
+        b, t, h = x.shape
+        dev, index, need = x.device, x.get_device(), ctx.needs_input_grad
+        dx = torch.empty((b, t, h), dtype=x.dtype, device=dev) if need[0] else None
+        dy = torch.empty((b, t, h), dtype=x.dtype, device=dev) if need[2] else None
+        wanted = (need[1], need[3], need[4], need[5], need[6])
+        grads = [None] * 5
+        if any(wanted[:3]):  # one buffer for the three: a view each
+            for i, v in enumerate(torch.empty((3, b, h), dtype=ctx.mod_dtype, device=dev).unbind(0)):
+                grads[i] = v if wanted[i] else None
+        if any(wanted[3:]):
+            for i, v in enumerate(torch.empty((2, h), dtype=torch.float32, device=dev).unbind(0), 3):
+                grads[i] = v if wanted[i] else None
+        rp, rs, zp, zs = 0, (0, 0), 0, (0, 0)
         if dr is not None:
             dr = _rows(dr)
-            g.dr, (g.dr_sample, g.dr_token) = _ptr(dr), _strides(dr)
+            rp, rs = dr.data_ptr(), dr.stride()
         if dz is not None:
             dz = _rows(dz)
-            g.dz, (g.dz_sample, g.dz_token) = _ptr(dz), _strides(dz)
-        with torch.cuda.device(dev):
-            ws = None
-            if any(v is not None for v in (dgate, dshift, dscale, dw, dpw)):
+            zp, zs = dz.data_ptr(), dz.stride()
+        at = [0 if v is None else v.data_ptr() for v in (dx, dy, *grads)]
+        g = _GRADS.pack(rp, zp, rs[0], rs[1], zs[0], zs[1], *at)
+        with _on_device(index):
+            ws, nbytes = None, 0
+            if any(wanted):
                 # of this call alone: from the pool of the current stream, or of the graph being captured
-                ws = torch.empty(L.lib().lq_residual_norm_workspace_bytes(b, t, h), dtype=torch.uint8, device=dev)
-            L.check(L.lib().lq_residual_norm_bwd(C.byref(args), C.byref(g), _ptr(ws), 0 if ws is None else ws.numel(),
-                                                 _stream_ptr(dev)))
-        back = [None if v is None else v.to(like[1]).reshape(like[0])
-                for v, like in zip((dgate, dshift, dscale, dw, dpw), ctx.like)]
-        return dx, back[0], dy, back[1], back[2], back[3], back[4], None, None, None
+                nbytes = _residual_norm_ws(index, b, t, h)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            L.check(L.lib().lq_residual_norm_bwd(ctx.args, g, None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index)))
+        for i, like in enumerate(ctx.like):
+            if grads[i] is not None:
+                v = grads[i] if grads[i].dtype == like[1] else grads[i].to(like[1])
+                grads[i] = v if v.shape == like[0] else v.view(like[0])
+        return dx, grads[0], dy, grads[1], grads[2], grads[3], grads[4], None, None, None
+
+
+def _apply_residual_norm(*inputs):
+    if torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in inputs[:7]):
+        return _ResidualNorm.apply(*inputs)
+    outs, _ = _residual_norm(*inputs, False)
+    return outs if len(outs) == 2 else outs[0]
 
 
 def modulated_zrmsnorm(x: torch.Tensor, weight: Optional[torch.Tensor], shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """`zrmsnorm(x, weight) * (1 + scale) + shift` (mmdit.rs:857-862 before a sub-block), one kernel each way; `weight`
     `[h]` or None.  Gradients flow to every argument that asks for one, the norm's weight among them."""
-    return _ResidualNorm.apply(x, None, None, shift, scale, weight, None, False, 1.0, ZRMS_EPS)
+    return _apply_residual_norm(x, None, None, shift, scale, weight, None, False, 1.0, ZRMS_EPS)
 
 
 def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
@@ -344,4 +372,4 @@ def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, sh
     if norm not in ("zrms", "layer"):
         raise ValueError(f"norm must be zrms or layer, got {norm!r}")
     eps = ZRMS_EPS if norm == "zrms" else LN_EPS
-    return _ResidualNorm.apply(x, gate, y, shift, scale, weight, post_weight, norm == "layer", float(residual_scale), eps)
+    return _apply_residual_norm(x, gate, y, shift, scale, weight, post_weight, norm == "layer", float(residual_scale), eps)

@@ -23,6 +23,7 @@
 
 #include "lq_internal.cuh"
 #include "lq_prof.cuh"
+#include "lq_stream.cuh"
 #include "lq_tc.cuh"
 #include "lq_umma.cuh"
 
@@ -105,6 +106,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__
     const int64_t kb = (k + 255) / 256;
     const int64_t items = pad_rows * kb;
     const int lane = threadIdx.x & 31;
+    lqstream::pdl_launch_dependents();  // a product behind this launch may start fetching its weight
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
         const int64_t row = it / kb, b = it - row * kb;
         const int64_t col = b * 256 + lane * 8;
@@ -214,8 +216,11 @@ struct CfgT {
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + 2 * S_BYTES;
     static constexpr int STAGES = (200 * 1024) / STAGE < 10 ? (200 * 1024) / STAGE : 10;
     static constexpr uint32_t TMEM = 512;
-    static constexpr uint32_t SCALE_COL = 2 * BN;  // behind the two accumulators: 16 columns per stage
-    static_assert(2 * BN + 16 * STAGES <= 512, "tensor memory");
+    // An MMA of few columns takes its latency, not its work, when the next one waits for its sum: the four MMAs
+    // of a k-block then go to an accumulator each.
+    static constexpr int ACCS = BN <= 32 ? 4 : 1;
+    static constexpr uint32_t SCALE_COL = 2 * ACCS * BN;  // behind the two sets of accumulators: 16 columns per stage
+    static_assert(SCALE_COL + 16 * STAGES <= 512, "tensor memory");
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 256;
 };
 
@@ -278,18 +283,36 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
             uint32_t phase = 0;
             bool ok = true;
             const int kt = 2 * p.kb;
+            auto load_w = [&](int st, int wt, int kb) {
+                const uint32_t bar = smem_u32(&full[st]);
+                mbar_expect_tx(bar, C::STAGE);
+                tma_load_2d(smem_u32(smem_a + (size_t)st * C::A_BYTES), &tmW, bar, kb * 128, wt * 128);
+                bulk_load(smem_u32(smem_s + (size_t)st * 2 * C::S_BYTES), p.w_scales + ((int64_t)wt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
+            };
+            auto load_x = [&](int st, int xt, int kb) {
+                const uint32_t bar = smem_u32(&full[st]);
+                tma_load_2d(smem_u32(smem_b + (size_t)st * C::B_BYTES), &tmX, bar, kb * 128, xt * BN);
+                bulk_load(smem_u32(smem_s + (size_t)st * 2 * C::S_BYTES + C::S_BYTES), p.x_scales + ((int64_t)xt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
+            };
+            // the weight does not depend on the launch before this one (the quantisation of x): its first stages
+            // are fetched while that runs
+            int wt, xt, z, k0, k1, ahead = 0;
+            if ((int)blockIdx.x < items) {
+                range(blockIdx.x, wt, xt, z, k0, k1);
+                ahead = min(STAGES, k1 - k0);
+                for (int i = 0; i < ahead; ++i) load_w(i, wt, k0 + i);
+            }
+            lqstream::pdl_wait();
             for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-                int wt, xt, z, k0, k1;
                 range(item, wt, xt, z, k0, k1);
                 for (int kb = k0; kb < k1; ++kb) {
-                    if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 71)) { ok = false; break; }
-                    const uint32_t bar = smem_u32(&full[s]);
-                    uint8_t* sc = smem_s + (size_t)s * 2 * C::S_BYTES;
-                    mbar_expect_tx(bar, C::STAGE);
-                    tma_load_2d(smem_u32(smem_a + (size_t)s * C::A_BYTES), &tmW, bar, kb * 128, wt * 128);
-                    tma_load_2d(smem_u32(smem_b + (size_t)s * C::B_BYTES), &tmX, bar, kb * 128, xt * BN);
-                    bulk_load(smem_u32(sc), p.w_scales + ((int64_t)wt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
-                    bulk_load(smem_u32(sc + C::S_BYTES), p.x_scales + ((int64_t)xt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
+                    if (ahead > 0) {
+                        --ahead;
+                    } else {
+                        if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 71)) { ok = false; break; }
+                        load_w(s, wt, kb);
+                    }
+                    load_x(s, xt, kb);
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
@@ -307,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
                 range(item, wt, xt, z, k0, k1);
                 if (!mbar_wait(smem_u32(&tempty[acc]), acc_phase ^ 1u, abort_flag, p.status, 72)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(acc * BN);
+                const uint32_t d = tmem + (uint32_t)(acc * C::ACCS * BN);
                 for (int kb = k0; kb < k1; ++kb) {
                     if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 73)) { ok = false; break; }
                     tc_fence_after();
@@ -321,8 +344,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
                     const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k)  // 64 elements = 32 bytes; scale pair k & 1 of tile k / 2
-                        mma_mxf4(d, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi), idesc_mxf4(128, BN, k & 1),
-                                 sfa + 4 * (k >> 1), sfb + 4 * (k >> 1), (kb > k0 || k > 0) ? 1u : 0u);
+                        mma_mxf4(d + k % C::ACCS * BN, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi),
+                                 idesc_mxf4(128, BN, k & 1), sfa + 4 * (k >> 1), sfb + 4 * (k >> 1),
+                                 (kb > k0 || k >= C::ACCS) ? 1u : 0u);
                     mma_commit(smem_u32(&empty[s]));
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
@@ -344,15 +368,19 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
             const float bias = (p.splits == 1 && p.bias && row < p.m) ? p.bias[row] : 0.f;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 16) {
-                uint32_t r[16];
-                tmem_ld_x16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN + c), r);
+                uint32_t r[C::ACCS][16];
+#pragma unroll
+                for (int a = 0; a < C::ACCS; ++a)
+                    tmem_ld_x16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((acc * C::ACCS + a) * BN + c), r[a]);
                 tmem_ld_wait();
                 if (row < p.m)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const int tok = xt * BN + c + j;
                         if (tok >= p.n) break;
-                        const float v = __uint_as_float(r[j]);
+                        float v = __uint_as_float(r[0][j]);
+#pragma unroll
+                        for (int a = 1; a < C::ACCS; ++a) v += __uint_as_float(r[a][j]);
                         const int64_t o = (int64_t)tok * p.m + row;
                         if (p.splits > 1) p.part[(int64_t)z * p.n * p.m + o] = v;
                         else if (p.y_f32) ((float*)p.y)[o] = v + bias;
@@ -374,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
 
 // y = sum of the splits in order + bias.
 __global__ void __launch_bounds__(256) mx4_join_kernel(ProductParams p) {
+    lqstream::pdl_wait();
     const int64_t n = (int64_t)p.n * p.m;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         float v = 0.f;
@@ -455,17 +484,53 @@ void launch_stream(ProductParams p, const void* w_codes, const void* x_codes, in
     LQ_CHECK_ARG(items < (int64_t)1 << 31, "too many tiles");
     {
         LqProf prof(LQ_K_GEMM_MAIN, st);
-        mx4_stream_kernel<BN><<<grid_of(items, sms, 1), kThreads, C::SMEM, st>>>(tw, tx, p);
+        lqstream::launch_pdl(mx4_stream_kernel<BN>, grid_of(items, sms, 1), kThreads, C::SMEM, st, tw, tx, p);
         LQ_CUDA(cudaGetLastError());
     }
     if (p.splits > 1) {
         LqProf prof(LQ_K_REDUCE, st);
-        mx4_join_kernel<<<grid_of(((int64_t)p.n * p.m + 255) / 256, sms, 8), 256, 0, st>>>(p);
+        lqstream::launch_pdl(mx4_join_kernel, grid_of(((int64_t)p.n * p.m + 255) / 256, sms, 8), 256, 0, st, p);
         LQ_CUDA(cudaGetLastError());
     }
 }
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+void quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, void* codes, void* scales, int dev, cudaStream_t st) {
+    const int64_t pad = row_tiles(rows) * 128;
+    const unsigned grid = grid_of((pad * ((k + 255) / 256) + 7) / 8, lq_tc_sm_count(dev), 16);
+    const int vec = al16(x) && (ld * (dtype == LQ_F32 ? 4 : 2)) % 16 == 0;
+    LqProf prof(LQ_K_QUANT, st);
+    if (dtype == LQ_F32)
+        mx4_quantize_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, k, ld, vec, pad, (uint32_t*)codes, (uint8_t*)scales);
+    else
+        mx4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, k, ld, vec, pad, (uint32_t*)codes,
+                                                                 (uint8_t*)scales);
+    LQ_CUDA(cudaGetLastError());
+}
+
+void product(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
+             const float* bias, void* y, int y_dtype, float* part, int dev, cudaStream_t st) {
+    const int sms = lq_tc_sm_count(dev), bn = bn_of(n);
+    ProductParams p;
+    p.w_scales = (const uint8_t*)w_scales;
+    p.x_scales = (const uint8_t*)x_scales;
+    p.m = (int)m;
+    p.n = (int)n;
+    p.kb = (int)((k + 255) / 256);
+    p.w_tiles = (int)((m + 127) / 128);
+    p.x_tiles = (int)((n + bn - 1) / bn);
+    p.splits = splits_of((int64_t)p.w_tiles * p.x_tiles, p.kb, sms);
+    p.part = part;
+    p.bias = bias;
+    p.y = y;
+    p.y_f32 = y_dtype == LQ_F32;
+    p.status = lq_tc_status_word(dev);
+    if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, sms, st);
+    else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, sms, st);
+    else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, sms, st);
+    else launch_stream<128>(p, w_codes, x_codes, k, sms, st);
+}
 
 }  // namespace
 
@@ -484,17 +549,7 @@ int lq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t l
         LQ_CHECK_ARG(x != nullptr, "NULL argument");
         check_tensor(codes, scales);
         LQ_CHECK_ARG(ld >= k || rows == 1, "rows overlap: the row stride is below their length");
-        cudaStream_t st = (cudaStream_t)stream;
-        const int64_t pad = row_tiles(rows) * 128;
-        const unsigned grid = grid_of((pad * ((k + 255) / 256) + 7) / 8, lq_tc_sm_count(current_device()), 16);
-        const int vec = al16(x) && (ld * (dtype == LQ_F32 ? 4 : 2)) % 16 == 0;
-        LqProf prof(LQ_K_QUANT, st);
-        if (dtype == LQ_F32)
-            mx4_quantize_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, k, ld, vec, pad, (uint32_t*)codes, (uint8_t*)scales);
-        else
-            mx4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, k, ld, vec, pad, (uint32_t*)codes,
-                                                                     (uint8_t*)scales);
-        LQ_CUDA(cudaGetLastError());
+        quantize(x, dtype, rows, k, ld, codes, scales, current_device(), (cudaStream_t)stream);
     });
 }
 
@@ -534,30 +589,37 @@ int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const vo
         check_tensor(x_codes, x_scales);
         check_tensor(w_codes, w_scales);
         LQ_CHECK_ARG(y != nullptr, "NULL argument");
-        cudaStream_t st = (cudaStream_t)stream;
-        const int dev = current_device(), sms = lq_tc_sm_count(dev);
-        if (ws_bytes < product_ws(n, m, k, sms) || (product_ws(n, m, k, sms) && !ws))
+        const int dev = current_device();
+        if (ws_bytes < product_ws(n, m, k, lq_tc_sm_count(dev)) || (ws_bytes && !ws))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled product");
         LQ_CHECK_ARG(al16(ws), "the workspace must be 16-byte aligned");
-        const int bn = bn_of(n);
-        ProductParams p;
-        p.w_scales = (const uint8_t*)w_scales;
-        p.x_scales = (const uint8_t*)x_scales;
-        p.m = (int)m;
-        p.n = (int)n;
-        p.kb = (int)((k + 255) / 256);
-        p.w_tiles = (int)((m + 127) / 128);
-        p.x_tiles = (int)((n + bn - 1) / bn);
-        p.splits = splits_of((int64_t)p.w_tiles * p.x_tiles, p.kb, sms);
-        p.part = (float*)ws;
-        p.bias = bias;
-        p.y = y;
-        p.y_f32 = y_dtype == LQ_F32;
-        p.status = lq_tc_status_word(dev);
-        if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, sms, st);
-        else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, sms, st);
-        else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, sms, st);
-        else launch_stream<128>(p, w_codes, x_codes, k, sms, st);
+        product(x_codes, x_scales, n, w_codes, w_scales, m, k, bias, y, y_dtype, (float*)ws, dev, (cudaStream_t)stream);
+    });
+}
+
+size_t lq_mx4_linear_workspace_bytes(int64_t n, int64_t m, int64_t k) {
+    if (n < 1 || m < 1 || k < 32) return 0;
+    return al256((size_t)n * k / 2) + al256(lq_mx4_scale_bytes(n, k)) + lq_mx4_matmul_workspace_bytes(n, m, k);
+}
+
+int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
+                  const float* bias, void* y, void* ws, size_t ws_bytes, void* stream) {
+    return guarded_call([&] {
+        LQ_CHECK_ARG(dtype == LQ_F32 || dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
+        check_dims(n, k);
+        check_dims(m, k);
+        if (n == 0 || m == 0) return;
+        check_tensor(w_codes, w_scales);
+        LQ_CHECK_ARG(x && y, "NULL argument");
+        LQ_CHECK_ARG(ldx >= k || n == 1, "rows overlap: the row stride is below their length");
+        LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
+        const int dev = current_device();
+        const size_t cb = al256((size_t)n * k / 2), sb = al256(lq_mx4_scale_bytes(n, k));
+        if (ws_bytes < cb + sb + product_ws(n, m, k, lq_tc_sm_count(dev)))
+            throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled linear");
+        uint8_t* codes = (uint8_t*)ws;
+        quantize(x, dtype, n, k, ldx, codes, codes + cb, dev, (cudaStream_t)stream);
+        product(codes, codes + cb, n, w_codes, w_scales, m, k, bias, y, dtype, (float*)(codes + cb + sb), dev, (cudaStream_t)stream);
     });
 }
 

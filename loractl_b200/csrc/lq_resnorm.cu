@@ -17,7 +17,9 @@
 //   S = sum_t dz rh,  T = sum_t dz,  G = sum_t D yh      per sample and column
 //   dscale = S (1 + w),  dshift = T,  dgate = G (1 + pw),  dw = sum_b S (1 + scale),  dpw = sum_b gate G
 // r is formed again from x and y instead of being read back: y is needed for G anyway, so it costs no
-// byte more than reading r and keeps rh at f32 accuracy.
+// byte more than reading r and keeps rh at f32 accuracy.  Forward and backward form it by the same operations in the same
+// order, fma(gate (1 + pw), y q, alpha x), since s and mu are those of the forward's r: where x and y nearly cancel, another
+// rounding of r would no longer fit them.
 #include <algorithm>
 
 #include <cuda_bf16.h>
@@ -25,6 +27,7 @@
 #include "lq_internal.cuh"
 #include "lq_prof.cuh"
 #include "lq_tc.cuh"
+#include "lq_umma.cuh"
 
 namespace {
 
@@ -33,314 +36,569 @@ typedef lq_residual_norm_args Args;
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// VEC elements of type T as f32, from an address aligned to the vector.  The token-shaped streams are read
-// past L1 (each byte is used once), so that the modulation vectors stay in it.
-template <typename T, int VEC>
-struct Io;
-template <typename T>
-struct Io<T, 1> {
-    static __device__ __forceinline__ void ld(const T* p, float (&f)[1]) { f[0] = to_f(*p); }
-    static __device__ __forceinline__ void st(T* p, const float (&f)[1]) { *p = (T)f[0]; }
-};
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-template <>
-struct Io<float, 4> {
-    static __device__ __forceinline__ void ld(const float* p, float (&f)[4]) {
-        const uint4 v = ld_stream(p);
-        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
-    }
-    static __device__ __forceinline__ void st(float* p, const float (&f)[4]) {
-        *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
-    }
-};
-template <>
-struct Io<__nv_bfloat16, 8> {
-    static __device__ __forceinline__ void ld(const __nv_bfloat16* p, float (&f)[8]) {
-        const uint4 v = ld_stream(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-    static __device__ __forceinline__ void st(__nv_bfloat16* p, const float (&f)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *(const uint32_t*)&h;
-        }
-        *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
+template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
 
-// VEC values of a modulation vector (f32 or bf16 by the call) starting at element `i` of `p`.
-template <int VEC>
-__device__ __forceinline__ void ld_mod(const void* p, int f32, int64_t i, float (&f)[VEC]) {
-    if (VEC == 1) {
-        f[0] = f32 ? ((const float*)p)[i] : to_f(((const __nv_bfloat16*)p)[i]);
-    } else if (f32) {
-#pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-            const float4 v = *(const float4*)((const float*)p + i + e);
-            f[e] = v.x, f[e + 1] = v.y, f[e + 2] = v.z, f[e + 3] = v.w;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-            const uint2 v = *(const uint2*)((const __nv_bfloat16*)p + i + e);
-            f[e] = __uint_as_float(v.x << 16), f[e + 1] = __uint_as_float(v.x & 0xFFFF0000u);
-            f[e + 2] = __uint_as_float(v.y << 16), f[e + 3] = __uint_as_float(v.y & 0xFFFF0000u);
-        }
-    }
+// One value of a modulation vector (f32 or bf16 by the call).
+__device__ __forceinline__ float mod_at(const void* p, int f32, int64_t i) {
+    return f32 ? ((const float*)p)[i] : to_f(((const __nv_bfloat16*)p)[i]);
 }
 
-// Sums of NV values over the threads of a block, in a fixed order; `buf` alternates between two areas,
-// so that one barrier per reduction is enough (whoever writes an area again has passed the barrier of the
-// reduction between).
-constexpr int kMaxWarps = 16;
+// Sums of NV values over the threads of a block, in a fixed order.  `area` has two halves that take turns, so that
+// one barrier per reduction is enough: whoever writes a half again has passed the barrier of the reduction between.
+// Its places behind the last warp hold zeros.
+constexpr int kMaxWarps = 32;
 template <int NV>
-__device__ __forceinline__ void block_sum(float (&v)[NV], float (*area)[kMaxWarps][2], int& buf) {
+__device__ __forceinline__ void warp_sum(float (&v)[NV]) {
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1)
 #pragma unroll
         for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
-    const int warps = blockDim.x >> 5;
-    if (warps == 1) return;
+}
+template <int MAXT, int NV>
+__device__ __forceinline__ void block_sum(float (&v)[NV], float (*area)[2][kMaxWarps], int& half) {
+    warp_sum<NV>(v);
+    if (MAXT <= 128 && blockDim.x == 32) {
+        __syncwarp();
+        return;
+    }
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
-        for (int k = 0; k < NV; ++k) area[buf][threadIdx.x >> 5][k] = v[k];
+        for (int k = 0; k < NV; ++k) area[half][k][threadIdx.x >> 5] = v[k];
     __syncthreads();
+    if (MAXT <= 256) {  // up to 8 partial sums: two vector reads are shorter than five exchanges
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        float s = 0.f;
-        for (int w = 0; w < warps; ++w) s += area[buf][w][k];
-        v[k] = s;
+        for (int k = 0; k < NV; ++k) {
+            v[k] = 0.f;
+#pragma unroll
+            for (int w = 0; w < MAXT / 32; w += 4) {
+                const float4 q = *(const float4*)&area[half][k][w];
+                v[k] += (q.x + q.y) + (q.z + q.w);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) v[k] = area[half][k][threadIdx.x & 31];
+        warp_sum<NV>(v);
     }
-    buf ^= 1;
+    half ^= 1;
+}
+__device__ __forceinline__ void clear_area(float (*area)[2][kMaxWarps]) {
+    for (int i = threadIdx.x; i < 2 * 2 * kMaxWarps; i += blockDim.x) (&area[0][0][0])[i] = 0.f;
+    __syncthreads();
 }
 
-// One block per row; thread t owns the vectors t, t + blockDim, ... of the row and keeps r in registers
-// between the statistics and the output.
-template <typename T, int VEC, int VPT>
-__global__ void __launch_bounds__(512) resnorm_fwd_kernel(const Args a) {
-    __shared__ float area[2][kMaxWarps][2];
-    int buf = 0;
-    const int64_t row = blockIdx.x, b = row / a.tokens, t = row - b * a.tokens;
-    const int h = (int)a.h, nvec = h / VEC;
+// 1 / sqrt(v): the hardware's estimate and one Newton step (the IEEE square root and quotient are forty
+// instructions that every thread of a row would run).
+__device__ __forceinline__ float rsqrt_f32(float v) {
+    const float y = rsqrtf(v);
+    return y * fmaf(-0.5f * v * y, y, 1.5f);
+}
+
+// The rows of one block: chunk `blockIdx.x % chunks` of a sample.
+struct Rows {
+    int64_t b, t0, t1;
+    __device__ __forceinline__ Rows(int64_t tokens, int chunks, int64_t per) {
+        b = blockIdx.x / chunks;
+        t0 = (blockIdx.x - b * chunks) * per;
+        t1 = min(tokens, t0 + per);
+    }
+};
+
+// ---- rows that start on 16 bytes ------------------------------------------------------------------
+// HBM-bound, so what counts is bytes in flight.  A block walks the rows of its chunk; a few threads keep a ring of
+// rows in shared memory filled with bulk copies (a row of each input per stage), and no other thread waits for HBM
+// itself.  A thread owns 8 columns for good: it keeps the modulation of the sample and, in the backward, its column
+// sums in registers, so that the only exchange is the row's own sums, and a stage may be refilled after the barrier
+// of the first of them.
+// Register rows instead of the ring (one row per block, loads straight to registers) took 29 us forward and 95 us
+// backward on 1536 rows of 6144 bf16 columns; the modulation read again from L1 for every row was part of that.
+constexpr int kMaxStages = 8;
+
+// Eight elements as they are stored (four registers in bf16): what is needed again behind a barrier waits like this.
+template <typename T>
+struct Raw8 {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ void ld(const uint8_t* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = ((const uint4*)p)[i];
+    }
+    __device__ __forceinline__ float operator[](int e) const {
+        const uint4 q = v[sizeof(T) == 4 ? e >> 2 : 0];
+        const int k = sizeof(T) == 4 ? e & 3 : e >> 1;
+        const uint32_t w = k == 0 ? q.x : (k == 1 ? q.y : (k == 2 ? q.z : q.w));
+        return sizeof(T) == 4 ? __uint_as_float(w) : __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+    }
+};
+template <typename T>
+__device__ __forceinline__ void ld8(const uint8_t* p, float (&f)[8]) {
+    Raw8<T> r;
+    r.ld(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = r[e];
+}
+__device__ __forceinline__ void st8(__nv_bfloat16* p, const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *(const uint32_t*)&h;
+    }
+    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void st8(float* p, const float (&f)[8]) {
+    *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
+    *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void ld_mod8(const void* p, int f32, int64_t i, float (&f)[8]) {
+    if (f32) ld8<float>((const uint8_t*)p + i * 4, f);
+    else ld8<__nv_bfloat16>((const uint8_t*)p + i * 2, f);
+}
+
+// The ring's filling: thread i < inputs copies input i's row of a stage (the same instruction of one warp), thread 0
+// announces the bytes.
+struct Feed {
+    const uint8_t* src;
+    int64_t step;
+    __device__ __forceinline__ void of(const void* p, int64_t first, int64_t token, int esz) {
+        src = (const uint8_t*)p + first * esz;
+        step = token * esz;
+    }
+    __device__ __forceinline__ void fill(uint32_t bar, uint32_t stage, uint32_t row_bytes, uint32_t stage_bytes) {
+        if (threadIdx.x == 0) umma::mbar_expect_tx(bar, stage_bytes);
+        umma::bulk_load(stage + threadIdx.x * row_bytes, src, row_bytes, bar);
+        src += step;
+    }
+};
+
+extern __shared__ __align__(128) uint8_t ring_smem[];
+
+template <typename T, bool POST, bool LAYER, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) resnorm_fwd_ring_kernel(const Args a, int chunks, int64_t per, int stages, int* status) {
+    __shared__ __align__(16) float area[2][2][kMaxWarps];
+    __shared__ __align__(8) uint64_t bars[kMaxStages];
+    __shared__ int abort_flag;
+    const Rows rows(a.tokens, chunks, per);
+    const int h = (int)a.h, c = threadIdx.x * 8;
+    const bool in = c < h;
     const float inv_h = 1.f / (float)h;
-    const T* xr = (const T*)a.x + b * a.x_sample + t * a.x_token;
-    float r[VPT][VEC];
+    const int n = (int)(rows.t1 - rows.t0);
+    if (n <= 0) return;
+    const int inputs = a.y ? 2 : 1;
+    const uint32_t row_bytes = (uint32_t)h * sizeof(T), stage_bytes = row_bytes * inputs;
+    const uint32_t ring = umma::smem_u32(ring_smem);
+    Feed feed;
+    if (threadIdx.x == 0) feed.of(a.x, rows.b * a.x_sample + rows.t0 * a.x_token, a.x_token, sizeof(T));
+    else feed.of(a.y, rows.b * a.y_sample + rows.t0 * a.y_token, a.y_token, sizeof(T));
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) umma::mbar_init(umma::smem_u32(&bars[s]), 1);
+        abort_flag = 0;
+        umma::fence_barrier_init();
+        umma::fence_proxy_async_smem();
+    }
+    if (threadIdx.x < 32) {
+        __syncwarp();  // the barriers are there before any of the copying threads names one
+        if (threadIdx.x < inputs)
+            for (int s = 0; s < min(stages, n); ++s) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
+    }
+    clear_area(area);
+    float gate[8], shift[8], mul[8], pw[8];  // of this thread's columns; mul = (1 + w)(1 + scale)
+    if (in) {
+        float w[8];
+        ld_mod8(a.shift, a.mod_f32, rows.b * a.shift_sample + c, shift);
+        ld_mod8(a.scale, a.mod_f32, rows.b * a.scale_sample + c, mul);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mul[e] += 1.f;
+        if (a.weight) {
+            ld_mod8(a.weight, 1, c, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mul[e] *= 1.f + w[e];
+        }
+        if (a.y) ld_mod8(a.gate, a.mod_f32, rows.b * a.gate_sample + c, gate);
+        if (POST) {
+            ld_mod8(a.post_weight, 1, c, pw);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate[e] *= 1.f + pw[e];
+        }
+    }
+    int half = 0, s = 0;
+    uint32_t phase = 0;
+    const int64_t row0 = rows.b * a.tokens + rows.t0;
+    T *rp = (T*)a.r + row0 * h + c, *zp = (T*)a.z + row0 * h + c;
+    for (int i = 0; i < n; ++i) {
+        const int64_t row = row0 + i;
+        // a wait that gives up marks the error word; the block goes through its remaining rows without waiting
+        umma::mbar_wait(umma::smem_u32(&bars[s]), phase, &abort_flag, status, 81);
+        const uint8_t* st = ring_smem + s * stage_bytes + threadIdx.x * 8 * sizeof(T);
+        float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        float v[1] = {0.f};
+        if (in) ld8<T>(st, r);
+        if (a.y) {
+            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (in) ld8<T>(st + row_bytes, y);
+            float q = 1.f;
+            if (POST) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[0] = fmaf(y[e], y[e], v[0]);
+                block_sum<MAXT, 1>(v, area, half);
+                q = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
+                if (threadIdx.x == 0 && a.rstd) a.post_rstd[row] = q;
+                v[0] = 0.f;
+            }
+            if (in) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[e] = fmaf(gate[e], POST ? y[e] * q : y[e], a.alpha * r[e]);
+            }
+        }
+        float mu = 0.f;
+        if (LAYER) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[0] += r[e];
+            block_sum<MAXT, 1>(v, area, half);
+            mu = v[0] * inv_h;
+            v[0] = 0.f;
+        }
+        if (in) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[0] = fmaf(r[e] - mu, r[e] - mu, v[0]);
+        }
+        block_sum<MAXT, 1>(v, area, half);  // every thread has read the stage
+        if (threadIdx.x < inputs && i + stages < n) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
+        const float rs = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
+        if (threadIdx.x == 0 && a.rstd) {
+            a.rstd[row] = rs;
+            if (LAYER) a.mean[row] = mu;
+        }
+        if (in) {
+            if (a.r) st8(rp, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = fmaf((r[e] - mu) * rs, mul[e], shift[e]);
+            st8(zp, r);
+            rp += h;
+            zp += h;
+        }
+        if (++s == stages) { s = 0; phase ^= 1u; }
+    }
+    if (abort_flag)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the block ends
+}
+
+template <typename T, bool POST, bool LAYER, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) resnorm_bwd_ring_kernel(const Args a, const lq_residual_norm_grads g, int chunks, int64_t per,
+                                                                      int stages, float* __restrict__ part, int* status) {
+    __shared__ __align__(16) float area[2][2][kMaxWarps];
+    __shared__ __align__(8) uint64_t bars[kMaxStages];
+    __shared__ int abort_flag;
+    const Rows rows(a.tokens, chunks, per);
+    const int h = (int)a.h, c = threadIdx.x * 8;
+    const bool in = c < h;
+    const float inv_h = 1.f / (float)h;
+    const int n = (int)max((int64_t)0, rows.t1 - rows.t0);
+    const uint32_t row_bytes = (uint32_t)h * sizeof(T);
+    // a stage holds x, then what there is of dz, dr, y
+    const int i_dz = 1, i_dr = i_dz + (g.dz ? 1 : 0), i_y = i_dr + (g.dr ? 1 : 0), inputs = i_y + (a.y ? 1 : 0);
+    const uint32_t at_dz = row_bytes, at_dr = i_dr * row_bytes, at_y = i_y * row_bytes, stage_bytes = inputs * row_bytes;
+    const uint32_t ring = umma::smem_u32(ring_smem);
+    Feed feed;
+    if (threadIdx.x == 0) feed.of(a.x, rows.b * a.x_sample + rows.t0 * a.x_token, a.x_token, sizeof(T));
+    else if (g.dz && threadIdx.x == i_dz) feed.of(g.dz, rows.b * g.dz_sample + rows.t0 * g.dz_token, g.dz_token, sizeof(T));
+    else if (g.dr && threadIdx.x == i_dr) feed.of(g.dr, rows.b * g.dr_sample + rows.t0 * g.dr_token, g.dr_token, sizeof(T));
+    else feed.of(a.y, rows.b * a.y_sample + rows.t0 * a.y_token, a.y_token, sizeof(T));
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) umma::mbar_init(umma::smem_u32(&bars[s]), 1);
+        abort_flag = 0;
+        umma::fence_barrier_init();
+        umma::fence_proxy_async_smem();
+    }
+    if (threadIdx.x < 32) {
+        __syncwarp();  // the barriers are there before any of the copying threads names one
+        if (threadIdx.x < inputs)
+            for (int s = 0; s < min(stages, n); ++s) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
+    }
+    clear_area(area);
+    float gate[8], mul[8], S[8], D1[8], G[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gate[e] = mul[e] = S[e] = D1[e] = G[e] = 0.f;
+    if (in) {
+        ld_mod8(a.scale, a.mod_f32, rows.b * a.scale_sample + c, mul);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mul[e] += 1.f;
+        if (a.weight) {
+            float w[8];
+            ld_mod8(a.weight, 1, c, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mul[e] *= 1.f + w[e];
+        }
+        if (a.y) ld_mod8(a.gate, a.mod_f32, rows.b * a.gate_sample + c, gate);
+        if (POST) {  // gate (1 + pw) is all that the row needs; dgate gets its (1 + pw) with the sums
+            float pw[8];
+            ld_mod8(a.post_weight, 1, c, pw);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gate[e] *= 1.f + pw[e];
+        }
+    }
+    int half = 0, s = 0;
+    uint32_t phase = 0;
+    const int64_t row0 = rows.b * a.tokens + rows.t0;
+    T *dxp = (T*)g.dx + row0 * h + c, *dyp = (T*)g.dy + row0 * h + c;
+    float rs = n > 0 ? a.rstd[row0] : 0.f, mu = n > 0 && LAYER ? a.mean[row0] : 0.f, q = n > 0 && POST ? a.post_rstd[row0] : 1.f;
+    for (int i = 0; i < n; ++i) {
+        const int64_t row = row0 + i;
+        umma::mbar_wait(umma::smem_u32(&bars[s]), phase, &abort_flag, status, 82);
+        const uint8_t* st = ring_smem + s * stage_bytes + threadIdx.x * 8 * sizeof(T);
+        float rh[8], gz[8];
+        Raw8<T> yr, dr;
+        yr.zero();
+        dr.zero();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rh[e] = gz[e] = 0.f;
+        float v[2] = {0.f, 0.f};
+        if (in) {
+            ld8<T>(st, rh);
+            if (g.dz) ld8<T>(st + at_dz, gz);
+            if (a.y) {
+                yr.ld(st + at_y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rh[e] = fmaf(gate[e], POST ? yr[e] * q : yr[e], a.alpha * rh[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                rh[e] = LAYER ? (rh[e] - mu) * rs : rh[e] * rs;
+                S[e] = fmaf(gz[e], rh[e], S[e]);
+                D1[e] += gz[e];
+                gz[e] *= mul[e];
+                v[0] = fmaf(gz[e], rh[e], v[0]);
+                if (LAYER) v[1] += gz[e];
+            }
+            if (g.dr) dr.ld(st + at_dr);
+        }
+        if (LAYER) {
+            block_sum<MAXT, 2>(v, area, half);
+        } else {
+            float v1[1] = {v[0]};
+            block_sum<MAXT, 1>(v1, area, half);
+            v[0] = v1[0];
+        }
+        // every thread has read the stage
+        if (threadIdx.x < inputs && i + stages < n) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
+        const float c1 = v[0] * inv_h, c0 = LAYER ? v[1] * inv_h : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rh[e] = fmaf(rs, gz[e] - c0 - rh[e] * c1, dr[e]);  // D
+        const float q_row = q;
+        if (i + 1 < n) {  // the next row's statistics, behind the stores of this one
+            rs = a.rstd[row + 1];
+            if (LAYER) mu = a.mean[row + 1];
+            if (POST) q = a.post_rstd[row + 1];
+        }
+        float p[1] = {0.f};
+        if (a.y && in) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float yh = POST ? yr[e] * q_row : yr[e];
+                G[e] = fmaf(rh[e], yh, G[e]);
+                gz[e] = gate[e] * rh[e];  // the gradient of yh
+                if (POST) p[0] = fmaf(gz[e], yh, p[0]);
+                rh[e] *= a.alpha;
+            }
+        }
+        if (g.dx && in) st8(dxp, rh);
+        dxp += h;
+        if (a.y && g.dy) {
+            if (POST) {
+                block_sum<MAXT, 1>(p, area, half);
+                const float pm = p[0] * inv_h;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) gz[e] = q_row * (gz[e] - yr[e] * q_row * pm);
+            }
+            if (in) st8(dyp, gz);
+            dyp += h;
+        }
+        if (++s == stages) { s = 0; phase ^= 1u; }
+    }
+    if (part && in) {
+        float* dst = part + (int64_t)blockIdx.x * 3 * h + c;
+        st8(dst, S);
+        st8(dst + h, D1);
+        st8(dst + 2 * h, G);
+    }
+    if (abort_flag)
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+}
+
+// ---- any rows -----------------------------------------------------------------------------------
+// Single elements, for rows that do not all start on 16 bytes (an odd width, an odd offset) and for rows too wide
+// for the ring: thread t owns the columns t, t + blockDim, ...  All of a row's loads are issued before the first is
+// used, whatever columns the thread has (a place behind the row reads column 0 and counts as zero).
+template <typename T, int VPT>
+__device__ __forceinline__ void ld_row(const T* p, int h, float (&f)[VPT]) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int c = threadIdx.x + i * blockDim.x;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) r[i][e] = 0.f;
-        if (c < nvec) Io<T, VEC>::ld(xr + c * VEC, r[i]);
+        const float v = to_f(p[c < h ? c : 0]);
+        f[i] = c < h ? v : 0.f;
     }
+}
+template <int VPT>
+__device__ __forceinline__ void ld_mods(const void* p, int f32, int64_t at, int h, float (&f)[VPT]) {
+    if (f32) ld_row<float, VPT>((const float*)p + at, h, f);
+    else ld_row<__nv_bfloat16, VPT>((const __nv_bfloat16*)p + at, h, f);
+}
+template <typename T, int VPT>
+__device__ __forceinline__ void st_row(T* p, int h, const float (&f)[VPT]) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = threadIdx.x + i * blockDim.x;
+        if (c < h) p[c] = from_f<T>(f[i]);
+    }
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(512) resnorm_fwd_kernel(const Args a) {
+    constexpr int MAXT = 512;
+    __shared__ __align__(16) float area[2][2][kMaxWarps];
+    int half = 0;
+    const int64_t row = blockIdx.x, b = row / a.tokens, t = row - b * a.tokens;
+    const int h = (int)a.h;
+    const float inv_h = 1.f / (float)h;
+    float r[VPT], m[VPT], v[1] = {0.f};
+    ld_row<T, VPT>((const T*)a.x + b * a.x_sample + t * a.x_token, h, r);
     if (a.y) {
-        const T* yr = (const T*)a.y + b * a.y_sample + t * a.y_token;
-        float y[VPT][VEC];
-        float q = 1.f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) y[i][e] = 0.f;
-            if (c < nvec) Io<T, VEC>::ld(yr + c * VEC, y[i]);
-        }
+        float y[VPT], gt[VPT];
+        ld_row<T, VPT>((const T*)a.y + b * a.y_sample + t * a.y_token, h, y);
+        ld_mods<VPT>(a.gate, a.mod_f32, b * a.gate_sample, h, gt);
+        if (a.post_weight) ld_row<float, VPT>(a.post_weight, h, m);
+        clear_area(area);
         if (a.post_weight) {
-            float v[1] = {0.f};
 #pragma unroll
-            for (int i = 0; i < VPT; ++i)
+            for (int i = 0; i < VPT; ++i) v[0] = fmaf(y[i], y[i], v[0]);
+            block_sum<MAXT, 1>(v, area, half);
+            const float q = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
+            if (threadIdx.x == 0 && a.rstd) a.post_rstd[row] = q;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[0] = fmaf(y[i][e], y[i][e], v[0]);
-            block_sum<1>(v, area, buf);
-            q = 1.f / sqrtf(v[0] * inv_h + a.eps);
-            if (threadIdx.x == 0 && a.post_rstd) a.post_rstd[row] = q;
-        }
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-            if (c < nvec) {
-                float g[VEC], pw[VEC];
-                ld_mod<VEC>(a.gate, a.mod_f32, b * a.gate_sample + c * VEC, g);
-                if (a.post_weight) ld_mod<VEC>(a.post_weight, 1, c * VEC, pw);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float u = a.post_weight ? y[i][e] * q * (1.f + pw[e]) : y[i][e];
-                    r[i][e] = fmaf(g[e], u, a.alpha * r[i][e]);
-                }
-                if (a.r) Io<T, VEC>::st((T*)a.r + row * h + c * VEC, r[i]);
+            for (int i = 0; i < VPT; ++i) {
+                gt[i] *= 1.f + m[i];
+                y[i] *= q;
             }
+            v[0] = 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) r[i] = fmaf(gt[i], y[i], a.alpha * r[i]);
+        if (a.r) st_row<T, VPT>((T*)a.r + row * h, h, r);
+    } else {
+        clear_area(area);
     }
     float mu = 0.f;
     if (a.layer) {
-        float v[1] = {0.f};
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[0] += r[i][e];
-        block_sum<1>(v, area, buf);
+        for (int i = 0; i < VPT; ++i) v[0] += r[i];
+        block_sum<MAXT, 1>(v, area, half);
         mu = v[0] * inv_h;
+        v[0] = 0.f;
     }
-    float v[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-        if (threadIdx.x + i * blockDim.x < nvec)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[0] = fmaf(r[i][e] - mu, r[i][e] - mu, v[0]);
-    block_sum<1>(v, area, buf);
-    const float s = 1.f / sqrtf(v[0] * inv_h + a.eps);
+        if (threadIdx.x + i * blockDim.x < h) v[0] = fmaf(r[i] - mu, r[i] - mu, v[0]);
+    float w[VPT], sh[VPT];
+    ld_mods<VPT>(a.scale, a.mod_f32, b * a.scale_sample, h, m);
+    ld_mods<VPT>(a.shift, a.mod_f32, b * a.shift_sample, h, sh);
+    if (a.weight) ld_row<float, VPT>(a.weight, h, w);
+    block_sum<MAXT, 1>(v, area, half);
+    const float s = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
     if (threadIdx.x == 0 && a.rstd) {
         a.rstd[row] = s;
         if (a.layer) a.mean[row] = mu;
     }
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int c = threadIdx.x + i * blockDim.x;
-        if (c < nvec) {
-            float sh[VEC], sc[VEC], w[VEC];
-            ld_mod<VEC>(a.shift, a.mod_f32, b * a.shift_sample + c * VEC, sh);
-            ld_mod<VEC>(a.scale, a.mod_f32, b * a.scale_sample + c * VEC, sc);
-            if (a.weight) ld_mod<VEC>(a.weight, 1, c * VEC, w);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float o = (r[i][e] - mu) * s;
-                if (a.weight) o *= 1.f + w[e];
-                sh[e] = fmaf(o, 1.f + sc[e], sh[e]);
-            }
-            Io<T, VEC>::st((T*)a.z + row * h + c * VEC, sh);
-        }
-    }
+    for (int i = 0; i < VPT; ++i) r[i] = fmaf((r[i] - mu) * s * (a.weight ? 1.f + w[i] : 1.f), 1.f + m[i], sh[i]);
+    st_row<T, VPT>((T*)a.z + row * h, h, r);
 }
 
-// One block per chunk of consecutive rows of one sample; thread t owns fixed columns, so that S, T and G
-// stay in registers over the chunk and leave as one partial row each.
-template <typename T, int VEC, int VPT>
-__global__ void __launch_bounds__(512) resnorm_bwd_kernel(const Args a, const lq_residual_norm_grads g, int chunks,
-                                                          int64_t rows_per_chunk, float* __restrict__ part) {
-    __shared__ float area[2][kMaxWarps][2];
-    int buf = 0;
-    const int64_t b = blockIdx.x / chunks;
-    const int chunk = (int)(blockIdx.x - b * chunks);
-    const int64_t t0 = chunk * rows_per_chunk, t1 = min(a.tokens, t0 + rows_per_chunk);
-    const int h = (int)a.h, nvec = h / VEC;
+template <typename T, int VPT>
+__global__ void __launch_bounds__(512) resnorm_bwd_kernel(const Args a, const lq_residual_norm_grads g, int chunks, int64_t per,
+                                                          float* __restrict__ part) {
+    constexpr int MAXT = 512;
+    __shared__ __align__(16) float area[2][2][kMaxWarps];
+    int half = 0;
+    const Rows rows(a.tokens, chunks, per);
+    const int64_t b = rows.b;
+    const int h = (int)a.h;
     const float inv_h = 1.f / (float)h;
-    float S[VPT][VEC], D1[VPT][VEC], G[VPT][VEC];
+    float S[VPT], D1[VPT], G[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) S[i][e] = D1[i][e] = G[i][e] = 0.f;
-
-    for (int64_t t = t0; t < t1; ++t) {
+    for (int i = 0; i < VPT; ++i) S[i] = D1[i] = G[i] = 0.f;
+    clear_area(area);
+    for (int64_t t = rows.t0; t < rows.t1; ++t) {
         const int64_t row = b * a.tokens + t;
+        float rh[VPT], gz[VPT], yh[VPT], d[VPT], m[VPT];
+        ld_row<T, VPT>((const T*)a.x + b * a.x_sample + t * a.x_token, h, rh);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) gz[i] = yh[i] = d[i] = 0.f;
+        if (g.dz) ld_row<T, VPT>((const T*)g.dz + b * g.dz_sample + t * g.dz_token, h, gz);
+        if (a.y) ld_row<T, VPT>((const T*)a.y + b * a.y_sample + t * a.y_token, h, yh);
+        if (g.dr) ld_row<T, VPT>((const T*)g.dr + b * g.dr_sample + t * g.dr_token, h, d);
         const float s = a.rstd[row], mu = a.layer ? a.mean[row] : 0.f, q = a.post_weight ? a.post_rstd[row] : 1.f;
-        float rh[VPT][VEC], gz[VPT][VEC], yh[VPT][VEC];
-        float v[2] = {0.f, 0.f};
+        if (a.y) {
+            ld_mods<VPT>(a.gate, a.mod_f32, b * a.gate_sample, h, m);
+            if (a.post_weight) {
+                float pw[VPT];
+                ld_row<float, VPT>(a.post_weight, h, pw);
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) rh[i][e] = gz[i][e] = yh[i][e] = 0.f;
-            if (c >= nvec) continue;
-            Io<T, VEC>::ld((const T*)a.x + b * a.x_sample + t * a.x_token + c * VEC, rh[i]);
-            if (g.dz) Io<T, VEC>::ld((const T*)g.dz + b * g.dz_sample + t * g.dz_token + c * VEC, gz[i]);
-            if (a.y) {
-                float gt[VEC], pw[VEC];
-                Io<T, VEC>::ld((const T*)a.y + b * a.y_sample + t * a.y_token + c * VEC, yh[i]);
-                ld_mod<VEC>(a.gate, a.mod_f32, b * a.gate_sample + c * VEC, gt);
-                if (a.post_weight) ld_mod<VEC>(a.post_weight, 1, c * VEC, pw);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float u = yh[i][e];
-                    if (a.post_weight) {
-                        yh[i][e] *= q;
-                        u = yh[i][e] * (1.f + pw[e]);
-                    }
-                    rh[i][e] = fmaf(gt[e], u, a.alpha * rh[i][e]);
+                for (int i = 0; i < VPT; ++i) {
+                    m[i] *= 1.f + pw[i];
+                    yh[i] *= q;
                 }
             }
-            float sc[VEC], w[VEC];
-            ld_mod<VEC>(a.scale, a.mod_f32, b * a.scale_sample + c * VEC, sc);
-            if (a.weight) ld_mod<VEC>(a.weight, 1, c * VEC, w);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                rh[i][e] = (rh[i][e] - mu) * s;
-                S[i][e] = fmaf(gz[i][e], rh[i][e], S[i][e]);
-                D1[i][e] += gz[i][e];
-                gz[i][e] *= 1.f + sc[e];
-                if (a.weight) gz[i][e] *= 1.f + w[e];
-                v[0] = fmaf(gz[i][e], rh[i][e], v[0]);
-                v[1] += gz[i][e];
-            }
+            for (int i = 0; i < VPT; ++i) rh[i] = fmaf(m[i], yh[i], a.alpha * rh[i]);
         }
-        block_sum<2>(v, area, buf);
+        float v[2] = {0.f, 0.f}, mul[VPT];
+        ld_mods<VPT>(a.scale, a.mod_f32, b * a.scale_sample, h, mul);
+        if (a.weight) {
+            float w[VPT];
+            ld_row<float, VPT>(a.weight, h, w);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) mul[i] = (1.f + mul[i]) * (1.f + w[i]) - 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            rh[i] = (rh[i] - mu) * s;  // gz is zero behind the row
+            S[i] = fmaf(gz[i], rh[i], S[i]);
+            D1[i] += gz[i];
+            gz[i] = fmaf(gz[i], mul[i], gz[i]);
+            v[0] = fmaf(gz[i], rh[i], v[0]);
+            v[1] += gz[i];
+        }
+        block_sum<MAXT, 2>(v, area, half);
         const float c1 = v[0] * inv_h, c0 = a.layer ? v[1] * inv_h : 0.f;
         float p[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-            if (c >= nvec) continue;
-            float d[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d[e] = 0.f;
-            if (g.dr) Io<T, VEC>::ld((const T*)g.dr + b * g.dr_sample + t * g.dr_token + c * VEC, d);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d[e] = fmaf(s, gz[i][e] - c0 - rh[i][e] * c1, d[e]);
+            d[i] = fmaf(s, gz[i] - c0 - rh[i] * c1, d[i]);
             if (a.y) {
-                float gt[VEC], pw[VEC];
-                ld_mod<VEC>(a.gate, a.mod_f32, b * a.gate_sample + c * VEC, gt);
-                if (a.post_weight) ld_mod<VEC>(a.post_weight, 1, c * VEC, pw);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    G[i][e] = fmaf(d[e], yh[i][e], G[i][e]);
-                    gz[i][e] = gt[e] * d[e];  // du
-                    if (a.post_weight) {
-                        gz[i][e] *= 1.f + pw[e];
-                        p[0] = fmaf(gz[i][e], yh[i][e], p[0]);
-                    }
-                    d[e] *= a.alpha;
-                }
+                G[i] = fmaf(d[i], yh[i], G[i]);
+                gz[i] = m[i] * d[i];
+                p[0] = fmaf(gz[i], yh[i], p[0]);  // yh is zero behind the row
+                d[i] *= a.alpha;
             }
-            if (g.dx) Io<T, VEC>::st((T*)g.dx + row * h + c * VEC, d);
         }
+        if (g.dx) st_row<T, VPT>((T*)g.dx + row * h, h, d);
         if (!a.y || !g.dy) continue;
-        if (a.post_weight) block_sum<1>(p, area, buf);
-        const float pm = p[0] * inv_h;
+        if (a.post_weight) {
+            block_sum<MAXT, 1>(p, area, half);
+            const float pm = p[0] * inv_h;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int c = threadIdx.x + i * blockDim.x;
-            if (c >= nvec) continue;
-            if (a.post_weight)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) gz[i][e] = q * (gz[i][e] - yh[i][e] * pm);
-            Io<T, VEC>::st((T*)g.dy + row * h + c * VEC, gz[i]);
+            for (int i = 0; i < VPT; ++i) gz[i] = q * (gz[i] - yh[i] * pm);
         }
+        st_row<T, VPT>((T*)g.dy + row * h, h, gz);
     }
     if (!part) return;
     float* dst = part + (int64_t)blockIdx.x * 3 * h;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int c = threadIdx.x + i * blockDim.x;
-        if (c >= nvec) continue;
-        Io<float, VEC == 1 ? 1 : 4> io;
-#pragma unroll
-        for (int e = 0; e < VEC; e += (VEC == 1 ? 1 : 4)) {
-            typedef float Q[VEC == 1 ? 1 : 4];
-            io.st(dst + c * VEC + e, *(const Q*)&S[i][e]);
-            io.st(dst + h + c * VEC + e, *(const Q*)&D1[i][e]);
-            io.st(dst + 2 * h + c * VEC + e, *(const Q*)&G[i][e]);
-        }
-    }
+    st_row<float, VPT>(dst, h, S);
+    st_row<float, VPT>(dst + h, h, D1);
+    st_row<float, VPT>(dst + 2 * h, h, G);
 }
 
 __device__ __forceinline__ void st_mod(void* p, int f32, int64_t i, float v) {
@@ -348,67 +606,50 @@ __device__ __forceinline__ void st_mod(void* p, int f32, int64_t i, float v) {
     else ((__nv_bfloat16*)p)[i] = __float2bfloat16(v);
 }
 
-// Sums the partial rows in a fixed order.  Block = 32 columns x 8 ranges of chunks; one sample per blockIdx.y,
-// or (gridDim.y == 1) all samples one after the other when a norm weight's gradient sums over them too.
-__global__ void __launch_bounds__(256) resnorm_final_kernel(const Args a, const lq_residual_norm_grads g, int chunks,
-                                                            const float* __restrict__ part) {
-    __shared__ float sm[3][8][33];
+// Sums the partial rows in a fixed order.  Block = 32 columns x 32 ranges of chunks.  blockIdx.y < samples: the sums of
+// that sample (dgate, dshift, dscale); blockIdx.y == samples: the norm weights' gradients, over all samples.
+__global__ void __launch_bounds__(1024) resnorm_final_kernel(const Args a, const lq_residual_norm_grads g, int chunks,
+                                                             const float* __restrict__ part) {
+    __shared__ float sm[3][32][33];
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, h = (int)a.h;
     const int j = blockIdx.x * 32 + lane;
-    float dw = 0.f, dpw = 0.f;
-    for (int64_t b = blockIdx.y; b < a.samples; b += gridDim.y) {
-        float s[3] = {0.f, 0.f, 0.f};
-        if (j < h)
-            for (int c = grp; c < chunks; c += 8)
+    const bool weights = blockIdx.y == a.samples;
+    const int64_t b = blockIdx.y;
+    float s[3] = {0.f, 0.f, 0.f};
+    if (j < h) {
+        if (!weights) {
+            for (int c = grp; c < chunks; c += 32)
 #pragma unroll
                 for (int k = 0; k < 3; ++k) s[k] += part[((b * chunks + c) * 3 + k) * h + j];
-        __syncthreads();  // the sums of the sample before have been read
-#pragma unroll
-        for (int k = 0; k < 3; ++k) sm[k][grp][lane] = s[k];
-        __syncthreads();
-        if (grp == 0 && j < h) {
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                s[k] = 0.f;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) s[k] += sm[k][q][lane];
+        } else {
+            for (int64_t c = grp; c < a.samples * chunks; c += 32) {
+                const int64_t bc = c / chunks;
+                s[0] = fmaf(part[c * 3 * h + j], 1.f + mod_at(a.scale, a.mod_f32, bc * a.scale_sample + j), s[0]);
+                if (a.y) s[2] = fmaf(part[(c * 3 + 2) * h + j], mod_at(a.gate, a.mod_f32, bc * a.gate_sample + j), s[2]);
             }
-            float sc[1], gt[1] = {0.f}, w = 0.f, pw = 0.f;
-            ld_mod<1>(a.scale, a.mod_f32, b * a.scale_sample + j, sc);
-            if (a.y) ld_mod<1>(a.gate, a.mod_f32, b * a.gate_sample + j, gt);
-            if (a.weight) w = a.weight[j];
-            if (a.post_weight) pw = a.post_weight[j];
-            if (g.dscale) st_mod(g.dscale, a.mod_f32, b * h + j, s[0] * (1.f + w));
-            if (g.dshift) st_mod(g.dshift, a.mod_f32, b * h + j, s[1]);
-            if (g.dgate) st_mod(g.dgate, a.mod_f32, b * h + j, s[2] * (1.f + pw));
-            dw = fmaf(s[0], 1.f + sc[0], dw);
-            dpw = fmaf(s[2], gt[0], dpw);
         }
     }
-    if (grp == 0 && j < h) {
-        if (g.dweight) g.dweight[j] = dw;
-        if (g.dpost_weight) g.dpost_weight[j] = dpw;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sm[k][grp][lane] = s[k];
+    __syncthreads();
+    if (grp >= 3 || j >= h) return;
+    float v = 0.f;  // warp k adds up sum k
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v += sm[grp][q][lane];
+    if (weights) {
+        if (grp == 0 && g.dweight) g.dweight[j] = v;
+        if (grp == 2 && g.dpost_weight) g.dpost_weight[j] = v;
+        return;
     }
+    if (grp == 0 && g.dscale) st_mod(g.dscale, a.mod_f32, b * h + j, v * (a.weight ? 1.f + a.weight[j] : 1.f));
+    if (grp == 1 && g.dshift) st_mod(g.dshift, a.mod_f32, b * h + j, v);
+    if (grp == 2 && g.dgate) st_mod(g.dgate, a.mod_f32, b * h + j, v * (a.post_weight ? 1.f + a.post_weight[j] : 1.f));
 }
 
 // ---- host ---------------------------------------------------------------------------------------
 
 constexpr int64_t kMaxH = 16384;  // 512 threads x 32 elements
-
-struct Shape {
-    int vec, ept, threads;  // elements per access, elements per thread, threads of a block
-};
-
-// 16-byte accesses need every row and vector to start on 16 bytes; otherwise single elements.  A thread holds
-// 8 elements up to 4096 columns, then 16, then 32, in blocks of at most 512 threads (128 registers each).
-Shape shape_of(int64_t h, int dtype, bool vectors) {
-    Shape s;
-    s.vec = vectors ? (dtype == LQ_F32 ? 4 : 8) : 1;
-    s.ept = h <= 4096 ? 8 : (h <= 8192 ? 16 : 32);
-    const int64_t per = (h / s.vec + s.ept / s.vec - 1) / (s.ept / s.vec);
-    s.threads = (int)((per + 31) / 32 * 32);
-    return s;
-}
+constexpr size_t kRingBytes = 216 * 1024;  // shared memory of an SM for the rings of its blocks
 
 inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -428,11 +669,25 @@ bool vectors_ok(const Args& a, const lq_residual_norm_grads* g) {
     return ok;
 }
 
-// Chunks of one sample: about as many blocks as fit the machine at 1024 threads an SM, each with at least one row.
+// Blocks of an SM by threads per block (8 columns each): what the launch bounds below leave registers for.
+int blocks_per_sm(int64_t h) {
+    const int64_t threads = (h + 255) / 256 * 32;
+    return threads <= 128 ? 6 : (threads <= 256 ? 3 : (threads <= 384 ? 2 : 1));
+}
+
+// Chunks of one sample: one block each, as many as the SMs hold at once, but four rows or more each where that
+// still gives every SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
 int chunks_of(int64_t samples, int64_t tokens, int64_t h, int sms) {
-    const int64_t threads = (h / 8 + 31) / 32 * 32;  // of the vector path up to 4096 columns; the rule only has to be fixed
-    const int64_t blocks = (int64_t)sms * std::max<int64_t>(1, 1024 / std::min<int64_t>(512, std::max<int64_t>(32, threads)));
-    return (int)std::max<int64_t>(1, std::min<int64_t>(tokens, (blocks + samples - 1) / samples));
+    const int64_t fill = ((int64_t)sms * blocks_per_sm(h) + samples - 1) / samples;
+    const int64_t one = (sms + samples - 1) / samples;
+    return (int)std::max<int64_t>(1, std::min(std::min(tokens, fill), std::max(tokens / 4, one)));
+}
+
+// Rows in the ring of a block, 0 when fewer than two fit.
+int stages_of(int64_t h, int dtype, int inputs) {
+    const size_t stage = (size_t)inputs * h * (dtype == LQ_F32 ? 4 : 2);
+    const size_t n = kRingBytes / blocks_per_sm(h) / stage;
+    return n < 2 ? 0 : (int)std::min<size_t>(n, kMaxStages);
 }
 
 void check(const Args& a) {
@@ -464,35 +719,87 @@ int guarded_call(F&& f) {
     }
 }
 
-int current_sms() {
+int current_device() {
     int dev = 0;
     LQ_CUDA(cudaGetDevice(&dev));
-    return lq_tc_sm_count(dev);
+    return dev;
 }
 
-template <typename T, int VEC, int EPT>
-void launch_fwd(const Args& a, const Shape& s, cudaStream_t st) {
-    resnorm_fwd_kernel<T, VEC, EPT / VEC><<<(unsigned)(a.samples * a.tokens), s.threads, 0, st>>>(a);
+template <typename K, typename... A>
+void launch_ring(K kern, unsigned grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    LQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kern<<<grid, threads, smem, st>>>(args...);
 }
-template <typename T, int VEC, int EPT>
-void launch_bwd(const Args& a, const lq_residual_norm_grads& g, const Shape& s, int chunks, float* part, cudaStream_t st) {
+
+#define LQ_RING_BOUNDS(KERN, T, P, Y, ...)                                                        \
+    do {                                                                                         \
+        if (threads <= 128) launch_ring(KERN<T, P, Y, 128, 6>, grid, threads, smem, st, __VA_ARGS__);      \
+        else if (threads <= 256) launch_ring(KERN<T, P, Y, 256, 3>, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 384) launch_ring(KERN<T, P, Y, 384, 2>, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 512) launch_ring(KERN<T, P, Y, 512, 1>, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 768) launch_ring(KERN<T, P, Y, 768, 1>, grid, threads, smem, st, __VA_ARGS__); \
+        else launch_ring(KERN<T, P, Y, 1024, 1>, grid, threads, smem, st, __VA_ARGS__);                    \
+    } while (0)
+#define LQ_RING(KERN, T, ...)                                                          \
+    do {                                                                              \
+        if (a.post_weight && a.layer) LQ_RING_BOUNDS(KERN, T, true, true, __VA_ARGS__); \
+        else if (a.post_weight) LQ_RING_BOUNDS(KERN, T, true, false, __VA_ARGS__);      \
+        else if (a.layer) LQ_RING_BOUNDS(KERN, T, false, true, __VA_ARGS__);            \
+        else LQ_RING_BOUNDS(KERN, T, false, false, __VA_ARGS__);                        \
+    } while (0)
+// 8 elements a thread up to 4096 columns, then 16, then 32: blocks of at most 512 threads, 128 registers each
+#define LQ_SCALAR(KERN, ...)                                                                                                        \
+    do {                                                                                                                           \
+        const int ept = a.h <= 4096 ? 8 : (a.h <= 8192 ? 16 : 32);                                                                  \
+        const int threads = (int)(((a.h + ept - 1) / ept + 31) / 32 * 32);                                                          \
+        if (a.dtype == LQ_F32) {                                                                                                    \
+            if (ept == 8) KERN<float, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);                                                    \
+            else if (ept == 16) KERN<float, 16><<<grid, threads, 0, st>>>(__VA_ARGS__);                                             \
+            else KERN<float, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);                                                            \
+        } else {                                                                                                                    \
+            if (ept == 8) KERN<__nv_bfloat16, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);                                            \
+            else if (ept == 16) KERN<__nv_bfloat16, 16><<<grid, threads, 0, st>>>(__VA_ARGS__);                                     \
+            else KERN<__nv_bfloat16, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);                                                    \
+        }                                                                                                                           \
+    } while (0)
+
+constexpr int64_t kRingMaxH = 8192;  // 1024 threads x 8 columns
+
+void forward(const Args& a, int dev, cudaStream_t st) {
+    const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype, inputs) : 0;
+    LqProf prof(LQ_K_PREP, st);
+    if (stages) {
+        const int chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev)), threads = (int)((a.h + 255) / 256 * 32);
+        const int64_t per = (a.tokens + chunks - 1) / chunks;
+        const unsigned grid = (unsigned)(a.samples * chunks);
+        const size_t smem = (size_t)std::min<int64_t>(stages, per) * inputs * a.h * (a.dtype == LQ_F32 ? 4 : 2);
+        int* status = lq_tc_status_word(dev);
+        if (a.dtype == LQ_F32) LQ_RING(resnorm_fwd_ring_kernel, float, a, chunks, per, stages, status);
+        else LQ_RING(resnorm_fwd_ring_kernel, __nv_bfloat16, a, chunks, per, stages, status);
+    } else {
+        const unsigned grid = (unsigned)(a.samples * a.tokens);
+        LQ_SCALAR(resnorm_fwd_kernel, a);
+    }
+    LQ_CUDA(cudaGetLastError());
+}
+
+void backward(const Args& a, const lq_residual_norm_grads& g, int chunks, float* part, int dev, cudaStream_t st) {
+    const int inputs = 1 + (a.y ? 1 : 0) + (g.dz ? 1 : 0) + (g.dr ? 1 : 0);
+    const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype, inputs) : 0;
     const int64_t per = (a.tokens + chunks - 1) / chunks;
-    resnorm_bwd_kernel<T, VEC, EPT / VEC><<<(unsigned)(a.samples * chunks), s.threads, 0, st>>>(a, g, chunks, per, part);
+    const unsigned grid = (unsigned)(a.samples * chunks);
+    LqProf prof(LQ_K_PREP, st);
+    if (stages) {
+        const int threads = (int)((a.h + 255) / 256 * 32);
+        const size_t smem = (size_t)std::min<int64_t>(stages, per) * inputs * a.h * (a.dtype == LQ_F32 ? 4 : 2);
+        int* status = lq_tc_status_word(dev);
+        if (a.dtype == LQ_F32) LQ_RING(resnorm_bwd_ring_kernel, float, a, g, chunks, per, stages, part, status);
+        else LQ_RING(resnorm_bwd_ring_kernel, __nv_bfloat16, a, g, chunks, per, stages, part, status);
+    } else {
+        LQ_SCALAR(resnorm_bwd_kernel, a, g, chunks, per, part);
+    }
+    LQ_CUDA(cudaGetLastError());
 }
-
-#define LQ_RESNORM_EPT(F, T, V, ...)                                             \
-    do {                                                                         \
-        if (s.ept == 8) F<T, V, 8>(__VA_ARGS__);                                 \
-        else if (s.ept == 16) F<T, V, 16>(__VA_ARGS__);                          \
-        else F<T, V, 32>(__VA_ARGS__);                                           \
-    } while (0)
-#define LQ_RESNORM_DISPATCH(F, ...)                                              \
-    do {                                                                         \
-        if (a.dtype == LQ_F32 && s.vec == 4) LQ_RESNORM_EPT(F, float, 4, __VA_ARGS__);          \
-        else if (a.dtype == LQ_F32) LQ_RESNORM_EPT(F, float, 1, __VA_ARGS__);                   \
-        else if (s.vec == 8) LQ_RESNORM_EPT(F, __nv_bfloat16, 8, __VA_ARGS__);                  \
-        else LQ_RESNORM_EPT(F, __nv_bfloat16, 1, __VA_ARGS__);                                  \
-    } while (0)
 
 }  // namespace
 
@@ -508,18 +815,14 @@ int lq_residual_norm_fwd(const lq_residual_norm_args* args, void* stream) {
         LQ_CHECK_ARG(a.z != nullptr, "NULL argument");
         LQ_CHECK_ARG(!a.rstd || !a.layer || a.mean, "mean must be given with rstd for the layer norm");
         LQ_CHECK_ARG(!a.rstd || !a.post_weight || a.post_rstd, "post_rstd must be given with rstd and post_weight");
-        cudaStream_t st = (cudaStream_t)stream;
-        const Shape s = shape_of(a.h, a.dtype, vectors_ok(a, nullptr));
-        LqProf prof(LQ_K_PREP, st);
-        LQ_RESNORM_DISPATCH(launch_fwd, a, s, st);
-        LQ_CUDA(cudaGetLastError());
+        forward(a, current_device(), (cudaStream_t)stream);
     });
 }
 
 size_t lq_residual_norm_workspace_bytes(int64_t samples, int64_t tokens, int64_t h) {
     if (samples < 1 || tokens < 1 || h < 1 || h > kMaxH) return 0;
     size_t n = 0;
-    if (guarded_call([&] { n = (size_t)samples * chunks_of(samples, tokens, h, current_sms()) * 3 * h * sizeof(float); }) != LQ_OK)
+    if (guarded_call([&] { n = (size_t)samples * chunks_of(samples, tokens, h, lq_tc_sm_count(current_device())) * 3 * h * sizeof(float); }) != LQ_OK)
         return 0;
     return n;
 }
@@ -546,23 +849,18 @@ int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_no
         LQ_CHECK_ARG(!g.dpost_weight || a.post_weight, "dpost_weight needs post_weight");
         LQ_CHECK_ARG(!g.dweight || a.weight, "dweight needs weight");
         LQ_CHECK_ARG(a.rstd && (!a.layer || a.mean) && (!a.post_weight || a.post_rstd), "the forward's statistics are needed");
-        const int chunks = chunks_of(a.samples, a.tokens, a.h, current_sms());
+        const int dev = current_device(), chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev));
         LQ_CHECK_ARG(a.samples * chunks < (int64_t)1 << 31, "too many samples");
         if (sums && (!ws || ws_bytes < (size_t)a.samples * chunks * 3 * a.h * sizeof(float)))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the residual-norm backward");
         LQ_CHECK_ARG(!sums || al16(ws), "the workspace must be 16-byte aligned");
-        const Shape s = shape_of(a.h, a.dtype, vectors_ok(a, &g));
+        LQ_CHECK_ARG(!sums || a.samples < 65535, "at most 65534 samples with gradients of the vectors");
         float* part = sums ? (float*)ws : nullptr;
-        {
-            LqProf prof(LQ_K_PREP, st);
-            LQ_RESNORM_DISPATCH(launch_bwd, a, g, s, chunks, part, st);
-            LQ_CUDA(cudaGetLastError());
-        }
+        backward(a, g, chunks, part, dev, st);
         if (sums) {
             LqProf prof(LQ_K_REDUCE, st);
-            const bool over_samples = g.dweight || g.dpost_weight;
-            const dim3 grid((unsigned)((a.h + 31) / 32), over_samples ? 1u : (unsigned)std::min<int64_t>(a.samples, 65535));
-            resnorm_final_kernel<<<grid, 256, 0, st>>>(a, g, chunks, part);
+            const dim3 grid((unsigned)((a.h + 31) / 32), (unsigned)(a.samples + (g.dweight || g.dpost_weight ? 1 : 0)));
+            resnorm_final_kernel<<<grid, 1024, 0, st>>>(a, g, chunks, part);
             LQ_CUDA(cudaGetLastError());
         }
     });
