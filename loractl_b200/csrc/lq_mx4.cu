@@ -17,6 +17,7 @@
 // The product Y[n, m] = sum_k X[n, k] W[m, k] (+ bias) multiplies codes and scales where they lie: nothing is
 // dequantised (tcgen05.mma kind::mxf4.block_scale, f32 accumulators).
 #include <algorithm>
+#include <mutex>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -400,6 +401,228 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
     }
 }
 
+// ---- many tokens: pairs of SMs ---------------------------------------------------------------------
+// D tiles of 256 tokens x 256 outputs on a cluster of two CTAs (cta_group::2): each stages its own 128 token rows and
+// HALF of the 256 weight rows, so an SM reads and writes 64 KB of shared memory per 16.8 MFLOP k-block instead of the 96 KB
+// of a tile of its own; the scales of its rows and of all 256 columns go to its own tensor memory, into the columns of
+// the stage they came with, so that a stage's release covers them.  The accumulator has one buffer (256 columns; two
+// would leave no room for scales): the epilogue empties it into registers at once and converts and stores
+// while the next tile's products run.
+struct Cfg2 {
+    static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = 128 * 128, SA_BYTES = 2 * kTile, SB_BYTES = 4 * kTile;
+    static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
+    static constexpr int STAGES = 5;
+    static constexpr uint32_t TMEM = 512, SCALE_COL = 256;
+    static_assert(SCALE_COL + 24 * STAGES <= 512, "tensor memory");
+    static constexpr uint32_t OUT = 8 * 2048;  // per epilogue warp: 32 rows x 32 bf16 (or 16 f32) columns
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE + OUT + 1024 + 256;
+};
+constexpr int kThreads2 = 320;  // TMA warp, MMA warp, eight epilogue warps
+constexpr int kGroupM = 8;      // token tiles per raster group
+
+__device__ __forceinline__ void mma2_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// A scale tile of each CTA's shared memory (the same offset in both) to its own tensor memory.
+__device__ __forceinline__ void cp2_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void tile2(const ProductParams& p, int item, int& xt, int& wt) {
+    const int per = kGroupM * p.w_tiles, g = item / per, first = g * kGroupM;
+    const int rows = min(kGroupM, p.x_tiles - first), r = item - g * per;
+    xt = first + r % rows;
+    wt = r / rows;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
+mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmXs,
+                const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmY, ProductParams p, int tma_store) {
+    using C = Cfg2;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem_a = smem;
+    uint8_t* smem_b = smem_a + (size_t)STAGES * C::A_BYTES;
+    uint8_t* smem_sa = smem_b + (size_t)STAGES * C::B_BYTES;
+    uint8_t* smem_sb = smem_sa + (size_t)STAGES * C::SA_BYTES;
+    uint8_t* stage_out = smem_sb + (size_t)STAGES * C::SB_BYTES;
+    uint64_t* bars = (uint64_t*)(stage_out + C::OUT);
+    uint64_t* full = bars;            // leader's: the bytes of both CTAs' copies
+    uint64_t* empty = bars + STAGES;  // in both, from the leader's multicast commit
+    uint64_t* tfull = bars + 2 * STAGES;
+    uint64_t* tempty = tfull + 1;     // leader's: the epilogue threads of both CTAs
+    uint32_t* tmem_slot = (uint32_t*)(tempty + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        mbar_init(smem_u32(tfull), 1);
+        mbar_init(smem_u32(tempty), 512);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmX);
+        prefetch_tmap(&tmW);
+        prefetch_tmap(&tmXs);
+        prefetch_tmap(&tmWs);
+    }
+    if (warp == 1) {
+        tmem_alloc2(smem_u32(tmem_slot), C::TMEM);
+        tmem_relinquish2();
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int items = p.x_tiles * p.w_tiles, cid = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            lqstream::pdl_wait();  // x is the output of the launch before
+            for (int item = cid; ok && item < items; item += pairs) {
+                int xt, wt;
+                tile2(p, item, xt, wt);
+                for (int kb = 0; kb < p.kb; ++kb) {
+                    if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 75)) { ok = false; break; }
+                    const uint32_t bar = smem_u32(&full[s]);
+                    if (leader) mbar_expect_tx(bar, 2 * C::STAGE);
+                    tma_load_2d_pair(smem_u32(smem_a + (size_t)s * C::A_BYTES), &tmX, bar, kb * 128, xt * 256 + (int)rank * 128);
+                    tma_load_2d_pair(smem_u32(smem_b + (size_t)s * C::B_BYTES), &tmW, bar, kb * 128, wt * 256 + (int)rank * 128);
+                    tma_load_2d_pair(smem_u32(smem_sa + (size_t)s * C::SA_BYTES), &tmXs, bar, kb * 256, xt * 2 + (int)rank);
+                    tma_load_2d_pair(smem_u32(smem_sb + (size_t)s * C::SB_BYTES), &tmWs, bar, kb * 256, wt * 2);
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok)
+                for (int i = 0; i < 64; ++i) __nanosleep(1000);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            const uint32_t d_hi = desc_hi(1024);
+            int s = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int item = cid; ok && item < items; item += pairs) {
+                if (!mbar_wait(smem_u32(tempty), acc_phase ^ 1u, abort_flag, p.status, 76)) { ok = false; break; }
+                acc_phase ^= 1u;
+                tc_fence_after();
+                for (int kb = 0; kb < p.kb; ++kb) {
+                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 77)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem_sa + (size_t)s * C::SA_BYTES), sb = smem_u32(smem_sb + (size_t)s * C::SB_BYTES);
+                    const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 24, sfb = sfa + 8;
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j) {  // tiles of 128 elements; B's rows 0-127 and 128-255
+                        cp2_scales(sfa + 4 * j, scale_desc(sa + j * kTile));
+                        cp2_scales(sfb + 8 * j, scale_desc(sb + j * kTile));
+                        cp2_scales(sfb + 8 * j + 4, scale_desc(sb + (2 + j) * kTile));
+                    }
+                    const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
+                    const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        mma2_mxf4(tmem, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi), idesc_mxf4(256, 256, k & 1),
+                                  sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
+                    mma2_commit_mc(smem_u32(&empty[s]), 3);
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                mma2_commit_mc(smem_u32(tfull), 3);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, chalf = (warp - 2) >> 2;
+        uint8_t* mine = stage_out + (warp - 2) * 2048;
+        uint32_t acc_phase = 0;
+        for (int item = cid; item < items; item += pairs) {
+            int xt, wt;
+            tile2(p, item, xt, wt);
+            if (!mbar_wait(smem_u32(tfull), acc_phase, abort_flag, p.status, 78)) break;
+            acc_phase ^= 1u;
+            tc_fence_after();
+            uint32_t r[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                tmem_ld_x32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(chalf * 128 + c * 32), r[c]);
+            tmem_ld_wait();
+            tc_fence_before();
+            if (leader) mbar_arrive(smem_u32(tempty));
+            else mbar_arrive_leader(smem_u32(tempty));
+            const int row0 = xt * 256 + (int)rank * 128 + quarter * 32, col0 = wt * 256 + chalf * 128;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int col = col0 + c * 32;
+                if (p.bias) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (col + j < p.m) r[c][j] = __float_as_uint(__uint_as_float(r[c][j]) + __ldg(p.bias + col + j));
+                }
+                if (tma_store) {
+                    if (lane == 0) bulk_wait_read0();
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[c][8 * q + 2 * e]), __uint_as_float(r[c][8 * q + 2 * e + 1]));
+                            w[e] = *(const uint32_t*)&h;
+                        }
+                        *(uint4*)(mine + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmY, smem_u32(mine), col, row0);
+                        bulk_commit();
+                    }
+                } else {  // f32, or rows that do not start on 16 bytes: turned in shared memory, 16 columns at a time
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        float* t = (float*)mine;
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) t[lane * 16 + ((j + lane) & 15)] = __uint_as_float(r[c][hf * 16 + j]);
+                        __syncwarp();
+                        const int j = lane & 15, cj = col + hf * 16 + j;
+#pragma unroll 4
+                        for (int i = lane >> 4; i < 32; i += 2) {
+                            const float v = t[i * 16 + ((j + i) & 15)];
+                            if (row0 + i < p.n && cj < p.m) {
+                                const int64_t o = (int64_t)(row0 + i) * p.m + cj;
+                                if (p.y_f32) ((float*)p.y)[o] = v;
+                                else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(v);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (lane == 0) bulk_wait0();
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc2(tmem, C::TMEM);
+    }
+}
+
 // y = sum of the splits in order + bias.
 __global__ void __launch_bounds__(256) mx4_join_kernel(ProductParams p) {
     lqstream::pdl_wait();
@@ -467,7 +690,11 @@ int splits_of(int64_t tiles, int64_t kb, int sms) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / tiles, kb / 2), 16));
 }
 
+// More than one tile of tokens and of outputs each: pairs of SMs.
+bool use_pair(int64_t n, int64_t m, int sms) { return n > 128 && m > 128 && sms >= 2; }
+
 size_t product_ws(int64_t n, int64_t m, int64_t k, int sms) {
+    if (use_pair(n, m, sms)) return 0;
     const int bn = bn_of(n);
     const int64_t tiles = ((m + 127) / 128) * ((n + bn - 1) / bn);
     const int s = splits_of(tiles, (k + 255) / 256, sms);
@@ -492,6 +719,41 @@ void launch_stream(ProductParams p, const void* w_codes, const void* x_codes, in
         lqstream::launch_pdl(mx4_join_kernel, grid_of(((int64_t)p.n * p.m + 255) / 256, sms, 8), 256, 0, st, p);
         LQ_CUDA(cudaGetLastError());
     }
+}
+
+// Pairs that can be resident at once, asked once per device.
+int resident_pairs(int dev, int sms) {
+    static std::mutex mu;
+    static int known[64] = {};
+    std::lock_guard<std::mutex> lk(mu);
+    if (known[dev & 63] == 0) {
+        LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(sms & ~1);
+        cfg.blockDim = dim3(kThreads2);
+        cfg.dynamicSmemBytes = Cfg2::SMEM;
+        int n = 0;
+        LQ_CUDA(cudaOccupancyMaxActiveClusters(&n, mx4_pair_kernel, &cfg));
+        known[dev & 63] = std::max(1, std::min(n, sms / 2));
+    }
+    return known[dev & 63];
+}
+
+void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int64_t k, int dev, int sms, cudaStream_t st) {
+    const CUtensorMap tx = lq_tc_make_map_u8(x_codes, k / 2, p.n, k / 2, 128);
+    const CUtensorMap tw = lq_tc_make_map_u8(w_codes, k / 2, p.m, k / 2, 128);
+    const CUtensorMap txs = lq_tc_make_map_u32(p.x_scales, k_tiles(k) * (kTile / 4), row_tiles(p.n), 256, 1);
+    const CUtensorMap tws = lq_tc_make_map_u32(p.w_scales, k_tiles(k) * (kTile / 4), row_tiles(p.m), 256, 2);
+    const int tma_store = !p.y_f32 && p.m % 8 == 0 && al16(p.y);
+    const CUtensorMap ty = tma_store ? lq_tc_make_store_map(p.y, p.m, p.n, p.m) : tx;
+    p.x_tiles = (p.n + 255) / 256;
+    p.w_tiles = (p.m + 255) / 256;
+    LQ_CHECK_ARG((int64_t)p.x_tiles * p.w_tiles < (int64_t)1 << 31, "too many tiles");
+    const int pairs = std::min(resident_pairs(dev, sms), p.x_tiles * p.w_tiles);
+    LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
+    LqProf prof(LQ_K_GEMM_MAIN, st);
+    lqstream::launch_pdl(mx4_pair_kernel, dim3(2 * pairs), dim3(kThreads2), Cfg2::SMEM, st, tx, tw, txs, tws, ty, p, tma_store);
+    LQ_CUDA(cudaGetLastError());
 }
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -526,7 +788,8 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
     p.y = y;
     p.y_f32 = y_dtype == LQ_F32;
     p.status = lq_tc_status_word(dev);
-    if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, sms, st);
+    if (use_pair(n, m, sms)) launch_pair(p, w_codes, x_codes, k, dev, sms, st);
+    else if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, sms, st);
     else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, sms, st);
     else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, sms, st);
     else launch_stream<128>(p, w_codes, x_codes, k, sms, st);

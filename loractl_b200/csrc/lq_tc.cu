@@ -725,6 +725,22 @@ CUtensorMap make_map(const void* base, int64_t inner, int64_t rows, int64_t ld, 
     return m;
 }
 
+CUtensorMap make_map_u32(const void* base, int64_t inner, int64_t rows, int box_inner, int box_rows) {
+    if (((uintptr_t)base & 15) != 0 || inner % 4 != 0)
+        throw LqError(LQ_ERR_INVALID, "tensor-core path: rows must start on 16 bytes");
+    CUtensorMap m;
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)inner * 4};
+    cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1u, 1u};
+    CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        throw LqError(LQ_ERR_CUDA, "cuTensorMapEncodeTiled (words) failed with CUresult " + std::to_string((int)r));
+    return m;
+}
+
 // bf16 output [rows, cols] (ld elements between rows): box 32 x 32, 64-byte swizzle, for TMA stores.
 CUtensorMap make_store_map(const void* base, int64_t cols, int64_t rows, int64_t ld) {
     if (((uintptr_t)base & 15) != 0) throw LqError(LQ_ERR_INVALID, "tensor-core path: output must be 16-byte aligned");
@@ -1502,6 +1518,9 @@ int lq_tc_pair_group_m(int sm_count, int block_n, int64_t Ng, int64_t K0, int b_
     static const int forced = [] { const char* e = getenv("LQ_GROUP_M"); return e ? atoi(e) : 0; }();
     if (forced > 0) group_m = forced;
     return group_m;
+}
+CUtensorMap lq_tc_make_map_u32(const void* base, int64_t inner, int64_t rows, int box_inner, int box_rows) {
+    return make_map_u32(base, inner, rows, box_inner, box_rows);
 }
 CUtensorMap lq_tc_make_store_map(const void* base, int64_t cols, int64_t rows, int64_t ld) {
     return make_store_map(base, cols, rows, ld);

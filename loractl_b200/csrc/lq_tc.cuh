@@ -42,6 +42,8 @@ void lq_tc_selftest_wait(int device, unsigned limit_ms, cudaStream_t st);
 CUtensorMap lq_tc_make_map(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_rows);
 // Same for a byte matrix: box 128 bytes x box_rows, 128-byte swizzle.
 CUtensorMap lq_tc_make_map_u8(const void* base, int64_t inner, int64_t rows, int64_t ld, int box_rows);
+// 32-bit words, no swizzle: box box_inner x box_rows (scale tiles of the microscaled product).
+CUtensorMap lq_tc_make_map_u32(const void* base, int64_t inner, int64_t rows, int box_inner, int box_rows);
 // bf16 output [rows, cols]: box 32 x 32, 64-byte swizzle, for the epilogues' TMA tensor stores.
 CUtensorMap lq_tc_make_store_map(const void* base, int64_t cols, int64_t rows, int64_t ld);
 // m-tiles per raster group of a CTA-pair GEMM (see the definition for the rule).
