@@ -9,7 +9,7 @@
 // Storage of [rows, k], k a multiple of 32:
 //   codes   row-major, two elements a byte, the even one in the low nibble: what a TMA tile and the MMA read
 //   scales  tiles of 128 rows x 4 scales (128 elements of k), 512 bytes each: row r, scale s at byte
-//           (r % 32) * 16 + (r / 32) * 4 + s, which is what one 32-lane x 128-bit copy to tensor memory wants;
+//           (r % 32) * 16 + (r / 32) * 4 + s, which is 32 lanes x 4 columns of tensor memory;
 //           tile (rt, kt) at (rt * k_tiles + kt) * 512 with k_tiles even (a k-block of the product is 256
 //           elements = two tiles) and, above 128 rows, an even number of row tiles (its pair of SMs loads 256 rows).
 //           Scales of padding are 0 (2^-127, never NaN: they meet zero codes).
@@ -182,13 +182,12 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
         "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
         : "memory");
 }
-// One scale tile (512 bytes of shared memory, 32 rows of 16) to 4 columns of all four lane quarters.
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// Shared-memory descriptor of a scale tile: no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+// Scales reach tensor memory through four warps of their own: a scale tile is 16 bytes for each of 32 lanes, which is
+// one vector read and one four-column store per warp, and every lane quarter holds the same copy.  The tensor pipe's own
+// copy (tcgen05.cp 32x128b.warpx4) needs no warps, but the products queue behind it: with six such copies per 256-element
+// k-block the pair kernel ran at 4.6 PFLOP/s, without any at 6.2.
+__device__ __forceinline__ void stage_scales(uint32_t taddr, const uint8_t* tile, int lane) {
+    tmem_st_x4(taddr, *(const uint4*)(tile + lane * 16));
 }
 // Instruction descriptor of kind::mxf4: [4,6) which scale pair of B's column word, [7,10) and [10,12) e2m1 = 1,
 // [17,23) N >> 3, [23] scales are e8m0, [24,29) M >> 4, [29,31) which scale pair of A's.
@@ -209,7 +208,7 @@ struct ProductParams {
     int* status;
 };
 
-constexpr int kThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr int kThreads = 320;  // TMA warp, MMA warp, four epilogue warps, four scale warps
 
 template <int BN>
 struct CfgT {
@@ -241,9 +240,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
     uint64_t* bars = (uint64_t*)(smem_s + (size_t)STAGES * 2 * C::S_BYTES);
     uint64_t* full = bars;
     uint64_t* empty = bars + STAGES;
-    uint64_t* tfull = bars + 2 * STAGES;
-    uint64_t* tempty = bars + 2 * STAGES + 2;
-    uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 4);
+    uint64_t* scaled = bars + 2 * STAGES;  // the stage's scales are in tensor memory
+    uint64_t* tfull = bars + 3 * STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint32_t* tmem_slot = (uint32_t*)(tempty + 2);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
+            mbar_init(smem_u32(&scaled[s]), 4);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&tfull[a]), 1);
@@ -333,14 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
                 tc_fence_after();
                 const uint32_t d = tmem + (uint32_t)(acc * C::ACCS * BN);
                 for (int kb = k0; kb < k1; ++kb) {
-                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 73)) { ok = false; break; }
+                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 73) ||
+                        !mbar_wait(smem_u32(&scaled[s]), phase, abort_flag, p.status, 79)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t sc = smem_u32(smem_s + (size_t)s * 2 * C::S_BYTES);
                     const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 16, sfb = sfa + 8;
-                    cp_scales(sfa, scale_desc(sc));
-                    cp_scales(sfa + 4, scale_desc(sc + kTile));
-                    cp_scales(sfb, scale_desc(sc + 2 * kTile));
-                    cp_scales(sfb + 4, scale_desc(sc + 3 * kTile));
                     const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
                     const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
 #pragma unroll
@@ -354,6 +351,27 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
                 if (!ok) break;
                 mma_commit(smem_u32(&tfull[acc]));
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            }
+        }
+    } else if (warp >= 6) {
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SCALE_COL;
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            int wt, xt, z, k0, k1;
+            range(item, wt, xt, z, k0, k1);
+            for (int kb = k0; kb < k1; ++kb) {
+                // the stage was released before its copies began, so its columns are free too
+                if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 80)) { ok = false; break; }
+                const uint8_t* sc = smem_s + (size_t)s * 2 * C::S_BYTES;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) stage_scales(lanes + (uint32_t)(s * 16 + 4 * t), sc + t * kTile, lane);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&scaled[s]));
+                if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
         }
     } else {
@@ -417,7 +435,7 @@ struct Cfg2 {
     static constexpr uint32_t OUT = 8 * 2048;  // per epilogue warp: 32 rows x 32 bf16 (or 16 f32) columns
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + OUT + 1024 + 256;
 };
-constexpr int kThreads2 = 320;  // TMA warp, MMA warp, eight epilogue warps
+constexpr int kThreads2 = 448;  // TMA warp, MMA warp, eight epilogue warps, four scale warps
 constexpr int kGroupM = 8;      // token tiles per raster group
 
 __device__ __forceinline__ void mma2_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -429,11 +447,6 @@ __device__ __forceinline__ void mma2_mxf4(uint32_t d, uint64_t a, uint64_t b, ui
         "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
         : "memory");
 }
-// A scale tile of each CTA's shared memory (the same offset in both) to its own tensor memory.
-__device__ __forceinline__ void cp2_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
 __device__ __forceinline__ void tile2(const ProductParams& p, int item, int& xt, int& wt) {
     const int per = kGroupM * p.w_tiles, g = item / per, first = g * kGroupM;
     const int rows = min(kGroupM, p.x_tiles - first), r = item - g * per;
@@ -441,9 +454,10 @@ __device__ __forceinline__ void tile2(const ProductParams& p, int item, int& xt,
     wt = r / rows;
 }
 
+template <bool TMA_OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmXs,
-                const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmY, ProductParams p, int tma_store) {
+                const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmY, ProductParams p) {
     using C = Cfg2;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -456,7 +470,9 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     uint64_t* bars = (uint64_t*)(stage_out + C::OUT);
     uint64_t* full = bars;            // leader's: the bytes of both CTAs' copies
     uint64_t* empty = bars + STAGES;  // in both, from the leader's multicast commit
-    uint64_t* tfull = bars + 2 * STAGES;
+    uint64_t* sfull = bars + 2 * STAGES;   // each CTA's own: its scale tiles have landed
+    uint64_t* scaled = bars + 3 * STAGES;  // leader's: the scale warps of both CTAs have stored them
+    uint64_t* tfull = bars + 4 * STAGES;
     uint64_t* tempty = tfull + 1;     // leader's: the epilogue threads of both CTAs
     uint32_t* tmem_slot = (uint32_t*)(tempty + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
@@ -468,6 +484,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
+            mbar_init(smem_u32(&sfull[s]), 1);
+            mbar_init(smem_u32(&scaled[s]), 8);
         }
         mbar_init(smem_u32(tfull), 1);
         mbar_init(smem_u32(tempty), 512);
@@ -500,11 +518,13 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 for (int kb = 0; kb < p.kb; ++kb) {
                     if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 75)) { ok = false; break; }
                     const uint32_t bar = smem_u32(&full[s]);
-                    if (leader) mbar_expect_tx(bar, 2 * C::STAGE);
+                    if (leader) mbar_expect_tx(bar, 2 * (C::A_BYTES + C::B_BYTES));
                     tma_load_2d_pair(smem_u32(smem_a + (size_t)s * C::A_BYTES), &tmX, bar, kb * 128, xt * 256 + (int)rank * 128);
                     tma_load_2d_pair(smem_u32(smem_b + (size_t)s * C::B_BYTES), &tmW, bar, kb * 128, wt * 256 + (int)rank * 128);
-                    tma_load_2d_pair(smem_u32(smem_sa + (size_t)s * C::SA_BYTES), &tmXs, bar, kb * 256, xt * 2 + (int)rank);
-                    tma_load_2d_pair(smem_u32(smem_sb + (size_t)s * C::SB_BYTES), &tmWs, bar, kb * 256, wt * 2);
+                    const uint32_t sbar = smem_u32(&sfull[s]);
+                    mbar_expect_tx(sbar, C::SA_BYTES + C::SB_BYTES);
+                    tma_load_2d(smem_u32(smem_sa + (size_t)s * C::SA_BYTES), &tmXs, sbar, kb * 256, xt * 2 + (int)rank);
+                    tma_load_2d(smem_u32(smem_sb + (size_t)s * C::SB_BYTES), &tmWs, sbar, kb * 256, wt * 2);
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
@@ -522,16 +542,10 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 acc_phase ^= 1u;
                 tc_fence_after();
                 for (int kb = 0; kb < p.kb; ++kb) {
-                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 77)) { ok = false; break; }
+                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 77) ||
+                        !mbar_wait(smem_u32(&scaled[s]), phase, abort_flag, p.status, 83)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem_sa + (size_t)s * C::SA_BYTES), sb = smem_u32(smem_sb + (size_t)s * C::SB_BYTES);
                     const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 24, sfb = sfa + 8;
-#pragma unroll
-                    for (uint32_t j = 0; j < 2; ++j) {  // tiles of 128 elements; B's rows 0-127 and 128-255
-                        cp2_scales(sfa + 4 * j, scale_desc(sa + j * kTile));
-                        cp2_scales(sfb + 8 * j, scale_desc(sb + j * kTile));
-                        cp2_scales(sfb + 8 * j + 4, scale_desc(sb + (2 + j) * kTile));
-                    }
                     const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
                     const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
 #pragma unroll
@@ -545,69 +559,105 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 mma2_commit_mc(smem_u32(tfull), 3);
             }
         }
+    } else if (warp >= 10) {
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SCALE_COL;
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int item = cid; ok && item < items; item += pairs) {
+            for (int kb = 0; kb < p.kb; ++kb) {
+                if (!mbar_wait(smem_u32(&sfull[s]), phase, abort_flag, p.status, 84)) { ok = false; break; }
+                const uint8_t *sa = smem_sa + (size_t)s * C::SA_BYTES, *sb = smem_sb + (size_t)s * C::SB_BYTES;
+                const uint32_t sfa = lanes + (uint32_t)s * 24, sfb = sfa + 8;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {  // tiles of 128 elements; B's rows 0-127 and 128-255
+                    stage_scales(sfa + 4 * j, sa + j * kTile, lane);
+                    stage_scales(sfb + 8 * j, sb + j * kTile, lane);
+                    stage_scales(sfb + 8 * j + 4, sb + (2 + j) * kTile, lane);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (leader) mbar_arrive(smem_u32(&scaled[s]));
+                    else mbar_arrive_leader(smem_u32(&scaled[s]));
+                }
+                if (++s == STAGES) { s = 0; phase ^= 1u; }
+            }
+        }
     } else {
         const int quarter = warp & 3, chalf = (warp - 2) >> 2;
         uint8_t* mine = stage_out + (warp - 2) * 2048;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(chalf * 128);
         uint32_t acc_phase = 0;
+        auto release = [&] {
+            tc_fence_before();
+            if (leader) mbar_arrive(smem_u32(tempty));
+            else mbar_arrive_leader(smem_u32(tempty));
+        };
+        auto biased = [&](uint32_t v, int col) {
+            return p.bias && col < p.m ? __uint_as_float(v) + __ldg(p.bias + col) : __uint_as_float(v);
+        };
         for (int item = cid; item < items; item += pairs) {
             int xt, wt;
             tile2(p, item, xt, wt);
             if (!mbar_wait(smem_u32(tfull), acc_phase, abort_flag, p.status, 78)) break;
             acc_phase ^= 1u;
             tc_fence_after();
-            uint32_t r[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                tmem_ld_x32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(chalf * 128 + c * 32), r[c]);
-            tmem_ld_wait();
-            tc_fence_before();
-            if (leader) mbar_arrive(smem_u32(tempty));
-            else mbar_arrive_leader(smem_u32(tempty));
             const int row0 = xt * 256 + (int)rank * 128 + quarter * 32, col0 = wt * 256 + chalf * 128;
+            if (TMA_OUT) {
+                uint32_t w[4][16];  // 128 columns as bf16 pairs
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int col = col0 + c * 32;
-                if (p.bias) {
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t r[2][32];
+                    tmem_ld_x32(lanes + (uint32_t)(hf * 64), r[0]);
+                    tmem_ld_x32(lanes + (uint32_t)(hf * 64 + 32), r[1]);
+                    tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (col + j < p.m) r[c][j] = __float_as_uint(__uint_as_float(r[c][j]) + __ldg(p.bias + col + j));
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int col = col0 + hf * 64 + c * 32 + 2 * j;
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(biased(r[c][2 * j], col), biased(r[c][2 * j + 1], col + 1));
+                            w[2 * hf + c][j] = *(const uint32_t*)&h;
+                        }
                 }
-                if (tma_store) {
+                release();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
                     if (lane == 0) bulk_wait_read0();
                     __syncwarp();
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[c][8 * q + 2 * e]), __uint_as_float(r[c][8 * q + 2 * e + 1]));
-                            w[e] = *(const uint32_t*)&h;
-                        }
-                        *(uint4*)(mine + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int q = 0; q < 4; ++q)
+                        *(uint4*)(mine + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
+                            make_uint4(w[c][4 * q], w[c][4 * q + 1], w[c][4 * q + 2], w[c][4 * q + 3]);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_2d(&tmY, smem_u32(mine), col, row0);
+                        tma_store_2d(&tmY, smem_u32(mine), col0 + c * 32, row0);
                         bulk_commit();
                     }
-                } else {  // f32, or rows that do not start on 16 bytes: turned in shared memory, 16 columns at a time
+                }
+            } else {  // f32, or rows that do not start on 16 bytes: turned in shared memory, 16 columns at a time
+#pragma unroll 1
+                for (int c = 0; c < 128; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld_x16(lanes + (uint32_t)c, r);
+                    tmem_ld_wait();
+                    if (c == 112) release();
+                    float* t = (float*)mine;
+                    __syncwarp();
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        float* t = (float*)mine;
-                        __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) t[lane * 16 + ((j + lane) & 15)] = __uint_as_float(r[c][hf * 16 + j]);
-                        __syncwarp();
-                        const int j = lane & 15, cj = col + hf * 16 + j;
+                    for (int j = 0; j < 16; ++j) t[lane * 16 + ((j + lane) & 15)] = biased(r[j], col0 + c + j);
+                    __syncwarp();
+                    const int j = lane & 15, cj = col0 + c + j;
 #pragma unroll 4
-                        for (int i = lane >> 4; i < 32; i += 2) {
-                            const float v = t[i * 16 + ((j + i) & 15)];
-                            if (row0 + i < p.n && cj < p.m) {
-                                const int64_t o = (int64_t)(row0 + i) * p.m + cj;
-                                if (p.y_f32) ((float*)p.y)[o] = v;
-                                else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(v);
-                            }
+                    for (int i = lane >> 4; i < 32; i += 2) {
+                        const float v = t[i * 16 + ((j + i) & 15)];
+                        if (row0 + i < p.n && cj < p.m) {
+                            const int64_t o = (int64_t)(row0 + i) * p.m + cj;
+                            if (p.y_f32) ((float*)p.y)[o] = v;
+                            else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(v);
                         }
                     }
                 }
@@ -727,13 +777,13 @@ int resident_pairs(int dev, int sms) {
     static int known[64] = {};
     std::lock_guard<std::mutex> lk(mu);
     if (known[dev & 63] == 0) {
-        LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
+        LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(sms & ~1);
         cfg.blockDim = dim3(kThreads2);
         cfg.dynamicSmemBytes = Cfg2::SMEM;
         int n = 0;
-        LQ_CUDA(cudaOccupancyMaxActiveClusters(&n, mx4_pair_kernel, &cfg));
+        LQ_CUDA(cudaOccupancyMaxActiveClusters(&n, mx4_pair_kernel<true>, &cfg));
         known[dev & 63] = std::max(1, std::min(n, sms / 2));
     }
     return known[dev & 63];
@@ -750,9 +800,10 @@ void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int6
     p.w_tiles = (p.m + 255) / 256;
     LQ_CHECK_ARG((int64_t)p.x_tiles * p.w_tiles < (int64_t)1 << 31, "too many tiles");
     const int pairs = std::min(resident_pairs(dev, sms), p.x_tiles * p.w_tiles);
-    LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
+    auto kern = tma_store ? mx4_pair_kernel<true> : mx4_pair_kernel<false>;
+    LQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
     LqProf prof(LQ_K_GEMM_MAIN, st);
-    lqstream::launch_pdl(mx4_pair_kernel, dim3(2 * pairs), dim3(kThreads2), Cfg2::SMEM, st, tx, tw, txs, tws, ty, p, tma_store);
+    lqstream::launch_pdl(kern, dim3(2 * pairs), dim3(kThreads2), Cfg2::SMEM, st, tx, tw, txs, tws, ty, p);
     LQ_CUDA(cudaGetLastError());
 }
 
