@@ -285,16 +285,14 @@ int lq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t l
 int lq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, void* out, int out_dtype, void* stream);
 
 /* Y[n, m] = X[n, k] . W[m, k]^T + bias[m] (f32, may be NULL), both operands microscaled, f32 accumulation, y contiguous
- * LQ_F32 or LQ_BF16 (rounded once).  `ws`: lq_mx4_matmul_workspace_bytes() bytes on the current device (may be 0),
- * 16-byte aligned; calls that can overlap need one each. */
-size_t lq_mx4_matmul_workspace_bytes(int64_t n, int64_t m, int64_t k);
+ * LQ_F32 or LQ_BF16 (rounded once).  No workspace. */
 int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales,
-                  int64_t m, int64_t k, const float* bias, void* y, int y_dtype, void* ws, size_t ws_bytes, void* stream);
+                  int64_t m, int64_t k, const float* bias, void* y, int y_dtype, void* stream);
 
 /* lq_mx4_quantize of x [n, k] (`ldx` elements between rows) and lq_mx4_matmul in one call, Y in x's type: the product's first
- * weight tiles are fetched while x is quantised.  `ws`: lq_mx4_linear_workspace_bytes() bytes on the current device,
- * 256-byte aligned. */
-size_t lq_mx4_linear_workspace_bytes(int64_t n, int64_t m, int64_t k);
+ * weight tiles are fetched while x is quantised.  `ws` holds the quantised x: lq_mx4_linear_workspace_bytes() bytes,
+ * 256-byte aligned; calls that can overlap need one each. */
+size_t lq_mx4_linear_workspace_bytes(int64_t n, int64_t k);
 int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* w_codes, const void* w_scales, int64_t m,
                   int64_t k, const float* bias, void* y, void* ws, size_t ws_bytes, void* stream);
 

@@ -92,9 +92,8 @@ SIGNATURES = {
     "lq_mx4_scale_bytes": (_SZ, [_I64, _I64]),
     "lq_mx4_quantize": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P]),
     "lq_mx4_dequantize": (_I, [_P, _P, _I64, _I64, _P, _I, _P]),
-    "lq_mx4_matmul_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
-    "lq_mx4_matmul": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I, _P, _SZ, _P]),
-    "lq_mx4_linear_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "lq_mx4_matmul": (_I, [_P, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I, _P]),
+    "lq_mx4_linear_workspace_bytes": (_SZ, [_I64, _I64]),
     "lq_mx4_linear": (_I, [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
     "lq_mx4_matmul_dx_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "lq_mx4_matmul_dx": (_I, [_P, _I, _I64, _P, _P, _I64, _I64, _P, _P, _SZ, _P]),

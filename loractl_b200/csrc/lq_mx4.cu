@@ -200,35 +200,46 @@ struct ProductParams {
     const uint8_t* x_scales;
     int m, n, kb;             // d_out, tokens, k-blocks of 256
     int w_tiles, x_tiles;     // 128 weight rows; BN tokens, which is 128 (a whole scale tile) when there are several
-    int splits;
-    float* part;              // [splits][n][m] f32 when splits > 1
+    int splits;               // blocks of a tile: ranges of the reduction, one cluster
     const float* bias;
     void* y;
     int y_f32;
     int* status;
 };
 
-constexpr int kThreads = 320;  // TMA warp, MMA warp, four epilogue warps, four scale warps
+constexpr int kThreads = 192;  // TMA warp, MMA warp, four warps that stage scales and then write the output
 
 template <int BN>
 struct CfgT {
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN * 128, S_BYTES = 2 * kTile;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + 2 * S_BYTES;
-    static constexpr int STAGES = (200 * 1024) / STAGE < 10 ? (200 * 1024) / STAGE : 10;
-    static constexpr uint32_t TMEM = 512;
+    static constexpr int STAGES = (104 * 1024) / STAGE;  // two blocks to an SM
+    static constexpr uint32_t TMEM = 256;
     // An MMA of few columns takes its latency, not its work, when the next one waits for its sum: the four MMAs
     // of a k-block then go to an accumulator each.
     static constexpr int ACCS = BN <= 32 ? 4 : 1;
-    static constexpr uint32_t SCALE_COL = 2 * ACCS * BN;  // behind the two sets of accumulators: 16 columns per stage
-    static_assert(SCALE_COL + 16 * STAGES <= 512, "tensor memory");
+    static constexpr uint32_t SCALE_COL = ACCS * BN;  // behind the accumulators: 16 columns per stage
+    static_assert(SCALE_COL + 16 * STAGES <= TMEM, "tensor memory");
+    static_assert(BN * 512 <= STAGES * STAGE, "the f32 tile takes the ring's place");
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 256;
 };
 
+__device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // Few tokens (or few weight rows): the weight is the 128-row operand and BN tokens are the columns, so that a
-// narrow batch wastes no tensor rows, and the reduction is cut into `splits` ranges so that every SM streams
-// weights.  D's lane is a weight row, so a store of one token writes 32 consecutive outputs.
+// narrow batch wastes no tensor rows.  The weight's bytes are the work, so every SM has to stream them: a tile's
+// reduction is cut into `splits` ranges, one block each, and the blocks of a tile are a cluster that adds its f32
+// tiles up through distributed shared memory, in rank order, each rank a share of the tokens.  (Partial tiles in HBM and
+// a second launch took 5.8 us of 14.6 at 77 x 2592 -> 6151.)  D's lane is a weight row, so a store of one
+// token writes 32 consecutive outputs.
 template <int BN>
-__global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_constant__ CUtensorMap tmW,
+__global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_constant__ CUtensorMap tmW,
                                                                  const __grid_constant__ CUtensorMap tmX, ProductParams p) {
     using C = CfgT<BN>;
     constexpr int STAGES = C::STAGES;
@@ -242,10 +253,13 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
     uint64_t* empty = bars + STAGES;
     uint64_t* scaled = bars + 2 * STAGES;  // the stage's scales are in tensor memory
     uint64_t* tfull = bars + 3 * STAGES;
-    uint64_t* tempty = tfull + 2;
-    uint32_t* tmem_slot = (uint32_t*)(tempty + 2);
+    uint32_t* tmem_slot = (uint32_t*)(tfull + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // block = split of a tile; the grid is tiles x splits with the splits of a tile next to one another
+    const int z = (int)blockIdx.x % p.splits, tile = (int)blockIdx.x / p.splits;
+    const int wt = tile % p.w_tiles, xt = tile / p.w_tiles;
+    const int k0 = (int)((long long)p.kb * z / p.splits), k1 = (int)((long long)p.kb * (z + 1) / p.splits);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -253,10 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
             mbar_init(smem_u32(&empty[s]), 1);
             mbar_init(smem_u32(&scaled[s]), 4);
         }
-        for (int a = 0; a < 2; ++a) {
-            mbar_init(smem_u32(&tfull[a]), 1);
-            mbar_init(smem_u32(&tempty[a]), 128);
-        }
+        mbar_init(smem_u32(tfull), 1);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&tmW);
@@ -270,53 +281,33 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int items = p.w_tiles * p.x_tiles * p.splits;
-    auto range = [&](int item, int& wt, int& xt, int& z, int& k0, int& k1) {
-        z = item % p.splits;
-        wt = item / p.splits % p.w_tiles;
-        xt = item / p.splits / p.w_tiles;
-        k0 = (int)((long long)p.kb * z / p.splits);
-        k1 = (int)((long long)p.kb * (z + 1) / p.splits);
-    };
 
     if (warp == 0) {
         if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 0;
-            bool ok = true;
             const int kt = 2 * p.kb;
-            auto load_w = [&](int st, int wt, int kb) {
+            auto load_w = [&](int st, int kb) {
                 const uint32_t bar = smem_u32(&full[st]);
                 mbar_expect_tx(bar, C::STAGE);
                 tma_load_2d(smem_u32(smem_a + (size_t)st * C::A_BYTES), &tmW, bar, kb * 128, wt * 128);
                 bulk_load(smem_u32(smem_s + (size_t)st * 2 * C::S_BYTES), p.w_scales + ((int64_t)wt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
             };
-            auto load_x = [&](int st, int xt, int kb) {
-                const uint32_t bar = smem_u32(&full[st]);
-                tma_load_2d(smem_u32(smem_b + (size_t)st * C::B_BYTES), &tmX, bar, kb * 128, xt * BN);
-                bulk_load(smem_u32(smem_s + (size_t)st * 2 * C::S_BYTES + C::S_BYTES), p.x_scales + ((int64_t)xt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
-            };
             // the weight does not depend on the launch before this one (the quantisation of x): its first stages
             // are fetched while that runs
-            int wt, xt, z, k0, k1, ahead = 0;
-            if ((int)blockIdx.x < items) {
-                range(blockIdx.x, wt, xt, z, k0, k1);
-                ahead = min(STAGES, k1 - k0);
-                for (int i = 0; i < ahead; ++i) load_w(i, wt, k0 + i);
-            }
+            const int ahead = min(STAGES, k1 - k0);
+            for (int i = 0; i < ahead; ++i) load_w(i, k0 + i);
             lqstream::pdl_wait();
-            for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-                range(item, wt, xt, z, k0, k1);
-                for (int kb = k0; kb < k1; ++kb) {
-                    if (ahead > 0) {
-                        --ahead;
-                    } else {
-                        if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 71)) { ok = false; break; }
-                        load_w(s, wt, kb);
-                    }
-                    load_x(s, xt, kb);
-                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = k0; kb < k1; ++kb) {
+                if (kb - k0 >= ahead) {
+                    if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 71)) { ok = false; break; }
+                    load_w(s, kb);
                 }
+                const uint32_t bar = smem_u32(&full[s]);
+                tma_load_2d(smem_u32(smem_b + (size_t)s * C::B_BYTES), &tmX, bar, kb * 128, xt * BN);
+                bulk_load(smem_u32(smem_s + (size_t)s * 2 * C::S_BYTES + C::S_BYTES), p.x_scales + ((int64_t)xt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
+                if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
             if (!ok)
                 for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the block ends
@@ -324,92 +315,91 @@ __global__ void __launch_bounds__(kThreads, 1) mx4_stream_kernel(const __grid_co
     } else if (warp == 1) {
         if (lane == 0) {
             const uint32_t d_hi = desc_hi(1024);
-            int s = 0, acc = 0;
-            uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
-            for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-                int wt, xt, z, k0, k1;
-                range(item, wt, xt, z, k0, k1);
-                if (!mbar_wait(smem_u32(&tempty[acc]), acc_phase ^ 1u, abort_flag, p.status, 72)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d = tmem + (uint32_t)(acc * C::ACCS * BN);
-                for (int kb = k0; kb < k1; ++kb) {
-                    if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 73) ||
-                        !mbar_wait(smem_u32(&scaled[s]), phase, abort_flag, p.status, 79)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 16, sfb = sfa + 8;
-                    const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
-                    const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)  // 64 elements = 32 bytes; scale pair k & 1 of tile k / 2
-                        mma_mxf4(d + k % C::ACCS * BN, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi),
-                                 idesc_mxf4(128, BN, k & 1), sfa + 4 * (k >> 1), sfb + 4 * (k >> 1),
-                                 (kb > k0 || k >= C::ACCS) ? 1u : 0u);
-                    mma_commit(smem_u32(&empty[s]));
-                    if (++s == STAGES) { s = 0; phase ^= 1u; }
-                }
-                if (!ok) break;
-                mma_commit(smem_u32(&tfull[acc]));
-                if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
-            }
-        }
-    } else if (warp >= 6) {
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::SCALE_COL;
-        int s = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-            int wt, xt, z, k0, k1;
-            range(item, wt, xt, z, k0, k1);
+            int s = 0;
+            uint32_t phase = 0;
             for (int kb = k0; kb < k1; ++kb) {
-                // the stage was released before its copies began, so its columns are free too
-                if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 80)) { ok = false; break; }
-                const uint8_t* sc = smem_s + (size_t)s * 2 * C::S_BYTES;
+                if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 73) ||
+                    !mbar_wait(smem_u32(&scaled[s]), phase, abort_flag, p.status, 79)) break;
+                tc_fence_after();
+                const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 16, sfb = sfa + 8;
+                const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
+                const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) stage_scales(lanes + (uint32_t)(s * 16 + 4 * t), sc + t * kTile, lane);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&scaled[s]));
+                for (uint32_t k = 0; k < 4; ++k)  // 64 elements = 32 bytes; scale pair k & 1 of tile k / 2
+                    mma_mxf4(tmem + k % C::ACCS * BN, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi),
+                             idesc_mxf4(128, BN, k & 1), sfa + 4 * (k >> 1), sfb + 4 * (k >> 1), (kb > k0 || k >= C::ACCS) ? 1u : 0u);
+                mma_commit(smem_u32(kb + 1 == k1 ? tfull : &empty[s]));
                 if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
         }
     } else {
-        const int quarter = warp & 3;
-        int acc = 0;
-        uint32_t acc_phase = 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x) {
-            int wt, xt, z, k0, k1;
-            range(item, wt, xt, z, k0, k1);
-            if (!mbar_wait(smem_u32(&tfull[acc]), acc_phase, abort_flag, p.status, 74)) break;
-            tc_fence_after();
-            const int row = wt * 128 + quarter * 32 + lane;
-            const float bias = (p.splits == 1 && p.bias && row < p.m) ? p.bias[row] : 0.f;
-#pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
-                uint32_t r[C::ACCS][16];
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = k0; kb < k1; ++kb) {
+            // the stage was released before its copies began, so its columns are free too
+            if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 80)) { ok = false; break; }
+            const uint8_t* sc = smem_s + (size_t)s * 2 * C::S_BYTES;
 #pragma unroll
-                for (int a = 0; a < C::ACCS; ++a)
-                    tmem_ld_x16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((acc * C::ACCS + a) * BN + c), r[a]);
-                tmem_ld_wait();
-                if (row < p.m)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int tok = xt * BN + c + j;
-                        if (tok >= p.n) break;
-                        float v = __uint_as_float(r[0][j]);
-#pragma unroll
-                        for (int a = 1; a < C::ACCS; ++a) v += __uint_as_float(r[a][j]);
-                        const int64_t o = (int64_t)tok * p.m + row;
-                        if (p.splits > 1) p.part[(int64_t)z * p.n * p.m + o] = v;
-                        else if (p.y_f32) ((float*)p.y)[o] = v + bias;
-                        else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(v + bias);
-                    }
-            }
+            for (int t = 0; t < 4; ++t) stage_scales(lanes + C::SCALE_COL + (uint32_t)(s * 16 + 4 * t), sc + t * kTile, lane);
+            tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(smem_u32(&tempty[acc]));
-            if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&scaled[s]));
+            if (++s == STAGES) { s = 0; phase ^= 1u; }
         }
+        if (ok && mbar_wait(smem_u32(tfull), 0, abort_flag, p.status, 74)) {
+            tc_fence_after();
+            const int r = (warp & 3) * 32 + lane, row = wt * 128 + r;
+            const float bias = (p.splits == 1 && p.bias && row < p.m) ? p.bias[row] : 0.f;
+            float* part = (float*)smem;  // [token][128 rows]: the last product has read the ring
+#pragma unroll 1
+            for (int c = 0; c < BN && xt * BN + c < p.n; c += 16) {
+                uint32_t v[C::ACCS][16];
+#pragma unroll
+                for (int a = 0; a < C::ACCS; ++a) tmem_ld_x16(lanes + (uint32_t)(a * BN + c), v[a]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float f = __uint_as_float(v[0][j]);
+#pragma unroll
+                    for (int a = 1; a < C::ACCS; ++a) f += __uint_as_float(v[a][j]);
+                    const int tok = xt * BN + c + j;
+                    if (p.splits > 1) {
+                        part[(c + j) * 128 + r] = f;
+                    } else if (tok < p.n && row < p.m) {
+                        const int64_t o = (int64_t)tok * p.m + row;
+                        if (p.y_f32) ((float*)p.y)[o] = f + bias;
+                        else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(f + bias);
+                    }
+                }
+            }
+        }
+    }
+    if (p.splits > 1) {
+        cluster_sync_all();
+        const uint32_t part = smem_u32(smem);
+        const int quads = min(BN, p.n - xt * BN) * 32;  // four weight rows of a token each
+        for (int e = (int)threadIdx.x * p.splits + z; e < quads; e += kThreads * p.splits) {  // every splits-th is this rank's
+            const int64_t row = wt * 128 + (e & 31) * 4, tok = xt * BN + (e >> 5);
+            float4 v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < p.splits) v[q] = ld_peer(part + (uint32_t)e * 16, (uint32_t)q);
+            float f[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int q = 1; q < 8; ++q)
+                if (q < p.splits) f[0] += v[q].x, f[1] += v[q].y, f[2] += v[q].z, f[3] += v[q].w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (row + i >= p.m) break;
+                if (p.bias) f[i] += p.bias[row + i];
+                if (p.y_f32) ((float*)p.y)[tok * p.m + row + i] = f[i];
+                else ((__nv_bfloat16*)p.y)[tok * p.m + row + i] = __float2bfloat16(f[i]);
+            }
+        }
+        cluster_sync_all();  // the other ranks have read this block's tile
     }
     tc_fence_before();
     __syncthreads();
@@ -473,7 +463,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     uint64_t* sfull = bars + 2 * STAGES;   // each CTA's own: its scale tiles have landed
     uint64_t* scaled = bars + 3 * STAGES;  // leader's: the scale warps of both CTAs have stored them
     uint64_t* tfull = bars + 4 * STAGES;
-    uint64_t* tempty = tfull + 1;     // leader's: the epilogue threads of both CTAs
+    uint64_t* tempty = tfull + 1;     // leader's: the epilogue warps of both CTAs
     uint32_t* tmem_slot = (uint32_t*)(tempty + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -488,7 +478,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             mbar_init(smem_u32(&scaled[s]), 8);
         }
         mbar_init(smem_u32(tfull), 1);
-        mbar_init(smem_u32(tempty), 512);
+        mbar_init(smem_u32(tempty), 16);
         *abort_flag = 0;
         fence_barrier_init();
         prefetch_tmap(&tmX);
@@ -592,8 +582,11 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         uint32_t acc_phase = 0;
         auto release = [&] {
             tc_fence_before();
-            if (leader) mbar_arrive(smem_u32(tempty));
-            else mbar_arrive_leader(smem_u32(tempty));
+            __syncwarp();
+            if (lane == 0) {
+                if (leader) mbar_arrive(smem_u32(tempty));
+                else mbar_arrive_leader(smem_u32(tempty));
+            }
         };
         auto biased = [&](uint32_t v, int col) {
             return p.bias && col < p.m ? __uint_as_float(v) + __ldg(p.bias + col) : __uint_as_float(v);
@@ -673,19 +666,6 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     }
 }
 
-// y = sum of the splits in order + bias.
-__global__ void __launch_bounds__(256) mx4_join_kernel(ProductParams p) {
-    lqstream::pdl_wait();
-    const int64_t n = (int64_t)p.n * p.m;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        float v = 0.f;
-        for (int z = 0; z < p.splits; ++z) v += p.part[z * n + i];
-        if (p.bias) v += p.bias[i % p.m];
-        if (p.y_f32) ((float*)p.y)[i] = v;
-        else ((__nv_bfloat16*)p.y)[i] = __float2bfloat16(v);
-    }
-}
-
 // [n, m] bf16 with a row stride of `ld` elements, for the tensor maps' 16-byte rows.
 __global__ void __launch_bounds__(256) pad_rows_kernel(const __nv_bfloat16* __restrict__ in, int64_t n, int64_t m, int64_t ld,
                                                        __nv_bfloat16* __restrict__ out) {
@@ -734,41 +714,39 @@ void check_tensor(const void* codes, const void* scales) {
 
 int bn_of(int64_t n) { return n <= 16 ? 16 : (n <= 32 ? 32 : (n <= 64 ? 64 : 128)); }
 
-// Ranges of the reduction: as many as fill the SMs when the tiles alone do not, each of at least two k-blocks.
+// Ranges of the reduction (blocks of a cluster: 1, 2, 4 or 8): as many as two blocks an SM leave room for, each of at
+// least two k-blocks.
 int splits_of(int64_t tiles, int64_t kb, int sms) {
-    if (tiles >= sms) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / tiles, kb / 2), 16));
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= 2 * (int64_t)sms && kb >= 4 * s) s *= 2;
+    return s;
 }
 
 // More than one tile of tokens and of outputs each: pairs of SMs.
 bool use_pair(int64_t n, int64_t m, int sms) { return n > 128 && m > 128 && sms >= 2; }
 
-size_t product_ws(int64_t n, int64_t m, int64_t k, int sms) {
-    if (use_pair(n, m, sms)) return 0;
-    const int bn = bn_of(n);
-    const int64_t tiles = ((m + 127) / 128) * ((n + bn - 1) / bn);
-    const int s = splits_of(tiles, (k + 255) / 256, sms);
-    return s > 1 ? (size_t)s * n * m * sizeof(float) : 0;
-}
-
 template <int BN>
-void launch_stream(ProductParams p, const void* w_codes, const void* x_codes, int64_t k, int sms, cudaStream_t st) {
+void launch_stream(const ProductParams& p, const void* w_codes, const void* x_codes, int64_t k, cudaStream_t st) {
     using C = CfgT<BN>;
     const CUtensorMap tw = lq_tc_make_map_u8(w_codes, k / 2, p.m, k / 2, 128);
     const CUtensorMap tx = lq_tc_make_map_u8(x_codes, k / 2, p.n, k / 2, BN);
     LQ_CUDA(cudaFuncSetAttribute(mx4_stream_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
-    const int64_t items = (int64_t)p.w_tiles * p.x_tiles * p.splits;
-    LQ_CHECK_ARG(items < (int64_t)1 << 31, "too many tiles");
-    {
-        LqProf prof(LQ_K_GEMM_MAIN, st);
-        lqstream::launch_pdl(mx4_stream_kernel<BN>, grid_of(items, sms, 1), kThreads, C::SMEM, st, tw, tx, p);
-        LQ_CUDA(cudaGetLastError());
-    }
-    if (p.splits > 1) {
-        LqProf prof(LQ_K_REDUCE, st);
-        lqstream::launch_pdl(mx4_join_kernel, grid_of(((int64_t)p.n * p.m + 255) / 256, sms, 8), 256, 0, st, p);
-        LQ_CUDA(cudaGetLastError());
-    }
+    const int64_t blocks = (int64_t)p.w_tiles * p.x_tiles * p.splits;
+    LQ_CHECK_ARG(blocks < (int64_t)1 << 31, "too many tiles");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)p.splits, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = lqstream::pdl_enabled() ? 2 : 1;
+    LqProf prof(LQ_K_GEMM_MAIN, st);
+    LQ_CUDA(cudaLaunchKernelEx(&cfg, mx4_stream_kernel<BN>, tw, tx, p));
 }
 
 // Pairs that can be resident at once, asked once per device.
@@ -823,7 +801,7 @@ void quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, voi
 }
 
 void product(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
-             const float* bias, void* y, int y_dtype, float* part, int dev, cudaStream_t st) {
+             const float* bias, void* y, int y_dtype, int dev, cudaStream_t st) {
     const int sms = lq_tc_sm_count(dev), bn = bn_of(n);
     ProductParams p;
     p.w_scales = (const uint8_t*)w_scales;
@@ -834,16 +812,15 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
     p.w_tiles = (int)((m + 127) / 128);
     p.x_tiles = (int)((n + bn - 1) / bn);
     p.splits = splits_of((int64_t)p.w_tiles * p.x_tiles, p.kb, sms);
-    p.part = part;
     p.bias = bias;
     p.y = y;
     p.y_f32 = y_dtype == LQ_F32;
     p.status = lq_tc_status_word(dev);
     if (use_pair(n, m, sms)) launch_pair(p, w_codes, x_codes, k, dev, sms, st);
-    else if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, sms, st);
-    else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, sms, st);
-    else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, sms, st);
-    else launch_stream<128>(p, w_codes, x_codes, k, sms, st);
+    else if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, st);
+    else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, st);
+    else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, st);
+    else launch_stream<128>(p, w_codes, x_codes, k, st);
 }
 
 }  // namespace
@@ -886,15 +863,8 @@ int lq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64
     });
 }
 
-size_t lq_mx4_matmul_workspace_bytes(int64_t n, int64_t m, int64_t k) {
-    if (n < 1 || m < 1 || k < 32) return 0;
-    size_t b = 0;
-    if (guarded_call([&] { b = product_ws(n, m, k, lq_tc_sm_count(current_device())); }) != LQ_OK) return 0;
-    return b;
-}
-
 int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
-                  int64_t k, const float* bias, void* y, int y_dtype, void* ws, size_t ws_bytes, void* stream) {
+                  int64_t k, const float* bias, void* y, int y_dtype, void* stream) {
     return guarded_call([&] {
         LQ_CHECK_ARG(y_dtype == LQ_F32 || y_dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
         check_dims(n, k);
@@ -903,17 +873,13 @@ int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const vo
         check_tensor(x_codes, x_scales);
         check_tensor(w_codes, w_scales);
         LQ_CHECK_ARG(y != nullptr, "NULL argument");
-        const int dev = current_device();
-        if (ws_bytes < product_ws(n, m, k, lq_tc_sm_count(dev)) || (ws_bytes && !ws))
-            throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled product");
-        LQ_CHECK_ARG(al16(ws), "the workspace must be 16-byte aligned");
-        product(x_codes, x_scales, n, w_codes, w_scales, m, k, bias, y, y_dtype, (float*)ws, dev, (cudaStream_t)stream);
+        product(x_codes, x_scales, n, w_codes, w_scales, m, k, bias, y, y_dtype, current_device(), (cudaStream_t)stream);
     });
 }
 
-size_t lq_mx4_linear_workspace_bytes(int64_t n, int64_t m, int64_t k) {
-    if (n < 1 || m < 1 || k < 32) return 0;
-    return al256((size_t)n * k / 2) + al256(lq_mx4_scale_bytes(n, k)) + lq_mx4_matmul_workspace_bytes(n, m, k);
+size_t lq_mx4_linear_workspace_bytes(int64_t n, int64_t k) {
+    if (n < 1 || k < 32) return 0;
+    return al256((size_t)n * k / 2) + lq_mx4_scale_bytes(n, k);
 }
 
 int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
@@ -928,12 +894,12 @@ int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* 
         LQ_CHECK_ARG(ldx >= k || n == 1, "rows overlap: the row stride is below their length");
         LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
         const int dev = current_device();
-        const size_t cb = al256((size_t)n * k / 2), sb = al256(lq_mx4_scale_bytes(n, k));
-        if (ws_bytes < cb + sb + product_ws(n, m, k, lq_tc_sm_count(dev)))
+        const size_t cb = al256((size_t)n * k / 2);
+        if (ws_bytes < lq_mx4_linear_workspace_bytes(n, k))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled linear");
         uint8_t* codes = (uint8_t*)ws;
         quantize(x, dtype, n, k, ldx, codes, codes + cb, dev, (cudaStream_t)stream);
-        product(codes, codes + cb, n, w_codes, w_scales, m, k, bias, y, dtype, (float*)(codes + cb + sb), dev, (cudaStream_t)stream);
+        product(codes, codes + cb, n, w_codes, w_scales, m, k, bias, y, dtype, dev, (cudaStream_t)stream);
     });
 }
 

@@ -68,9 +68,8 @@ class Mx4Tensor:
 
 
 @functools.lru_cache(maxsize=512)
-def _sizes(index: int, n: int, m: int, k: int) -> Tuple[int, int]:
-    """Workspace bytes of the product and of the linear on a device."""
-    return L.lib().lq_mx4_matmul_workspace_bytes(n, m, k), L.lib().lq_mx4_linear_workspace_bytes(n, m, k)
+def _linear_ws(n: int, k: int) -> int:
+    return L.lib().lq_mx4_linear_workspace_bytes(n, k)
 
 
 def _as_rows(x: torch.Tensor, k: int) -> torch.Tensor:
@@ -118,12 +117,8 @@ def mx4_matmul_t(x: Mx4Tensor, w: Mx4Tensor, bias: Optional[torch.Tensor] = None
     y = torch.empty((x.rows, w.rows), dtype=dtype, device=x.device)
     code = _dtype_code(y)
     with _on_device(index):
-        nbytes = _sizes(index, x.rows, w.rows, x.k)[0]
-        # of this call alone: from the pool of the current stream, or of the graph being captured
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         L.check(L.lib().lq_mx4_matmul(x.codes.data_ptr(), x.scales.data_ptr(), x.rows, w.codes.data_ptr(), w.scales.data_ptr(), w.rows,
-                                      x.k, None if bias is None else bias.data_ptr(), y.data_ptr(), code,
-                                      None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index)))
+                                      x.k, None if bias is None else bias.data_ptr(), y.data_ptr(), code, _raw_stream(index)))
     return y
 
 
@@ -159,7 +154,7 @@ def _linear(x: torch.Tensor, w: Mx4Tensor, bias: Optional[torch.Tensor]) -> torc
     x = _as_rows(x, k)
     y = torch.empty((n, m), dtype=x.dtype, device=x.device)
     with _on_device(index):
-        nbytes = _sizes(index, n, m, k)[1]
+        nbytes = _linear_ws(n, k)  # of this call alone: from the pool of the current stream, or of the graph being captured
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         L.check(L.lib().lq_mx4_linear(x.data_ptr(), dtype, n, x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), m, k,
                                       None if bias is None else bias.data_ptr(), y.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(index)))

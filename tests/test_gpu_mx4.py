@@ -272,7 +272,7 @@ def test_refusals_without_a_gpu():
     assert lib.lq_mx4_quantize(16, 9, 1, 32, 32, 16, 16, None) == L.LQ_ERR_INVALID
     assert lib.lq_mx4_quantize(16, L.LQ_BF16, 2, 32, 16, 16, 16, None) == L.LQ_ERR_INVALID and b"overlap" in lib.lq_last_error()
     assert lib.lq_mx4_quantize(16, L.LQ_BF16, 1, 32, 32, 8, 16, None) == L.LQ_ERR_INVALID and b"aligned" in lib.lq_last_error()
-    assert lib.lq_mx4_matmul(16, 16, 1, 16, 16, 1, 32, None, None, L.LQ_F32, None, 0, None) == L.LQ_ERR_INVALID
-    assert lib.lq_mx4_matmul(16, 16, 0, 16, 16, 1, 32, None, None, L.LQ_F32, None, 0, None) == L.LQ_OK
+    assert lib.lq_mx4_matmul(16, 16, 1, 16, 16, 1, 32, None, None, L.LQ_F32, None) == L.LQ_ERR_INVALID
+    assert lib.lq_mx4_matmul(16, 16, 0, 16, 16, 1, 32, None, None, L.LQ_F32, None) == L.LQ_OK
     assert lib.lq_mx4_dequantize(16, 16, 1, 32, 8, L.LQ_F32, None) == L.LQ_ERR_INVALID
     assert lib.lq_mx4_matmul_dx(16, L.LQ_F32, 1, 16, 16, 4, 32, 16, None, 0, None) == L.LQ_ERR_INVALID
