@@ -224,6 +224,9 @@ struct CfgT {
     static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 256;
 };
 
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_x32(taddr, r); }
+
 __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
     uint32_t at;
     float4 v;
@@ -353,25 +356,30 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
             tc_fence_after();
             const int r = (warp & 3) * 32 + lane, row = wt * 128 + r;
             const float bias = (p.splits == 1 && p.bias && row < p.m) ? p.bias[row] : 0.f;
-            float* part = (float*)smem;  // [token][128 rows]: the last product has read the ring
+            const uint32_t part = smem_u32(smem) + (uint32_t)r * 4;  // [token][128 rows]: the last product has read the ring
+            constexpr int W = BN < 32 ? BN : 32;
 #pragma unroll 1
-            for (int c = 0; c < BN && xt * BN + c < p.n; c += 16) {
-                uint32_t v[C::ACCS][16];
+            for (int c = 0; c < BN && xt * BN + c < p.n; c += W) {
+                float f[W];
 #pragma unroll
-                for (int a = 0; a < C::ACCS; ++a) tmem_ld_x16(lanes + (uint32_t)(a * BN + c), v[a]);
-                tmem_ld_wait();
+                for (int a = 0; a < C::ACCS; ++a) {
+                    uint32_t v[W];
+                    tmem_ld_cols(lanes + (uint32_t)(a * BN + c), v);
+                    tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float f = __uint_as_float(v[0][j]);
+                    for (int j = 0; j < W; ++j) f[j] = a == 0 ? __uint_as_float(v[j]) : f[j] + __uint_as_float(v[j]);
+                }
+                if (p.splits > 1) {
 #pragma unroll
-                    for (int a = 1; a < C::ACCS; ++a) f += __uint_as_float(v[a][j]);
-                    const int tok = xt * BN + c + j;
-                    if (p.splits > 1) {
-                        part[(c + j) * 128 + r] = f;
-                    } else if (tok < p.n && row < p.m) {
-                        const int64_t o = (int64_t)tok * p.m + row;
-                        if (p.y_f32) ((float*)p.y)[o] = f + bias;
-                        else ((__nv_bfloat16*)p.y)[o] = __float2bfloat16(f + bias);
+                    for (int j = 0; j < W; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + (uint32_t)(c + j) * 512), "f"(f[j]) : "memory");
+                } else if (row < p.m) {
+                    const int toks = p.n - xt * BN - c;
+                    const int64_t o = (int64_t)(xt * BN + c) * p.m + row;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        if (j >= toks) break;
+                        if (p.y_f32) ((float*)p.y)[o + (int64_t)j * p.m] = f[j] + bias;
+                        else ((__nv_bfloat16*)p.y)[o + (int64_t)j * p.m] = __float2bfloat16(f[j] + bias);
                     }
                 }
             }
@@ -380,9 +388,11 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
     if (p.splits > 1) {
         cluster_sync_all();
         const uint32_t part = smem_u32(smem);
-        const int quads = min(BN, p.n - xt * BN) * 32;  // four weight rows of a token each
-        for (int e = (int)threadIdx.x * p.splits + z; e < quads; e += kThreads * p.splits) {  // every splits-th is this rank's
-            const int64_t row = wt * 128 + (e & 31) * 4, tok = xt * BN + (e >> 5);
+        const int quads = min(BN, p.n - xt * BN) * 32;  // four weight rows of a token each; rank z's share is one run of them
+        const int e1 = quads * (z + 1) / p.splits;
+        const bool whole = p.m % 4 == 0 && ((uintptr_t)p.y & 15) == 0;
+        for (int e = quads * z / p.splits + (int)threadIdx.x; e < e1; e += kThreads) {
+            const int64_t row = wt * 128 + (e & 31) * 4, tok = xt * BN + (e >> 5), o = tok * p.m + row;
             float4 v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q)
@@ -391,12 +401,22 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
 #pragma unroll
             for (int q = 1; q < 8; ++q)
                 if (q < p.splits) f[0] += v[q].x, f[1] += v[q].y, f[2] += v[q].z, f[3] += v[q].w;
+            if (p.bias) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (row + i >= p.m) break;
-                if (p.bias) f[i] += p.bias[row + i];
-                if (p.y_f32) ((float*)p.y)[tok * p.m + row + i] = f[i];
-                else ((__nv_bfloat16*)p.y)[tok * p.m + row + i] = __float2bfloat16(f[i]);
+                for (int i = 0; i < 4; ++i) f[i] += row + i < p.m ? p.bias[row + i] : 0.f;
+            }
+            if (whole && row < p.m && !p.y_f32) {  // rows of four start on 8 bytes
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(f[0], f[1]), hi = __floats2bfloat162_rn(f[2], f[3]);
+                *(uint2*)((__nv_bfloat16*)p.y + o) = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+            } else if (whole && row < p.m) {
+                *(float4*)((float*)p.y + o) = make_float4(f[0], f[1], f[2], f[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (row + i >= p.m) break;
+                    if (p.y_f32) ((float*)p.y)[o + i] = f[i];
+                    else ((__nv_bfloat16*)p.y)[o + i] = __float2bfloat16(f[i]);
+                }
             }
         }
         cluster_sync_all();  // the other ranks have read this block's tile
