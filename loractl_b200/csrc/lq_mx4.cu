@@ -74,98 +74,139 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __uint_as_float(bits);
 }
 
-__device__ __forceinline__ void load8(const float* p, bool vec, float (&v)[8]) {
-    if (vec) {
-        const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = p[i];
-    }
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool vec, float (&v)[8]) {
-    if (vec) {
-        const uint4 u = *(const uint4*)p;
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
-    }
-}
-
-// One warp per (row, 256 elements): a lane holds 8 elements, 4 lanes a block, so that loads and code stores are
-// whole lines.  HBM-bound; the padding rows of the last scale tile are items too and get zero scales.
+// Eight elements as they are stored, zeros where `in` is false; `vec`: they start on 16 bytes.
 template <typename T>
-__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__ x, int64_t rows, int64_t k, int64_t ld, int vec,
+struct In8 {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void ld(const T* p, bool in, bool vec) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (!in) return;
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg((const uint4*)p + i);
+        } else {
+            T* e = (T*)v;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = p[i];
+        }
+    }
+    // The largest magnitude as f32 bits: an integer maximum, in which an Inf or a NaN stands above everything finite.
+    __device__ __forceinline__ uint32_t top() const {
+        if (sizeof(T) == 4) {
+            const uint32_t m = 0x7FFFFFFFu;
+            const uint4 a = v[0], b = v[sizeof(T) / 2 - 1];
+            const uint32_t p = __vimax3_u32(a.x & m, a.y & m, a.z & m), q = __vimax3_u32(b.x & m, b.y & m, b.z & m);
+            return __vimax3_u32(max(p, q), a.w & m, b.w & m);
+        }
+        const uint32_t m = 0x7FFF7FFFu;  // two bf16 magnitudes a word
+        const uint32_t p = __vmaxu2(__vimax3_u16x2(v[0].x & m, v[0].y & m, v[0].z & m), v[0].w & m);
+        return max(p & 0xFFFF0000u, p << 16);
+    }
+    __device__ __forceinline__ void scaled(float s, float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (sizeof(T) == 4) {
+                    f[4 * i + j] = __uint_as_float(w[j]) * s;
+                } else {
+                    f[2 * j] = __uint_as_float(w[j] << 16) * s;
+                    f[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u) * s;
+                }
+            }
+        }
+    }
+};
+
+// One warp per run of kRun pieces of 256 elements of a row: a lane holds 8 elements, 4 lanes a block, so that loads and
+// code stores are whole lines; the run's loads are all in flight before the first is used.  The padding rows of the last
+// scale tile are runs too and get zero scales.  Bound by instruction issue before HBM (1536 x 16384 bf16: 171
+// instructions a piece 21 us, 75 % of the issue slots and 27 % of the HBM rate): hence the packed maxima and the runs
+// within one row.
+constexpr int kRun = 4;
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* __restrict__ x, int64_t rows, int k, int64_t ld, int vec,
                                                            int64_t pad_rows, uint32_t* __restrict__ codes,
                                                            uint8_t* __restrict__ scales) {
-    const int64_t kb = (k + 255) / 256;
-    const int64_t items = pad_rows * kb;
+    const int kb = (k + 255) / 256, runs = (kb + kRun - 1) / kRun;
+    const int64_t items = pad_rows * runs;
     const int lane = threadIdx.x & 31;
     lqstream::pdl_launch_dependents();  // a product behind this launch may start fetching its weight
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
-        const int64_t row = it / kb, b = it - row * kb;
-        const int64_t col = b * 256 + lane * 8;
-        const bool in = row < rows && col < k;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (in) load8(x + row * ld + col, vec, v);
-        uint32_t top = 0;
+        const int64_t row = it / runs;
+        const int b0 = (int)(it - row * runs) * kRun, col = b0 * 256 + lane * 8;
+        const bool real = row < rows;
+        const T* src = x + row * ld + col;
+        In8<T> in[kRun];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the exponent field f stands for 2^(f - 127): e = f - 129, stored as e + 127; subnormals fall to the lowest
-        uint32_t byte = (uint32_t)max((int)(top >> 23) - 2, 0);
-        const bool bad = top >= 0x7F800000u;
-        if (bad) byte = 255;
-        const float inv = __uint_as_float((254u - (bad ? 252u : byte)) << 23);
-        uint32_t w = 0;
+        for (int i = 0; i < kRun; ++i) in[i].ld(src + i * 256, real && col + i * 256 < k, vec);
+        uint32_t* dst = codes + ((row * k + col) >> 3);
+        const int r = (int)(row & 127);
+        uint8_t* sc = scales + ((row >> 7) * (2 * kb) + 2 * b0 + (lane >> 4)) * kTile + (r & 31) * 16 + (r >> 5) * 4;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= inv;
-        if (!bad) w = pack_e2m1(v);
-        if (in) codes[(row * k + col) >> 3] = w;
-        // the four scales of 128 elements as one word, from the lanes 0, 4, 8, 12 of each half-warp
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xffffffffu, byte, (lane & 16) + 4 * i) << (8 * i);
-        if ((lane & 15) == 0) {
-            const int64_t tile = (row >> 7) * (2 * kb) + 2 * b + (lane >> 4);
-            const int r = (int)(row & 127);
-            *(uint32_t*)(scales + tile * kTile + (r & 31) * 16 + (r >> 5) * 4) = word;
+        for (int i = 0; i < kRun; ++i) {
+            if (b0 + i >= kb) break;
+            uint32_t top = in[i].top();
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the exponent field f stands for 2^(f - 127): e = f - 129, stored as e + 127; subnormals fall to the lowest
+            const bool bad = top >= 0x7F800000u;
+            const uint32_t e = max(top >> 23, 2u) - 2u, byte = bad ? 255u : e;
+            float v[8];
+            in[i].scaled(__uint_as_float((254u - e) << 23), v);
+            const uint32_t w = bad ? 0u : pack_e2m1(v);
+            if (real && col + i * 256 < k) dst[i * 32] = w;
+            // the four scales of 128 elements as one word in the first lane of each half-warp
+            uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+            word |= __shfl_down_sync(0xffffffffu, word, 8) << 16;
+            if ((lane & 15) == 0) *(uint32_t*)(sc + i * 2 * kTile) = word;
         }
     }
 }
 
-// out[row, col .. col + 7] = code * scale, 8 elements a thread; exact in f32 and in bf16.
+// out[row, col .. col + 7] = code * scale, 8 elements a lane, a warp the same runs; exact in f32 and in bf16.
 template <typename T>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                             int64_t rows, int64_t k, T* __restrict__ out) {
-    const int64_t n = rows * (k / 8), kt = k_tiles(k);
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / (k / 8), col = (i - row * (k / 8)) * 8;
+                                                             int64_t rows, int k, T* __restrict__ out) {
+    const int kb = (k + 255) / 256, runs = (kb + kRun - 1) / kRun;
+    const int64_t items = rows * runs;
+    const int lane = threadIdx.x & 31;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
+        const int64_t row = it / runs;
+        const int b0 = (int)(it - row * runs) * kRun, col = b0 * 256 + lane * 8;
+        const int64_t at = row * k + col;
         const int r = (int)(row & 127);
-        const int64_t tile = (row >> 7) * kt + (col >> 7);
-        const float s = scale_value(scales[tile * kTile + (r & 31) * 16 + (r >> 5) * 4 + ((col >> 5) & 3)]);
-        float v[8];
-        unpack_e2m1(codes[i], v);
+        const uint8_t* sc = scales + ((row >> 7) * (2 * kb) + 2 * b0 + (lane >> 4)) * kTile + (r & 31) * 16 + (r >> 5) * 4 + ((lane >> 2) & 3);
+        uint32_t w[kRun], byte[kRun];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= s;
-        if (sizeof(T) == 4) {
-            ((float4*)out)[2 * i] = make_float4(v[0], v[1], v[2], v[3]);
-            ((float4*)out)[2 * i + 1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint32_t w[4];
+        for (int i = 0; i < kRun; ++i) {
+            const bool in = col + i * 256 < k;
+            w[i] = in ? __ldg(codes + (at >> 3) + i * 32) : 0u;
+            byte[i] = in ? __ldg(sc + i * 2 * kTile) : 0u;
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                w[e] = *(const uint32_t*)&h;
+        for (int i = 0; i < kRun; ++i) {
+            if (col + i * 256 >= k) break;
+            const float s = scale_value(byte[i]);
+            float v[8];
+            unpack_e2m1(w[i], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= s;
+            T* o = out + at + i * 256;
+            if (sizeof(T) == 4) {
+                ((float4*)o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                ((float4*)o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+                uint32_t q[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                    q[e] = *(const uint32_t*)&h;
+                }
+                *(uint4*)o = make_uint4(q[0], q[1], q[2], q[3]);
             }
-            ((uint4*)out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
@@ -723,9 +764,11 @@ inline unsigned grid_of(int64_t items, int sms, int per_sm) {
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, (int64_t)sms * per_sm));
 }
 
+inline int64_t runs_of(int64_t k) { return ((k + 255) / 256 + kRun - 1) / kRun; }
+
 void check_dims(int64_t rows, int64_t k) {
     LQ_CHECK_ARG(rows >= 0 && rows < (int64_t)1 << 31, "row count out of range");
-    LQ_CHECK_ARG(k >= 32 && k % 32 == 0 && k < (int64_t)1 << 31, "the block axis must be a positive multiple of 32");
+    LQ_CHECK_ARG(k >= 32 && k % 32 == 0 && k <= (int64_t)1 << 30, "the block axis must be a positive multiple of 32");
 }
 void check_tensor(const void* codes, const void* scales) {
     LQ_CHECK_ARG(codes && scales, "NULL argument");
@@ -742,8 +785,11 @@ int splits_of(int64_t tiles, int64_t kb, int sms) {
     return s;
 }
 
-// More than one tile of tokens and of outputs each: pairs of SMs.
-bool use_pair(int64_t n, int64_t m, int sms) { return n > 128 && m > 128 && sms >= 2; }
+// Pairs of SMs where their 256 x 256 tiles occupy two thirds of them; below, 128 x 128 tiles split along k spread
+// wider.  At k = 6144 (pair | stream, us): 24 tiles 16.1 | 14.4, 48 tiles 16.4 | 16.1, 72 tiles 16.9 | 16.9, 128 tiles 28 | 35, 384 tiles 71 | 93.
+bool use_pair(int64_t n, int64_t m, int sms) {
+    return n > 128 && m > 128 && ((n + 255) / 256) * ((m + 255) / 256) * 3 > sms;
+}
 
 template <int BN>
 void launch_stream(const ProductParams& p, const void* w_codes, const void* x_codes, int64_t k, cudaStream_t st) {
@@ -809,13 +855,13 @@ size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 void quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, void* codes, void* scales, int dev, cudaStream_t st) {
     const int64_t pad = row_tiles(rows) * 128;
-    const unsigned grid = grid_of((pad * ((k + 255) / 256) + 7) / 8, lq_tc_sm_count(dev), 16);
+    const unsigned grid = grid_of((pad * runs_of(k) + 7) / 8, lq_tc_sm_count(dev), 16);
     const int vec = al16(x) && (ld * (dtype == LQ_F32 ? 4 : 2)) % 16 == 0;
     LqProf prof(LQ_K_QUANT, st);
     if (dtype == LQ_F32)
-        mx4_quantize_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, k, ld, vec, pad, (uint32_t*)codes, (uint8_t*)scales);
+        mx4_quantize_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, (int)k, ld, vec, pad, (uint32_t*)codes, (uint8_t*)scales);
     else
-        mx4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, k, ld, vec, pad, (uint32_t*)codes,
+        mx4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, (int)k, ld, vec, pad, (uint32_t*)codes,
                                                                  (uint8_t*)scales);
     LQ_CUDA(cudaGetLastError());
 }
@@ -872,12 +918,12 @@ int lq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64
         check_tensor(codes, scales);
         LQ_CHECK_ARG(out && al16(out), "the output must be 16-byte aligned");
         cudaStream_t st = (cudaStream_t)stream;
-        const unsigned grid = grid_of((rows * (k / 8) + 255) / 256, lq_tc_sm_count(current_device()), 16);
+        const unsigned grid = grid_of((rows * runs_of(k) + 7) / 8, lq_tc_sm_count(current_device()), 16);
         LqProf prof(LQ_K_DEQUANT, st);
         if (out_dtype == LQ_F32)
-            mx4_dequantize_kernel<float><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, k, (float*)out);
+            mx4_dequantize_kernel<float><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, (int)k, (float*)out);
         else
-            mx4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, k,
+            mx4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, (int)k,
                                                                        (__nv_bfloat16*)out);
         LQ_CUDA(cudaGetLastError());
     });
