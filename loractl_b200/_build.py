@@ -4,7 +4,8 @@ Usage: `python -m loractl_b200._build` (or `__graft_entry__.build()`).  nvcc
 cross-compiles without a GPU; the resulting `lib/libloractl_b200.so` is what
 `loractl_b200._lib` loads.  Every translation unit is compiled to its own object
 (in parallel, and only when it or a header changed), then linked; internal C++
-symbols are hidden, only the C ABI of include/loractl_b200.h is exported.
+symbols are hidden, only the C ABI of include/loractl_b200.h is exported.  The PyTorch binding of the
+short calls (`lib/_lq_torch.so`, csrc/lq_torch.cpp) is built with g++ against the installed torch.
 """
 from __future__ import annotations
 
@@ -21,6 +22,9 @@ LIB = PKG / "lib" / "libloractl_b200.so"
 HEADER = PKG.parent / "include" / "loractl_b200.h"
 SOURCES = ["lq_api.cu", "lq_quant.cu", "lq_simt.cu", "lq_tc.cu", "lq_w4.cu", "lq_prof.cu", "lq_step.cu", "lq_fused.cu", "lq_bwd_small.cu",
            "lq_block.cu", "lq_resnorm.cu", "lq_gradnorm.cu", "lq_mx4.cu"]
+# the PyTorch binding of the short calls: a Python module that links the library and torch
+TORCH_SRC = CSRC / "lq_torch.cpp"
+TORCH_MODULE = PKG / "lib" / "_lq_torch.so"
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -37,13 +41,38 @@ def _stale(out: pathlib.Path, deps_mtime: float) -> bool:
 
 def needs_build() -> bool:
     hdr = _headers_mtime()
-    if _stale(LIB, hdr):
+    if _stale(LIB, hdr) or _stale(TORCH_MODULE, max(HEADER.stat().st_mtime, TORCH_SRC.stat().st_mtime)):
         return True
     return any((CSRC / s).stat().st_mtime > LIB.stat().st_mtime for s in SOURCES)
 
 
+def _build_torch_module(force: bool) -> None:
+    """g++ on csrc/lq_torch.cpp against the installed torch; finds the library beside itself."""
+    if not force and not _stale(TORCH_MODULE, max(HEADER.stat().st_mtime, TORCH_SRC.stat().st_mtime)):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    libs = pathlib.Path(torch.__file__).resolve().parent / "lib"
+    cuda = pathlib.Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_lq_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in [*include_paths(), sysconfig.get_paths()["include"], cuda / "include"]],
+           "-o", str(TORCH_MODULE), str(TORCH_SRC), f"-L{LIB.parent}", f"-l:{LIB.name}", f"-L{libs}", "-lc10", "-lc10_cuda",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed on {TORCH_SRC.name} ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     if not force and not needs_build():
+        return LIB
+    stale_lib = force or _stale(LIB, _headers_mtime()) or any((CSRC / s).stat().st_mtime > LIB.stat().st_mtime for s in SOURCES)
+    if not stale_lib:
+        _build_torch_module(force)
         return LIB
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     OBJ.mkdir(parents=True, exist_ok=True)
@@ -70,6 +99,7 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     proc = subprocess.run(link, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"link failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    _build_torch_module(force)
     return LIB
 
 

@@ -129,6 +129,26 @@ SIGNATURES = {
 }
 
 _lib = None
+_ext = None
+
+
+def ext():
+    """The PyTorch binding of the short calls (csrc/lq_torch.cpp); raises if it has not been built."""
+    global _ext
+    if _ext is None:
+        path = LIB_PATH.parent / "_lq_torch.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m loractl_b200._build`. There is no fallback for it.")
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries come first)
+
+        lib()
+        spec = importlib.util.spec_from_file_location("_lq_torch", str(path))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _ext = mod
+    return _ext
 
 
 def lib() -> C.CDLL:

@@ -17,15 +17,12 @@ CUDA tensors only (f32 or bf16): like every other op of this package there is no
 """
 from __future__ import annotations
 
-import functools
-import struct
 from typing import Dict, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .quant import _dtype_code, _on_device, _raw_stream, _require_cuda, _stream_ptr
+from .quant import _dtype_code, _require_cuda, _stream_ptr
 
 LN_EPS = 1e-5  # torch.nn.functional.layer_norm's default, which the harness block used before
 
@@ -212,147 +209,10 @@ def zrmsnorm(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 
 # ---- the seam between two sub-blocks --------------------------------------------------------------
 
-# `lq_residual_norm_args` and `lq_residual_norm_grads` as one pack each: setting thirty ctypes fields takes longer
-# than the kernel of a short call
-_ARGS = struct.Struct("@12P10q3i2f0P")
-_GRADS = struct.Struct("@2P4q7P")
-
-
-@functools.lru_cache(maxsize=256)
-def _residual_norm_ws(index: int, b: int, t: int, h: int) -> int:
-    return L.lib().lq_residual_norm_workspace_bytes(b, t, h)
-
-
-def _rows(v: torch.Tensor) -> torch.Tensor:
-    """`v` itself when its rows are contiguous (any sample and token stride), a copy otherwise."""
-    return v if v.stride(-1) == 1 or v.shape[-1] == 1 else v.contiguous()
-
-
-def _vector(v: torch.Tensor, b: int, h: int, dtype: torch.dtype, name: str) -> torch.Tensor:
-    """A modulation vector as a `[b, h]` view (a copy where its type differs or its rows are not contiguous)."""
-    shape = v.shape
-    if shape[-1] != h or shape[0] != b or v.numel() != b * h:
-        raise ValueError(f"{name} must be [b = {b}, h = {h}] or [b, 1, h], got {list(shape)}")
-    if v.dtype != dtype:
-        v = v.to(dtype)
-    if len(shape) != 2:
-        v = v.reshape(b, h)
-    return v if v.stride(1) == 1 or h == 1 else v.contiguous()
-
-
-def _norm_weight(w: Optional[torch.Tensor], h: int, name: str) -> Optional[torch.Tensor]:
-    if w is None:
-        return None
-    if w.numel() != h:
-        raise ValueError(f"{name} must hold {h} values, got {list(w.shape)}")
-    if w.dtype != torch.float32 or w.dim() != 1:
-        w = w.to(torch.float32).reshape(h)
-    return w if w.stride(0) == 1 else w.contiguous()
-
-
-def _residual_norm(x, gate, y, shift, scale, weight, post_weight, layer, alpha, eps, want_stats):
-    """The checks and the forward launch; returns (outputs, what the backward needs)."""
-    _require_cuda(x, "x")
-    b, t, h = _dims(x)
-    dtype, device = _dtype_code(x), x.device
-    if y is not None and (y.shape != x.shape or y.dtype != x.dtype):
-        raise ValueError(f"x and y must agree in shape and dtype, got {list(x.shape)} {x.dtype} / {list(y.shape)} {y.dtype}")
-    index = x.get_device()
-    for name, v in (("gate", gate), ("y", y), ("shift", shift), ("scale", scale), ("weight", weight), ("post_weight", post_weight)):
-        if v is not None and v.get_device() != index:
-            raise RuntimeError(f"{name} is on {v.device}, x on {device}")
-    # one type for the modulation vectors: theirs when they agree on f32 or bf16, else f32
-    kinds = {v.dtype for v in (gate, shift, scale) if v is not None}
-    if not kinds <= {torch.float32, torch.bfloat16}:
-        raise TypeError(f"unsupported dtype of gate, shift or scale {sorted(map(str, kinds))}: f32 or bf16")
-    mod_dtype = shift.dtype if len(kinds) == 1 else torch.float32
-    gate = None if y is None else _vector(gate, b, h, mod_dtype, "gate")
-    shift, scale = _vector(shift, b, h, mod_dtype, "shift"), _vector(scale, b, h, mod_dtype, "scale")
-    w, pw = _norm_weight(weight, h, "weight"), _norm_weight(post_weight, h, "post_weight")
-    x = _rows(x)
-    z = torch.empty((b, t, h), dtype=x.dtype, device=device)
-    r, yp, ys, gp, gs, rp = None, 0, (0, 0, 0), 0, 0, 0
-    if y is not None:
-        y = _rows(y)
-        r = torch.empty_like(z)
-        yp, ys, gp, gs, rp = y.data_ptr(), y.stride(), gate.data_ptr(), gate.stride(0), r.data_ptr()
-    stats, sp = None, (0, 0, 0)
-    if want_stats:
-        stats = torch.empty((3, b * t), dtype=torch.float32, device=device)
-        p = stats.data_ptr()
-        sp = (p, p + 4 * b * t, p + 8 * b * t)
-    xs = x.stride()
-    args = _ARGS.pack(x.data_ptr(), yp, gp, shift.data_ptr(), scale.data_ptr(), 0 if w is None else w.data_ptr(),
-                      0 if pw is None else pw.data_ptr(), rp, z.data_ptr(), *sp, xs[0], xs[1], ys[0], ys[1], gs, shift.stride(0),
-                      scale.stride(0), b, t, h, dtype, mod_dtype == torch.float32, layer, alpha, eps)
-    with _on_device(index):
-        L.check(L.lib().lq_residual_norm_fwd(args, _raw_stream(index)))
-    return (z,) if r is None else (r, z), (args, mod_dtype, (x, y, gate, shift, scale, w, pw, stats))
-
-
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, *inputs):
-        outs, (ctx.args, ctx.mod_dtype, saved) = _residual_norm(*inputs, True)
-        # the addresses in `args` are those of the saved tensors; r and z among them are not read by the backward
-        ctx.save_for_backward(*saved)
-        ctx.like = [None if v is None else (v.shape, v.dtype) for v in (inputs[1], *inputs[3:7])]
-        ctx.set_materialize_grads(False)
-        return outs if len(outs) == 2 else outs[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *douts):
-        dr, dz = douts if len(douts) == 2 else (None, douts[0])
-        if dr is None and dz is None:
-            return (None,) * 10
-        x = ctx.saved_tensors[0]  # the others only have to live
-        b, t, h = x.shape
-        dev, index, need = x.device, x.get_device(), ctx.needs_input_grad
-        dx = torch.empty((b, t, h), dtype=x.dtype, device=dev) if need[0] else None
-        dy = torch.empty((b, t, h), dtype=x.dtype, device=dev) if need[2] else None
-        wanted = (need[1], need[3], need[4], need[5], need[6])
-        grads = [None] * 5
-        if any(wanted[:3]):  # one buffer for the three: a view each
-            for i, v in enumerate(torch.empty((3, b, h), dtype=ctx.mod_dtype, device=dev).unbind(0)):
-                grads[i] = v if wanted[i] else None
-        if any(wanted[3:]):
-            for i, v in enumerate(torch.empty((2, h), dtype=torch.float32, device=dev).unbind(0), 3):
-                grads[i] = v if wanted[i] else None
-        rp, rs, zp, zs = 0, (0, 0), 0, (0, 0)
-        if dr is not None:
-            dr = _rows(dr)
-            rp, rs = dr.data_ptr(), dr.stride()
-        if dz is not None:
-            dz = _rows(dz)
-            zp, zs = dz.data_ptr(), dz.stride()
-        at = [0 if v is None else v.data_ptr() for v in (dx, dy, *grads)]
-        g = _GRADS.pack(rp, zp, rs[0], rs[1], zs[0], zs[1], *at)
-        with _on_device(index):
-            ws, nbytes = None, 0
-            if any(wanted):
-                # of this call alone: from the pool of the current stream, or of the graph being captured
-                nbytes = _residual_norm_ws(index, b, t, h)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            L.check(L.lib().lq_residual_norm_bwd(ctx.args, g, None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index)))
-        for i, like in enumerate(ctx.like):
-            if grads[i] is not None:
-                v = grads[i] if grads[i].dtype == like[1] else grads[i].to(like[1])
-                grads[i] = v if v.shape == like[0] else v.view(like[0])
-        return dx, grads[0], dy, grads[1], grads[2], grads[3], grads[4], None, None, None
-
-
-def _apply_residual_norm(*inputs):
-    if torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in inputs[:7]):
-        return _ResidualNorm.apply(*inputs)
-    outs, _ = _residual_norm(*inputs, False)
-    return outs if len(outs) == 2 else outs[0]
-
-
 def modulated_zrmsnorm(x: torch.Tensor, weight: Optional[torch.Tensor], shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """`zrmsnorm(x, weight) * (1 + scale) + shift` (mmdit.rs:857-862 before a sub-block), one kernel each way; `weight`
     `[h]` or None.  Gradients flow to every argument that asks for one, the norm's weight among them."""
-    return _apply_residual_norm(x, None, None, shift, scale, weight, None, False, 1.0, ZRMS_EPS)
+    return L.ext().residual_norm(x, None, None, shift, scale, weight, None, False, 1.0, ZRMS_EPS)[0]
 
 
 def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *,
@@ -372,4 +232,5 @@ def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, sh
     if norm not in ("zrms", "layer"):
         raise ValueError(f"norm must be zrms or layer, got {norm!r}")
     eps = ZRMS_EPS if norm == "zrms" else LN_EPS
-    return _apply_residual_norm(x, gate, y, shift, scale, weight, post_weight, norm == "layer", float(residual_scale), eps)
+    r, z = L.ext().residual_norm(x, gate, y, shift, scale, weight, post_weight, norm == "layer", residual_scale, eps)
+    return r, z

@@ -8,16 +8,12 @@ views, NCCL all-reduces the one buffer, the finite check is one kernel and AdamW
 """
 from __future__ import annotations
 
-from array import array
-from operator import attrgetter
 from typing import List, Optional, Sequence, Tuple
 
-import numpy as np
 import torch
 
 from . import _lib as L
 from .adapters import LoraAdapters
-from .quant import _on_device, _raw_stream
 
 # crates/loractl-core/src/diffusion_trainer.rs:270-276
 INITIAL_LOSS_SCALE = 16384.0
@@ -109,11 +105,7 @@ class FlatAdapters:
     def clip_coefficient(self, max_norm: float, grad_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
         """One read of the gradient bucket: its 2-norm times `grad_scale`, the factor that brings that norm down to
         `max_norm` (for `AdamW.step`), both as f32 device scalars, and the finite check into `flag`."""
-        if not self.grads.is_cuda:
-            raise RuntimeError("the b200 backend has no CPU path")
-        norm, coef = torch.empty((2,), dtype=torch.float32, device=self.grads.device)
-        _grad_norm(self.grads.get_device(), _addresses([self.grads]), None, array("q", [self.numel]), array("i", [L.LQ_F32]),
-                   float(grad_scale), float(max_norm), norm, coef, self.flag)
+        norm, coef = L.ext().bucket_norm(self.grads, max_norm, grad_scale, self.flag)
         return norm, coef
 
     def grad_views(self, index: int):
@@ -153,75 +145,17 @@ def nonfinite_flag(grads: torch.Tensor, flag: torch.Tensor) -> None:
         L.check(L.lib().lq_grad_nonfinite_flag(grads.data_ptr(), grads.numel(), flag.data_ptr(), _stream(grads)))
 
 
-_CODES = {torch.float32: L.LQ_F32, torch.bfloat16: L.LQ_BF16}
-
-
-_DTYPE, _SHAPE = attrgetter("dtype"), attrgetter("shape")
-_addresses = lambda tensors: array("q", map(torch.Tensor.data_ptr, tensors))
-
-
-def _check_outputs(at: array, out: array, nbytes: np.ndarray) -> None:
-    """Outputs (`out[i]`, `nbytes[i]` bytes) may be the gradients themselves, one for one, and share no byte with
-    anything else."""
-    lo = np.frombuffer(out, np.int64)
-    hi = lo + nbytes
-    full = nbytes > 0
-    order = np.argsort(lo[full], kind="stable")
-    if (lo[full][order][1:] < hi[full][order][:-1]).any():
-        raise ValueError("the clipped tensors overlap one another (the same tensor twice?)")
-    if out is at:
-        return
-    glo = np.frombuffer(at, np.int64)
-    starts, ends = np.sort(glo[full]), np.sort((glo + nbytes)[full])
-    # gradients that begin before an output ends, less those that end before it begins: its own alone may be one
-    met = np.searchsorted(starts, hi, side="left") - np.searchsorted(ends, lo, side="right")
-    if (met[full] > (lo == glo)[full]).any():
-        raise ValueError("an output overlaps a gradient tensor other than its own")
-
-
-def _grad_norm(index: int, at: array, out: Optional[array], counts: array, kinds: array, grad_scale: float, max_norm: float,
-               norm: Optional[torch.Tensor], coef: Optional[torch.Tensor], flag: Optional[torch.Tensor]) -> None:
-    n, lib = len(at), L.lib()
-    with _on_device(index):
-        ws = torch.empty(lib.lq_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=torch.device("cuda", index))
-        L.check(lib.lq_grad_norm(at.buffer_info()[0], out.buffer_info()[0] if out is not None else None, counts.buffer_info()[0],
-                                 kinds.buffer_info()[0], n, grad_scale, max_norm, norm.data_ptr() if norm is not None else None,
-                                 coef.data_ptr() if coef is not None else None, flag.data_ptr() if flag is not None else None,
-                                 ws.data_ptr(), ws.numel(), _raw_stream(index)))
-
-
-def _gradients(grads) -> Tuple[List[torch.Tensor], int, array]:
-    """The list, its device and its element types."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if not grads:
-        raise ValueError("no gradient tensors")
-    if not grads[0].is_cuda:
-        raise RuntimeError("gradients must live on a CUDA device: the b200 backend has no CPU path")
-    devices = set(map(torch.Tensor.get_device, grads))
-    if len(devices) > 1:
-        raise RuntimeError(f"gradients must live on one CUDA device, got {sorted(map(str, set(t.device for t in grads)))}")
-    try:
-        return grads, devices.pop(), array("i", map(_CODES.__getitem__, map(_DTYPE, grads)))
-    except KeyError as e:
-        raise TypeError(f"unsupported gradient dtype {e.args[0]}: f32 or bf16") from None
-
-
-def _contiguous(grads: List[torch.Tensor]) -> List[torch.Tensor]:
-    return grads if all(map(torch.Tensor.is_contiguous, grads)) else [t.contiguous() for t in grads]
+def _tensors(grads) -> Sequence[torch.Tensor]:
+    return [grads] if isinstance(grads, torch.Tensor) else grads if isinstance(grads, list) else list(grads)
 
 
 def global_grad_norm(grads: Sequence[torch.Tensor], grad_scale: float = 1.0) -> torch.Tensor:
     """The 2-norm of all `grads` (f32 and bf16 tensors of any shape on one device) taken as one vector, times
     `|grad_scale|`, as an f32 device scalar: two launches for up to 128 tensors, no host synchronisation.  Squares and
     sums are 64-bit; the norm is NaN or Inf exactly when some gradient is."""
-    grads, index, kinds = _gradients(grads)
-    grads = _contiguous(grads)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _grad_norm(index, _addresses(grads), None, array("q", map(torch.Tensor.numel, grads)), kinds, float(grad_scale), 0.0, norm, None, None)
-    return norm
+    return L.ext().global_grad_norm(_tensors(grads), grad_scale)
 
 
-@torch.no_grad()
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
                    grad_scale: float = 1.0) -> torch.Tensor:
     """Scales every gradient by `grad_scale * min(1, max_norm / (norm + 1e-6))`, where `norm` is their
@@ -229,30 +163,7 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
     synchronisation.  `grads` are scaled in place (they must be contiguous and must not overlap), or written to `out`:
     contiguous tensors of the same shapes and types that overlap nothing but their own gradient.  A norm that is not
     finite gives what the formula gives: zeros and NaN for Inf, NaN for NaN."""
-    grads, index, kinds = _gradients(grads)
-    if not max_norm >= 0.0:
-        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
-    at = _addresses(grads)
-    counts = array("q", map(torch.Tensor.numel, grads))
-    if out is None:
-        outs, to = grads, at
-    else:
-        outs, out_index, out_kinds = _gradients(out)
-        if out_kinds != kinds or list(map(_SHAPE, outs)) != list(map(_SHAPE, grads)):
-            raise ValueError("out must hold one tensor of the same shape and type for each gradient")
-        if out_index != index:
-            raise RuntimeError(f"gradients must live on one CUDA device, got {grads[0].device} and {outs[0].device}")
-        to = _addresses(outs)
-    if not all(map(torch.Tensor.is_contiguous, outs)):
-        raise ValueError("gradients that are clipped in place must be contiguous" if out is None else "out tensors must be contiguous")
-    _check_outputs(at, to, np.frombuffer(counts, np.int64) * np.where(np.frombuffer(kinds, np.int32) == L.LQ_F32, 4, 2))
-    if out is not None:
-        whole = _contiguous(grads)  # copies of strided gradients live until the launch below is enqueued
-        at = at if whole is grads else _addresses(whole)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _grad_norm(index, at, to, counts, kinds, float(grad_scale), float(max_norm), norm, None, None)
-    torch.autograd.graph.increment_version(outs)
-    return norm
+    return L.ext().clip_grad_norm(_tensors(grads), max_norm, None if out is None else _tensors(out), grad_scale)
 
 
 class AdamW:

@@ -49,28 +49,6 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class _NoSwitch:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_SWITCH = _NoSwitch()
-
-
-def _on_device(index: int):
-    """`torch.cuda.device(index)`, or nothing to enter when that device is current already (a short call's own
-    time on the host is what it costs, and switching there and back is a tenth of it)."""
-    return _NO_SWITCH if torch.cuda.current_device() == index else torch.cuda.device(index)
-
-
-def _raw_stream(index: int) -> int:
-    """`_stream_ptr` by device index, without building the Stream object."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
 def _dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.float32:
         return L.LQ_F32

@@ -4,7 +4,6 @@ captured calls, the trainer's option, and what is refused.
 
 Tolerances: sums are 64-bit, so the norm is off by its one rounding to f32 (2^-24) plus 2^-53 a term; a clipped value by
 the rounding of the factor to f32, of the product, and of the type it is held in (2^-24 + 2^-24, and 2^-8 more in bf16)."""
-import numpy as np
 import pytest
 import torch
 
@@ -234,12 +233,9 @@ def test_refusals_on_the_gpu():
 
 def test_refusals_without_a_gpu():
     import loractl_b200 as lb
-    from loractl_b200.optim import _addresses, _check_outputs as check
+    from loractl_b200._lib import ext
 
-    def _check_outputs(grads, outs):
-        at = _addresses(grads)
-        check(at, at if outs is grads else _addresses(outs), np.array([4 * v.numel() for v in grads]))
-
+    _check_outputs = ext().check_outputs
     t = torch.ones(100)
     with pytest.raises(ValueError, match="no gradient"):
         lb.global_grad_norm([])
