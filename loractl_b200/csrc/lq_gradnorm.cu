@@ -68,6 +68,23 @@ __device__ __forceinline__ double block_sum(double v, double* sm) {
     return v;
 }
 
+// Single elements: the end of a tensor, or all of a chunk where source and output do not both start on 16 bytes.
+// Sixteen are read before the first is used (source and output may share memory, so the compiler keeps the order that
+// it is given).
+constexpr int kBatch = 16;
+template <typename T>
+__device__ __forceinline__ double sq_elements(const T* src, int from, int n) {
+    double s = 0.0;
+    for (int k = from + threadIdx.x; k < n; k += kBatch * kThreads) {
+        T v[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) v[e] = k + e * kThreads < n ? src[k + e * kThreads] : T(0.f);
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) s += sq((float)v[e]);
+    }
+    return s;
+}
+
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant__ List<CAP> l, double* __restrict__ part) {
     __shared__ double sm[kThreads / 32];
@@ -107,10 +124,7 @@ __global__ void __launch_bounds__(kThreads) grad_sq_kernel(const __grid_constant
             }
             done = nv * (16 / esz);
         }
-        // single elements: the end of a tensor, or all of a chunk that does not start on 16 bytes
-#pragma unroll 8
-        for (int k = done + threadIdx.x; k < n; k += kThreads)
-            s[0] += sq(bf ? __bfloat162float(((const __nv_bfloat16*)base)[k]) : ((const float*)base)[k]);
+        s[0] += bf ? sq_elements((const __nv_bfloat16*)base, done, n) : sq_elements((const float*)base, done, n);
     }
     const double t = block_sum((s[0] + s[1]) + (s[2] + s[3]), sm);
     if (threadIdx.x == 0) part[blockIdx.x] = t;
@@ -166,6 +180,17 @@ __device__ __forceinline__ uint32_t scale2(uint32_t w, const Factor& f) {
     return *(const uint32_t*)&h;
 }
 
+template <typename T>
+__device__ __forceinline__ void scale_elements(const T* src, T* dst, int from, int n, const Factor& f) {
+    for (int k = from + threadIdx.x; k < n; k += kBatch * kThreads) {
+        T v[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) v[e] = k + e * kThreads < n ? src[k + e * kThreads] : T(0.f);
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+            if (k + e * kThreads < n) dst[k + e * kThreads] = T(f((float)v[e]));
+    }
+}
 template <int CAP>
 __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_constant__ List<CAP> l, const Norm q, int publishes) {
     __shared__ double sm[kThreads / 32];
@@ -206,11 +231,8 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
             }
             done = nv * (16 / esz);
         }
-#pragma unroll 8
-        for (int k = done + threadIdx.x; k < n; k += kThreads) {
-            if (bf) ((__nv_bfloat16*)dst)[k] = __float2bfloat16(f(__bfloat162float(((const __nv_bfloat16*)base)[k])));
-            else ((float*)dst)[k] = f(((const float*)base)[k]);
-        }
+        if (bf) scale_elements((const __nv_bfloat16*)base, (__nv_bfloat16*)dst, done, n, f);
+        else scale_elements((const float*)base, (float*)dst, done, n, f);
     }
 }
 

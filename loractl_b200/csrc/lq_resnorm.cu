@@ -618,14 +618,18 @@ __global__ void __launch_bounds__(1024) resnorm_final_kernel(const Args a, const
     float s[3] = {0.f, 0.f, 0.f};
     if (j < h) {
         if (!weights) {
-            for (int c = grp; c < chunks; c += 32)
-#pragma unroll
-                for (int k = 0; k < 3; ++k) s[k] += part[((b * chunks + c) * 3 + k) * h + j];
+#pragma unroll 4
+            for (int c = grp; c < chunks; c += 32) {
+                const float* p = part + (b * chunks + c) * 3 * h + j;
+                s[0] += __ldg(p), s[1] += __ldg(p + h), s[2] += __ldg(p + 2 * h);
+            }
         } else {
-            for (int64_t c = grp; c < a.samples * chunks; c += 32) {
-                const int64_t bc = c / chunks;
-                s[0] = fmaf(part[c * 3 * h + j], 1.f + mod_at(a.scale, a.mod_f32, bc * a.scale_sample + j), s[0]);
-                if (a.y) s[2] = fmaf(part[(c * 3 + 2) * h + j], mod_at(a.gate, a.mod_f32, bc * a.gate_sample + j), s[2]);
+#pragma unroll 4
+            for (int c = grp; c < (int)a.samples * chunks; c += 32) {
+                const int bc = c / chunks;
+                const float* p = part + (int64_t)c * 3 * h + j;
+                s[0] = fmaf(__ldg(p), 1.f + mod_at(a.scale, a.mod_f32, bc * a.scale_sample + j), s[0]);
+                if (a.y) s[2] = fmaf(__ldg(p + 2 * h), mod_at(a.gate, a.mod_f32, bc * a.gate_sample + j), s[2]);
             }
         }
     }
