@@ -606,11 +606,12 @@ __device__ __forceinline__ void st_mod(void* p, int f32, int64_t i, float v) {
     else ((__nv_bfloat16*)p)[i] = __float2bfloat16(v);
 }
 
-// Sums the partial rows in a fixed order.  Block = 32 columns x 32 ranges of chunks.  blockIdx.y < samples: the sums of
-// that sample (dgate, dshift, dscale); blockIdx.y == samples: the norm weights' gradients, over all samples.
-__global__ void __launch_bounds__(1024) resnorm_final_kernel(const Args a, const lq_residual_norm_grads g, int chunks,
+// Sums the partial rows in a fixed order.  Block = 32 columns x 16 ranges of chunks.  blockIdx.y < samples: the sums of
+// that sample (dgate, dshift, dscale; of a single sample also the norm weights' gradients); blockIdx.y == samples > 1: the
+// norm weights' gradients, over all samples.
+__global__ void __launch_bounds__(512) resnorm_final_kernel(const Args a, const lq_residual_norm_grads g, int chunks,
                                                              const float* __restrict__ part) {
-    __shared__ float sm[3][32][33];
+    __shared__ float sm[3][16][33];
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, h = (int)a.h;
     const int j = blockIdx.x * 32 + lane;
     const bool weights = blockIdx.y == a.samples;
@@ -619,13 +620,13 @@ __global__ void __launch_bounds__(1024) resnorm_final_kernel(const Args a, const
     if (j < h) {
         if (!weights) {
 #pragma unroll 4
-            for (int c = grp; c < chunks; c += 32) {
+            for (int c = grp; c < chunks; c += 16) {
                 const float* p = part + (b * chunks + c) * 3 * h + j;
                 s[0] += __ldg(p), s[1] += __ldg(p + h), s[2] += __ldg(p + 2 * h);
             }
         } else {
 #pragma unroll 4
-            for (int c = grp; c < (int)a.samples * chunks; c += 32) {
+            for (int c = grp; c < (int)a.samples * chunks; c += 16) {
                 const int bc = c / chunks;
                 const float* p = part + (int64_t)c * 3 * h + j;
                 s[0] = fmaf(__ldg(p), 1.f + mod_at(a.scale, a.mod_f32, bc * a.scale_sample + j), s[0]);
@@ -639,11 +640,15 @@ __global__ void __launch_bounds__(1024) resnorm_final_kernel(const Args a, const
     if (grp >= 3 || j >= h) return;
     float v = 0.f;  // warp k adds up sum k
 #pragma unroll
-    for (int q = 0; q < 32; ++q) v += sm[grp][q][lane];
+    for (int q = 0; q < 16; ++q) v += sm[grp][q][lane];
     if (weights) {
         if (grp == 0 && g.dweight) g.dweight[j] = v;
         if (grp == 2 && g.dpost_weight) g.dpost_weight[j] = v;
         return;
+    }
+    if (a.samples == 1) {
+        if (grp == 0 && g.dweight) g.dweight[j] = v * (1.f + mod_at(a.scale, a.mod_f32, j));
+        if (grp == 2 && g.dpost_weight) g.dpost_weight[j] = v * mod_at(a.gate, a.mod_f32, j);
     }
     if (grp == 0 && g.dscale) st_mod(g.dscale, a.mod_f32, b * h + j, v * (a.weight ? 1.f + a.weight[j] : 1.f));
     if (grp == 1 && g.dshift) st_mod(g.dshift, a.mod_f32, b * h + j, v);
@@ -863,8 +868,8 @@ int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_no
         backward(a, g, chunks, part, dev, st);
         if (sums) {
             LqProf prof(LQ_K_REDUCE, st);
-            const dim3 grid((unsigned)((a.h + 31) / 32), (unsigned)(a.samples + (g.dweight || g.dpost_weight ? 1 : 0)));
-            resnorm_final_kernel<<<grid, 1024, 0, st>>>(a, g, chunks, part);
+            const dim3 grid((unsigned)((a.h + 31) / 32), (unsigned)(a.samples + (a.samples > 1 && (g.dweight || g.dpost_weight) ? 1 : 0)));
+            resnorm_final_kernel<<<grid, 512, 0, st>>>(a, g, chunks, part);
             LQ_CUDA(cudaGetLastError());
         }
     });

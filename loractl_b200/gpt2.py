@@ -23,7 +23,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .adapters import LoraAdapters, LoraSite
-from .linear import BaseLinear, QuantLinear, site
+from .linear import BaseLinear, site
 
 
 @dataclass
@@ -154,18 +154,16 @@ class Gpt2(nn.Module):
         """gpt2.rs:428-456: every per-block projection with the widths a delta must match."""
         return [LoraSite(path, base.d_in, base.d_out) for path, base in self.base_linears()]
 
-    def into_quantized(self, value: int, block: int = 32):
-        """Quantizes every per-block projection whose input width is a multiple of the quant block
+    def into_quantized(self, value, block: int = 32):
+        """Quantizes (`value`: 8, 4 or "mxfp4") every per-block projection whose input width is a multiple of the quant block
         (the rule of crates/loractl-core/src/mmdit.rs:1266-1280 applied to this model); embeddings,
         norms and the tied head stay as they are.  Returns (quantized, left plain)."""
         done = left = 0
         for _, base in self.base_linears():
-            lin = base.as_plain()
-            if lin.in_features % block != 0:
+            if base.quantize_(value, block):
+                done += 1
+            else:
                 left += 1
-                continue
-            base.inner = QuantLinear.from_linear(lin, value, block=block)
-            done += 1
         return done, left
 
     # ---- forward --------------------------------------------------------------------------

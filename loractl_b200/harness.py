@@ -20,7 +20,7 @@ dynamic loss scale, AdamW over the adapter set.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 import torch.nn.functional as F
@@ -29,8 +29,9 @@ from torch import nn
 from . import dp
 from .adapters import LoraAdapters, LoraConfig, LoraSite, TargetSpec, build_adapters
 from .block_ckpt import checkpointed_step
-from .block_ops import gated_residual, modulated_layer_norm
+from .block_ops import gated_residual, gated_residual_norm, modulated_layer_norm
 from .linear import BaseLinear, QuantLinear, site, site_group
+from .mx4 import Mx4Linear, mx4_quantize
 from .prefetch import BlockWeightPrefetcher
 from .optim import AdamW, DynamicLossScale, FlatAdapters, nonfinite_flag
 from .quant import quantize_linear_weight
@@ -43,7 +44,7 @@ class BlockConfig:
     mlp: int = 12288
     img_tokens: int = 4096
     txt_tokens: int = 512
-    quant_bits: int = 4
+    quant_bits: Union[int, str] = 4  # 4, 8 or "mxfp4"
     quant_block: int = 64
 
 
@@ -51,6 +52,8 @@ def _quant_site(d_in: int, d_out: int, cfg: BlockConfig, gen: torch.Generator, d
     """A frozen base linear with N(0, 0.02) weights, quantized on the device (the random-init
     stand-in for `Mmdit::into_quantized`, crates/loractl-core/src/mmdit.rs:1122-1158)."""
     w = torch.randn((d_out, d_in), generator=gen, device=device, dtype=torch.float32) * 0.02
+    if cfg.quant_bits == "mxfp4":
+        return BaseLinear.mx4(Mx4Linear(mx4_quantize(w)))
     return BaseLinear.quant(QuantLinear(quantize_linear_weight(w, cfg.quant_bits, cfg.quant_block)))
 
 
@@ -93,6 +96,7 @@ class DoubleStreamBlock(nn.Module):
         self.adapters: Optional[LoraAdapters] = None
         self.cond: Optional[torch.Tensor] = None  # [b, hidden] conditioning, set per step
         self.two_cuda_streams = False
+        self.fused_norms = False
 
     def sites(self) -> List[LoraSite]:
         return [LoraSite(self.path(s, n), self.bases[f"{s}_{n}"].d_in, self.bases[f"{s}_{n}"].d_out)
@@ -146,8 +150,12 @@ class DoubleStreamBlock(nn.Module):
 
         def after_attention(s):
             _, _, gate1, shift2, scale2, gate2 = mods[s]
-            x = gated_residual(xs[s], gate1, self._lin(s, "out", atts[s]))
-            xn = modulated_layer_norm(x, shift2, scale2)
+            out = self._lin(s, "out", atts[s])
+            if self.fused_norms:
+                x, xn = gated_residual_norm(xs[s], gate1, out, shift2, scale2, norm="layer")
+            else:
+                x = gated_residual(xs[s], gate1, out)
+                xn = modulated_layer_norm(x, shift2, scale2)
             return gated_residual(x, gate2, self._lin(s, "down", F.gelu(self._lin(s, "up", xn), approximate="tanh")))
 
         outs = self._on_two_streams(after_attention)
@@ -158,17 +166,22 @@ class BlockStack(nn.Module):
     """`n_blocks` double-stream blocks with one LoRA adapter set over every linear."""
 
     def __init__(self, n_blocks: int, cfg: BlockConfig, rank: int, alpha: float, device, seed: int = 5,
-                 dtype: torch.dtype = torch.bfloat16, weight_copies="none", two_cuda_streams: bool = False):
+                 dtype: torch.dtype = torch.bfloat16, weight_copies="none", two_cuda_streams: bool = False,
+                 fused_norms: bool = False):
         """`weight_copies`: "none" — every call dequantises into its workspace; "resident" (or True) —
         keep a bf16 copy of every frozen weight (2 bytes per element beside the packed 0.5), so that no
         call dequantises: the memory-for-time trade a 180 GB GPU allows; "block" — two arenas of one
         block's copies each, refilled one block ahead of the sweep on a side stream
         (`prefetch.BlockWeightPrefetcher`).  The one-token modulation sites never read a copy (their
-        forward streams the packed bytes) and get none."""
+        forward streams the packed bytes) and get none.  MXFP4 weights are multiplied as they are stored and take no
+        copies.  `fused_norms`: the gate, residual and norm between a stream's two sub-blocks as one kernel
+        (`block_ops.gated_residual_norm`; one rounding to bf16 less in between)."""
         super().__init__()
         weight_copies = {True: "resident", False: "none", None: "none"}.get(weight_copies, weight_copies)
         if weight_copies not in ("none", "resident", "block"):
             raise ValueError(f"weight_copies must be none, resident or block, got {weight_copies!r}")
+        if cfg.quant_bits == "mxfp4" and weight_copies != "none":
+            raise ValueError("weight_copies are bf16 copies of int4 / int8 weights: MXFP4 weights take none")
         self.weight_copies = weight_copies
         gen = torch.Generator(device=device).manual_seed(seed)
         self.cfg, self.dtype = cfg, dtype
@@ -183,6 +196,7 @@ class BlockStack(nn.Module):
                 d.lora_b.copy_(torch.randn(d.lora_b.shape, generator=g2, device=device) * 0.01)
         for blk in self.blocks:
             blk.adapters = self.adapters
+            blk.fused_norms = bool(fused_norms)
             blk.two_cuda_streams = bool(two_cuda_streams)  # text and image chains of a block on two CUDA streams
             if weight_copies == "resident":
                 for w in self._copy_weights(blk):

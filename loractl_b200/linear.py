@@ -16,6 +16,7 @@ from torch import nn
 from . import quant as Q
 from .adapters import LoraAdapters
 from .lora import LoraDelta
+from .mx4 import MX4_BLOCK, Mx4Linear
 
 
 class QuantLinear(nn.Module):
@@ -51,7 +52,8 @@ class QuantLinear(nn.Module):
 
 
 class BaseLinear(nn.Module):
-    """crates/loractl-core/src/mmdit.rs:451-520: `Plain(Linear)` or `Quant(QuantLinear)`."""
+    """crates/loractl-core/src/mmdit.rs:451-520: `Plain(Linear)` or `Quant(QuantLinear)`; here also
+    `Mx4(Mx4Linear)`, whose adapter delta is added outside the kernel as a plain linear's is."""
 
     def __init__(self, inner: nn.Module):
         super().__init__()
@@ -65,22 +67,40 @@ class BaseLinear(nn.Module):
     def quant(q: QuantLinear) -> "BaseLinear":
         return BaseLinear(q)
 
+    @staticmethod
+    def mx4(q: Mx4Linear) -> "BaseLinear":
+        return BaseLinear(q)
+
     @property
     def is_quant(self) -> bool:
         return isinstance(self.inner, QuantLinear)
 
     @property
+    def is_mx4(self) -> bool:
+        return isinstance(self.inner, Mx4Linear)
+
+    @property
     def d_in(self) -> int:
-        return self.inner.d_in if self.is_quant else self.inner.in_features
+        return self.inner.d_in if self.is_quant or self.is_mx4 else self.inner.in_features
 
     @property
     def d_out(self) -> int:
-        return self.inner.d_out if self.is_quant else self.inner.out_features
+        return self.inner.d_out if self.is_quant or self.is_mx4 else self.inner.out_features
 
     def as_plain(self) -> nn.Linear:
-        if self.is_quant:
-            raise RuntimeError("BaseLinear::as_plain called on a quantized (Quant) site")
+        if self.is_quant or self.is_mx4:
+            raise RuntimeError(f"BaseLinear::as_plain called on a quantized ({'Quant' if self.is_quant else 'Mx4'}) site")
         return self.inner
+
+    def quantize_(self, value: Union[int, str], block: int = Q.QUANT_BLOCK) -> bool:
+        """`Mmdit::into_quantized` for one site (mmdit.rs:1266-1280): replaces the plain linear by its quantized form
+        (`value`: 8, 4 or "mxfp4", whose block is always 32) when its input width is a multiple of the block; says
+        whether it did."""
+        lin = self.as_plain()
+        if lin.in_features % (MX4_BLOCK if value == "mxfp4" else block) != 0:
+            return False
+        self.inner = Mx4Linear.from_linear(lin) if value == "mxfp4" else QuantLinear.from_linear(lin, value, block=block)
+        return True
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.inner(x)

@@ -83,11 +83,12 @@ class LoraLinear(nn.Module):
     """crates/loractl-core/src/lora.rs:34-111: a frozen base plus a LoRA adapter,
     `y = base(x) + (alpha / rank) * B(A(dropout(x)))`.  The base may be a plain `nn.Linear`
     or a quantized `QuantLinear`; with the latter the whole forward/backward is one fused
-    call into the CUDA library."""
+    call into the CUDA library.  An `Mx4Linear` base runs its own kernels, with the delta added to them."""
 
     def __init__(self, base: nn.Module, rank: int, alpha: float, dropout_prob: float = 0.0, device=None):
         super().__init__()
         from .linear import BaseLinear, QuantLinear  # local import: linear.py imports this module
+        from .mx4 import Mx4Linear
 
         if isinstance(base, nn.Linear):
             d_in, d_out = base.in_features, base.out_features
@@ -95,6 +96,9 @@ class LoraLinear(nn.Module):
         elif isinstance(base, QuantLinear):
             d_in, d_out = base.d_in, base.d_out
             base = BaseLinear.quant(base)
+        elif isinstance(base, Mx4Linear):
+            d_in, d_out = base.d_in, base.d_out
+            base = BaseLinear.mx4(base)
         elif isinstance(base, BaseLinear):
             d_in, d_out = base.d_in, base.d_out
         else:

@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 
@@ -21,11 +21,13 @@ QUANT_BLOCK = 32  # crates/loractl-core/src/quant.rs:52
 
 
 class Quant(enum.Enum):
-    """crates/loractl-core/src/config.rs:637-649; spellings of `FromStr` at :655-664."""
+    """crates/loractl-core/src/config.rs:637-649; spellings of `FromStr` at :655-664.  MXFP4 (`mx4.py`) is this
+    backend's own."""
 
     NONE = "none"
     INT8 = "int8"
     INT4 = "int4"
+    MXFP4 = "mxfp4"
 
     @staticmethod
     def parse(s: str) -> "Quant":
@@ -36,13 +38,15 @@ class Quant(enum.Enum):
             return Quant.INT8
         if k in ("int4", "i4"):
             return Quant.INT4
-        raise ValueError(f"unknown quant {s!r} (none|int8|int4)")
+        if k == "mxfp4":
+            return Quant.MXFP4
+        raise ValueError(f"unknown quant {s!r} (none|int8|int4|mxfp4)")
 
 
-def quant_value(q: Quant) -> Optional[int]:
+def quant_value(q: Quant) -> Union[None, int, str]:
     """crates/loractl-core/src/quant.rs:156-162: None -> no quantization, Int8 -> Q8S (8 bits),
-    Int4 -> Q4S (4 bits)."""
-    return {Quant.NONE: None, Quant.INT8: 8, Quant.INT4: 4}[q]
+    Int4 -> Q4S (4 bits); "mxfp4" for MXFP4.  What the models' `into_quantized` take."""
+    return {Quant.NONE: None, Quant.INT8: 8, Quant.INT4: 4, Quant.MXFP4: "mxfp4"}[q]
 
 
 def _stream_ptr(device: torch.device) -> int:

@@ -12,14 +12,14 @@ libloractl_b200 (sites that are not stay `Plain`, crates/loractl-core/src/mmdit.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
 from .adapters import LoraAdapters, LoraSite
-from .linear import BaseLinear, QuantLinear, site
+from .linear import BaseLinear, site
 
 MASK_NEG = -3.0e4   # crates/loractl-core/src/mmdit.rs:85
 SEQUENCE_PAD = 256  # crates/loractl-core/src/mmdit.rs:92
@@ -173,6 +173,10 @@ class SwiGlu(nn.Module):
 class SingleStreamBlock(nn.Module):
     """One trunk block: modulated pre-norm attention + SwiGLU residuals (mmdit.rs:820-870)."""
 
+    # one kernel for each modulated norm and for each gate, residual and norm between the two sub-blocks (`block_ops`), in
+    # place of the tensor ops below: GPU only, the same f32 formulas with fewer roundings to bf16 in between
+    fused_norms = False
+
     SITES = ("attn.wq", "attn.wk", "attn.wv", "attn.wo", "mlp.gate", "mlp.up", "mlp.down")
 
     def __init__(self, config: MmditConfig):
@@ -210,18 +214,16 @@ class SingleStreamBlock(nn.Module):
         sizes = dict((n, b) for n, b in self.base_linears())
         return [LoraSite(f"{prefix}.{n}", sizes[n].d_in, sizes[n].d_out) for n in self.SITES]
 
-    def into_quantized(self, value: int, block: int = 32) -> Tuple[int, int]:
+    def into_quantized(self, value: Union[int, str], block: int = 32) -> Tuple[int, int]:
         """`Mmdit::into_quantized` for this block (mmdit.rs:1122-1158,1266-1280): every base linear
-        whose input width is a multiple of the quant block becomes `Quant`; the rest stay `Plain`.
+        whose input width is a multiple of the quant block becomes `Quant` (`Mx4` for value "mxfp4"); the rest stay `Plain`.
         Returns (quantized, left plain)."""
         done = left = 0
         for _, base in self.base_linears():
-            lin = base.as_plain()
-            if lin.in_features % block != 0:
+            if base.quantize_(value, block):
+                done += 1
+            else:
                 left += 1
-                continue
-            base.inner = QuantLinear.from_linear(lin, value, block=block)
-            done += 1
         return done, left
 
     # ---- forward --------------------------------------------------------------------------
@@ -230,6 +232,12 @@ class SingleStreamBlock(nn.Module):
         f = self.config.features
         mod = tvec + self.mod_lin.to(tvec.dtype)  # [b, 1, 6f]
         prescale, preshift, pregate, postscale, postshift, postgate = (mod[..., i * f:(i + 1) * f] for i in range(6))
+        if self.fused_norms and x.is_cuda:
+            from .block_ops import gated_residual, gated_residual_norm, modulated_zrmsnorm
+
+            att = self.attn(modulated_zrmsnorm(x, self.prenorm.scale, preshift, prescale), rope, mask4, adapters, f"{prefix}.attn")
+            x, mlp_in = gated_residual_norm(x, pregate, att, postshift, postscale, weight=self.postnorm.scale)
+            return gated_residual(x, postgate, self.mlp(mlp_in, adapters, f"{prefix}.mlp"))
         attn_in = (prescale + 1.0) * self.prenorm(x) + preshift
         x = x + pregate * self.attn(attn_in, rope, mask4, adapters, f"{prefix}.attn")
         mlp_in = (postscale + 1.0) * self.postnorm(x) + postshift

@@ -258,6 +258,14 @@ def test_refusals_on_the_gpu():
         lb.Mx4Tensor(q.codes, q.scales[:-1], 4, 64)
 
 
+def test_quant_spelling():
+    import loractl_b200 as lb
+
+    assert lb.Quant.parse("MXFP4") is lb.Quant.MXFP4 and lb.quant_value(lb.Quant.MXFP4) == "mxfp4"
+    with pytest.raises(ValueError, match="unknown quant"):
+        lb.Quant.parse("nvfp4")
+
+
 def test_refusals_without_a_gpu():
     import loractl_b200 as lb
     from loractl_b200 import _lib as L
