@@ -21,6 +21,7 @@
 // order, fma(gate (1 + pw), y q, alpha x), since s and mu are those of the forward's r: where x and y nearly cancel, another
 // rounding of r would no longer fit them.
 #include <algorithm>
+#include <atomic>
 
 #include <cuda_bf16.h>
 
@@ -684,10 +685,11 @@ int blocks_per_sm(int64_t h) {
     return threads <= 128 ? 6 : (threads <= 256 ? 3 : (threads <= 384 ? 2 : 1));
 }
 
-// Chunks of one sample: one block each, as many as the SMs hold at once, but four rows or more each where that
-// still gives every SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
+// Chunks of one sample: one block each, as many as the SMs hold at once and not one more (448 blocks on 444 places took
+// 292 us where 440 take 256, 8 x 4096 x 2048 forward and backward), but four rows or more each where that still gives every
+// SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
 int chunks_of(int64_t samples, int64_t tokens, int64_t h, int sms) {
-    const int64_t fill = ((int64_t)sms * blocks_per_sm(h) + samples - 1) / samples;
+    const int64_t fill = std::max<int64_t>(1, (int64_t)sms * blocks_per_sm(h) / samples);
     const int64_t one = (sms + samples - 1) / samples;
     return (int)std::max<int64_t>(1, std::min(std::min(tokens, fill), std::max(tokens / 4, one)));
 }
@@ -734,20 +736,26 @@ int current_device() {
     return dev;
 }
 
-template <typename K, typename... A>
-void launch_ring(K kern, unsigned grid, int threads, size_t smem, cudaStream_t st, A... args) {
-    LQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<grid, threads, smem, st>>>(args...);
+// Each kernel is allowed its largest ring once per device (the attribute is a driver call).
+template <auto KERN, typename... A>
+void launch_ring(int dev, unsigned grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    static std::atomic<uint64_t> allowed{0};
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(allowed.load() & bit)) {
+        LQ_CUDA(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes));
+        allowed.fetch_or(bit);
+    }
+    KERN<<<grid, threads, smem, st>>>(args...);
 }
 
 #define LQ_RING_BOUNDS(KERN, T, P, Y, ...)                                                        \
     do {                                                                                         \
-        if (threads <= 128) launch_ring(KERN<T, P, Y, 128, 6>, grid, threads, smem, st, __VA_ARGS__);      \
-        else if (threads <= 256) launch_ring(KERN<T, P, Y, 256, 3>, grid, threads, smem, st, __VA_ARGS__); \
-        else if (threads <= 384) launch_ring(KERN<T, P, Y, 384, 2>, grid, threads, smem, st, __VA_ARGS__); \
-        else if (threads <= 512) launch_ring(KERN<T, P, Y, 512, 1>, grid, threads, smem, st, __VA_ARGS__); \
-        else if (threads <= 768) launch_ring(KERN<T, P, Y, 768, 1>, grid, threads, smem, st, __VA_ARGS__); \
-        else launch_ring(KERN<T, P, Y, 1024, 1>, grid, threads, smem, st, __VA_ARGS__);                    \
+        if (threads <= 128) launch_ring<KERN<T, P, Y, 128, 6>>(dev, grid, threads, smem, st, __VA_ARGS__);      \
+        else if (threads <= 256) launch_ring<KERN<T, P, Y, 256, 3>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 384) launch_ring<KERN<T, P, Y, 384, 2>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 512) launch_ring<KERN<T, P, Y, 512, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 768) launch_ring<KERN<T, P, Y, 768, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else launch_ring<KERN<T, P, Y, 1024, 1>>(dev, grid, threads, smem, st, __VA_ARGS__);                    \
     } while (0)
 #define LQ_RING(KERN, T, ...)                                                          \
     do {                                                                              \
