@@ -608,15 +608,15 @@ __device__ __forceinline__ void st_mod(void* p, int f32, int64_t i, float v) {
 }
 
 // Sums the partial rows in a fixed order.  Block = 32 columns x 16 ranges of chunks.  blockIdx.y < samples: the sums of
-// that sample (dgate, dshift, dscale; of a single sample also the norm weights' gradients); blockIdx.y == samples > 1: the
-// norm weights' gradients, over all samples.
+// that sample (dgate, dshift, dscale; of a single sample also the norm weights' gradients; into `totals`, when there is
+// one); blockIdx.y == samples: the norm weights' gradients, over all samples and chunks.
 __global__ void __launch_bounds__(512) resnorm_final_kernel(const Args a, const lq_residual_norm_grads g, int chunks,
-                                                             const float* __restrict__ part) {
+                                                            const float* __restrict__ part, float* __restrict__ totals, int first) {
     __shared__ float sm[3][16][33];
     const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, h = (int)a.h;
     const int j = blockIdx.x * 32 + lane;
-    const bool weights = blockIdx.y == a.samples;
-    const int64_t b = blockIdx.y;
+    const int64_t b = blockIdx.y + first;
+    const bool weights = b == a.samples;
     float s[3] = {0.f, 0.f, 0.f};
     if (j < h) {
         if (!weights) {
@@ -647,6 +647,7 @@ __global__ void __launch_bounds__(512) resnorm_final_kernel(const Args a, const 
         if (grp == 2 && g.dpost_weight) g.dpost_weight[j] = v;
         return;
     }
+    if (totals) totals[(b * 3 + grp) * h + j] = v;
     if (a.samples == 1) {
         if (grp == 0 && g.dweight) g.dweight[j] = v * (1.f + mod_at(a.scale, a.mod_f32, j));
         if (grp == 2 && g.dpost_weight) g.dpost_weight[j] = v * mod_at(a.gate, a.mod_f32, j);
@@ -679,27 +680,36 @@ bool vectors_ok(const Args& a, const lq_residual_norm_grads* g) {
     return ok;
 }
 
-// Blocks of an SM by threads per block (8 columns each): what the launch bounds below leave registers for.
-int blocks_per_sm(int64_t h) {
-    const int64_t threads = (h + 255) / 256 * 32;
-    return threads <= 128 ? 6 : (threads <= 256 ? 3 : (threads <= 384 ? 2 : 1));
-}
+int threads_of(int64_t h) { return (int)((h + 255) / 256 * 32); }  // 8 columns each
 
-// Chunks of one sample: one block each, as many as the SMs hold at once and not one more (448 blocks on 444 places took
+// Blocks of an SM: 1024 threads with the forward's 64 registers, 768 with the backward's 80 (the launch bounds below).
+int blocks_per_sm(int64_t h, bool backward) { return std::max(1, (backward ? 768 : 1024) / threads_of(h)); }
+
+// Chunks of one sample, one block each: such that all blocks fill the SMs' places once, or w times where one round
+// would leave too many empty (a round beyond the last full one costs as much as a whole one: 448 blocks on 444 places took
 // 292 us where 440 take 256, 8 x 4096 x 2048 forward and backward), but four rows or more each where that still gives every
 // SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
-int chunks_of(int64_t samples, int64_t tokens, int64_t h, int sms) {
-    const int64_t fill = std::max<int64_t>(1, (int64_t)sms * blocks_per_sm(h) / samples);
-    const int64_t one = (sms + samples - 1) / samples;
-    return (int)std::max<int64_t>(1, std::min(std::min(tokens, fill), std::max(tokens / 4, one)));
+int chunks_of(int64_t samples, int64_t tokens, int64_t h, int sms, bool backward) {
+    const int64_t places = (int64_t)sms * blocks_per_sm(h, backward), one = (sms + samples - 1) / samples;
+    const int64_t most = std::max<int64_t>(1, std::min(tokens, std::max(tokens / 4, one)));
+    int64_t best = 1, cost = -1;
+    for (int64_t w = 1; w <= 4; ++w) {
+        const int64_t c = std::min(most, std::max<int64_t>(1, places * w / samples));
+        const int64_t t = (samples * c + places - 1) / places * ((tokens + c - 1) / c + 2);
+        if (cost < 0 || t < cost) best = c, cost = t;
+    }
+    return (int)best;
 }
 
 // Rows in the ring of a block, 0 when fewer than two fit.
-int stages_of(int64_t h, int dtype, int inputs) {
+int stages_of(int64_t h, int dtype, int inputs, bool backward) {
     const size_t stage = (size_t)inputs * h * (dtype == LQ_F32 ? 4 : 2);
-    const size_t n = kRingBytes / blocks_per_sm(h) / stage;
+    const size_t n = kRingBytes / blocks_per_sm(h, backward) / stage;
     return n < 2 ? 0 : (int)std::min<size_t>(n, kMaxStages);
 }
+
+// Three partial rows a chunk, then three totals a sample.
+size_t ws_bytes_of(int64_t samples, int64_t chunks, int64_t h) { return (size_t)samples * (chunks + 1) * 3 * h * sizeof(float); }
 
 void check(const Args& a) {
     LQ_CHECK_ARG(a.dtype == LQ_F32 || a.dtype == LQ_BF16, "dtype must be LQ_F32 or LQ_BF16");
@@ -748,21 +758,29 @@ void launch_ring(int dev, unsigned grid, int threads, size_t smem, cudaStream_t 
     KERN<<<grid, threads, smem, st>>>(args...);
 }
 
-#define LQ_RING_BOUNDS(KERN, T, P, Y, ...)                                                        \
-    do {                                                                                         \
-        if (threads <= 128) launch_ring<KERN<T, P, Y, 128, 6>>(dev, grid, threads, smem, st, __VA_ARGS__);      \
-        else if (threads <= 256) launch_ring<KERN<T, P, Y, 256, 3>>(dev, grid, threads, smem, st, __VA_ARGS__); \
-        else if (threads <= 384) launch_ring<KERN<T, P, Y, 384, 2>>(dev, grid, threads, smem, st, __VA_ARGS__); \
-        else if (threads <= 512) launch_ring<KERN<T, P, Y, 512, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
-        else if (threads <= 768) launch_ring<KERN<T, P, Y, 768, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
-        else launch_ring<KERN<T, P, Y, 1024, 1>>(dev, grid, threads, smem, st, __VA_ARGS__);                    \
+#define LQ_RING_FWD(T, P, Y, ...)                                                                                          \
+    do {                                                                                                                   \
+        if (threads <= 64) launch_ring<resnorm_fwd_ring_kernel<T, P, Y, 64, 16>>(dev, grid, threads, smem, st, __VA_ARGS__);     \
+        else if (threads <= 256) launch_ring<resnorm_fwd_ring_kernel<T, P, Y, 256, 4>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 512) launch_ring<resnorm_fwd_ring_kernel<T, P, Y, 512, 2>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 768) launch_ring<resnorm_fwd_ring_kernel<T, P, Y, 768, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else launch_ring<resnorm_fwd_ring_kernel<T, P, Y, 1024, 1>>(dev, grid, threads, smem, st, __VA_ARGS__);                  \
     } while (0)
-#define LQ_RING(KERN, T, ...)                                                          \
-    do {                                                                              \
-        if (a.post_weight && a.layer) LQ_RING_BOUNDS(KERN, T, true, true, __VA_ARGS__); \
-        else if (a.post_weight) LQ_RING_BOUNDS(KERN, T, true, false, __VA_ARGS__);      \
-        else if (a.layer) LQ_RING_BOUNDS(KERN, T, false, true, __VA_ARGS__);            \
-        else LQ_RING_BOUNDS(KERN, T, false, false, __VA_ARGS__);                        \
+#define LQ_RING_BWD(T, P, Y, ...)                                                                                          \
+    do {                                                                                                                   \
+        if (threads <= 64) launch_ring<resnorm_bwd_ring_kernel<T, P, Y, 64, 12>>(dev, grid, threads, smem, st, __VA_ARGS__);     \
+        else if (threads <= 256) launch_ring<resnorm_bwd_ring_kernel<T, P, Y, 256, 3>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 384) launch_ring<resnorm_bwd_ring_kernel<T, P, Y, 384, 2>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 512) launch_ring<resnorm_bwd_ring_kernel<T, P, Y, 512, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else if (threads <= 768) launch_ring<resnorm_bwd_ring_kernel<T, P, Y, 768, 1>>(dev, grid, threads, smem, st, __VA_ARGS__); \
+        else launch_ring<resnorm_bwd_ring_kernel<T, P, Y, 1024, 1>>(dev, grid, threads, smem, st, __VA_ARGS__);                  \
+    } while (0)
+#define LQ_RING(DIR, T, ...)                                          \
+    do {                                                             \
+        if (a.post_weight && a.layer) DIR(T, true, true, __VA_ARGS__); \
+        else if (a.post_weight) DIR(T, true, false, __VA_ARGS__);      \
+        else if (a.layer) DIR(T, false, true, __VA_ARGS__);            \
+        else DIR(T, false, false, __VA_ARGS__);                        \
     } while (0)
 // 8 elements a thread up to 4096 columns, then 16, then 32: blocks of at most 512 threads, 128 registers each
 #define LQ_SCALAR(KERN, ...)                                                                                                        \
@@ -783,16 +801,16 @@ void launch_ring(int dev, unsigned grid, int threads, size_t smem, cudaStream_t 
 constexpr int64_t kRingMaxH = 8192;  // 1024 threads x 8 columns
 
 void forward(const Args& a, int dev, cudaStream_t st) {
-    const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype, inputs) : 0;
+    const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype, inputs, false) : 0;
     LqProf prof(LQ_K_PREP, st);
     if (stages) {
-        const int chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev)), threads = (int)((a.h + 255) / 256 * 32);
+        const int chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev), false), threads = threads_of(a.h);
         const int64_t per = (a.tokens + chunks - 1) / chunks;
         const unsigned grid = (unsigned)(a.samples * chunks);
         const size_t smem = (size_t)std::min<int64_t>(stages, per) * inputs * a.h * (a.dtype == LQ_F32 ? 4 : 2);
         int* status = lq_tc_status_word(dev);
-        if (a.dtype == LQ_F32) LQ_RING(resnorm_fwd_ring_kernel, float, a, chunks, per, stages, status);
-        else LQ_RING(resnorm_fwd_ring_kernel, __nv_bfloat16, a, chunks, per, stages, status);
+        if (a.dtype == LQ_F32) LQ_RING(LQ_RING_FWD, float, a, chunks, per, stages, status);
+        else LQ_RING(LQ_RING_FWD, __nv_bfloat16, a, chunks, per, stages, status);
     } else {
         const unsigned grid = (unsigned)(a.samples * a.tokens);
         LQ_SCALAR(resnorm_fwd_kernel, a);
@@ -802,16 +820,16 @@ void forward(const Args& a, int dev, cudaStream_t st) {
 
 void backward(const Args& a, const lq_residual_norm_grads& g, int chunks, float* part, int dev, cudaStream_t st) {
     const int inputs = 1 + (a.y ? 1 : 0) + (g.dz ? 1 : 0) + (g.dr ? 1 : 0);
-    const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype, inputs) : 0;
+    const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype, inputs, true) : 0;
     const int64_t per = (a.tokens + chunks - 1) / chunks;
     const unsigned grid = (unsigned)(a.samples * chunks);
     LqProf prof(LQ_K_PREP, st);
     if (stages) {
-        const int threads = (int)((a.h + 255) / 256 * 32);
+        const int threads = threads_of(a.h);
         const size_t smem = (size_t)std::min<int64_t>(stages, per) * inputs * a.h * (a.dtype == LQ_F32 ? 4 : 2);
         int* status = lq_tc_status_word(dev);
-        if (a.dtype == LQ_F32) LQ_RING(resnorm_bwd_ring_kernel, float, a, g, chunks, per, stages, part, status);
-        else LQ_RING(resnorm_bwd_ring_kernel, __nv_bfloat16, a, g, chunks, per, stages, part, status);
+        if (a.dtype == LQ_F32) LQ_RING(LQ_RING_BWD, float, a, g, chunks, per, stages, part, status);
+        else LQ_RING(LQ_RING_BWD, __nv_bfloat16, a, g, chunks, per, stages, part, status);
     } else {
         LQ_SCALAR(resnorm_bwd_kernel, a, g, chunks, per, part);
     }
@@ -839,8 +857,7 @@ int lq_residual_norm_fwd(const lq_residual_norm_args* args, void* stream) {
 size_t lq_residual_norm_workspace_bytes(int64_t samples, int64_t tokens, int64_t h) {
     if (samples < 1 || tokens < 1 || h < 1 || h > kMaxH) return 0;
     size_t n = 0;
-    if (guarded_call([&] { n = (size_t)samples * chunks_of(samples, tokens, h, lq_tc_sm_count(current_device())) * 3 * h * sizeof(float); }) != LQ_OK)
-        return 0;
+    if (guarded_call([&] { n = ws_bytes_of(samples, chunks_of(samples, tokens, h, lq_tc_sm_count(current_device()), true), h); }) != LQ_OK) return 0;
     return n;
 }
 
@@ -866,9 +883,9 @@ int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_no
         LQ_CHECK_ARG(!g.dpost_weight || a.post_weight, "dpost_weight needs post_weight");
         LQ_CHECK_ARG(!g.dweight || a.weight, "dweight needs weight");
         LQ_CHECK_ARG(a.rstd && (!a.layer || a.mean) && (!a.post_weight || a.post_rstd), "the forward's statistics are needed");
-        const int dev = current_device(), chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev));
+        const int dev = current_device(), chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev), true);
         LQ_CHECK_ARG(a.samples * chunks < (int64_t)1 << 31, "too many samples");
-        if (sums && (!ws || ws_bytes < (size_t)a.samples * chunks * 3 * a.h * sizeof(float)))
+        if (sums && (!ws || ws_bytes < ws_bytes_of(a.samples, chunks, a.h)))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the residual-norm backward");
         LQ_CHECK_ARG(!sums || al16(ws), "the workspace must be 16-byte aligned");
         LQ_CHECK_ARG(!sums || a.samples < 65535, "at most 65534 samples with gradients of the vectors");
@@ -876,8 +893,12 @@ int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_no
         backward(a, g, chunks, part, dev, st);
         if (sums) {
             LqProf prof(LQ_K_REDUCE, st);
-            const dim3 grid((unsigned)((a.h + 31) / 32), (unsigned)(a.samples + (a.samples > 1 && (g.dweight || g.dpost_weight) ? 1 : 0)));
-            resnorm_final_kernel<<<grid, 512, 0, st>>>(a, g, chunks, part);
+            const unsigned cols = (unsigned)((a.h + 31) / 32), b = (unsigned)a.samples;
+            const bool weights = a.samples > 1 && (g.dweight || g.dpost_weight);
+            // the weights' sums over many partial rows would be one block's work per 32 columns: over the samples' totals instead
+            float* totals = weights && a.samples * chunks > 64 ? part + (size_t)a.samples * chunks * 3 * a.h : nullptr;
+            resnorm_final_kernel<<<dim3(cols, b + (weights && !totals ? 1 : 0)), 512, 0, st>>>(a, g, chunks, part, totals, 0);
+            if (totals) resnorm_final_kernel<<<dim3(cols, 1), 512, 0, st>>>(a, g, 1, totals, nullptr, (int)b);
             LQ_CUDA(cudaGetLastError());
         }
     });
