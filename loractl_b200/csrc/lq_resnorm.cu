@@ -432,15 +432,29 @@ __global__ void __launch_bounds__(MAXT, MINB) resnorm_bwd_ring_kernel(const Args
 // ---- any rows -----------------------------------------------------------------------------------
 // Single elements, for rows that do not all start on 16 bytes (an odd width, an odd offset) and for rows too wide
 // for the ring: thread t owns the columns t, t + blockDim, ...  All of a row's loads are issued before the first is
-// used, whatever columns the thread has (a place behind the row reads column 0 and counts as zero).
+// used, whatever columns the thread has (a place behind the row reads column 0 and counts as zero).  Up to 4096 columns
+// (VPT = 8) the modulation stays in registers over the rows of a chunk and the next row is fetched into registers behind
+// the current one's arithmetic; wider rows have no registers for either.
+template <typename T, int VPT>
+struct Raw {
+    T v[VPT];
+    __device__ __forceinline__ void ld(const T* p, int h) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = threadIdx.x + i * blockDim.x;
+            v[i] = p[c < h ? c : 0];
+        }
+    }
+    __device__ __forceinline__ void get(int h, float (&f)[VPT]) const {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) f[i] = threadIdx.x + i * blockDim.x < h ? to_f(v[i]) : 0.f;
+    }
+};
 template <typename T, int VPT>
 __device__ __forceinline__ void ld_row(const T* p, int h, float (&f)[VPT]) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int c = threadIdx.x + i * blockDim.x;
-        const float v = to_f(p[c < h ? c : 0]);
-        f[i] = c < h ? v : 0.f;
-    }
+    Raw<T, VPT> r;
+    r.ld(p, h);
+    r.get(h, f);
 }
 template <int VPT>
 __device__ __forceinline__ void ld_mods(const void* p, int f32, int64_t at, int h, float (&f)[VPT]) {
@@ -455,120 +469,172 @@ __device__ __forceinline__ void st_row(T* p, int h, const float (&f)[VPT]) {
         if (c < h) p[c] = from_f<T>(f[i]);
     }
 }
-
-template <typename T, int VPT>
-__global__ void __launch_bounds__(512) resnorm_fwd_kernel(const Args a) {
-    constexpr int MAXT = 512;
-    __shared__ __align__(16) float area[2][2][kMaxWarps];
-    int half = 0;
-    const int64_t row = blockIdx.x, b = row / a.tokens, t = row - b * a.tokens;
-    const int h = (int)a.h;
-    const float inv_h = 1.f / (float)h;
-    float r[VPT], m[VPT], v[1] = {0.f};
-    ld_row<T, VPT>((const T*)a.x + b * a.x_sample + t * a.x_token, h, r);
-    if (a.y) {
-        float y[VPT], gt[VPT];
-        ld_row<T, VPT>((const T*)a.y + b * a.y_sample + t * a.y_token, h, y);
-        ld_mods<VPT>(a.gate, a.mod_f32, b * a.gate_sample, h, gt);
-        if (a.post_weight) ld_row<float, VPT>(a.post_weight, h, m);
-        clear_area(area);
-        if (a.post_weight) {
+// gate (1 + pw) and (1 + w)(1 + scale) of a sample, in this thread's columns.
+template <int VPT>
+__device__ __forceinline__ void ld_gate(const Args& a, int64_t b, int h, float (&f)[VPT]) {
+    ld_mods<VPT>(a.gate, a.mod_f32, b * a.gate_sample, h, f);
+    if (a.post_weight) {
+        float pw[VPT];
+        ld_row<float, VPT>(a.post_weight, h, pw);
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) v[0] = fmaf(y[i], y[i], v[0]);
-            block_sum<MAXT, 1>(v, area, half);
-            const float q = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
-            if (threadIdx.x == 0 && a.rstd) a.post_rstd[row] = q;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                gt[i] *= 1.f + m[i];
-                y[i] *= q;
-            }
-            v[0] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) r[i] = fmaf(gt[i], y[i], a.alpha * r[i]);
-        if (a.r) st_row<T, VPT>((T*)a.r + row * h, h, r);
-    } else {
-        clear_area(area);
+        for (int i = 0; i < VPT; ++i) f[i] *= 1.f + pw[i];
     }
-    float mu = 0.f;
-    if (a.layer) {
+}
+template <int VPT>
+__device__ __forceinline__ void ld_mul(const Args& a, int64_t b, int h, float (&f)[VPT]) {
+    ld_mods<VPT>(a.scale, a.mod_f32, b * a.scale_sample, h, f);
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) v[0] += r[i];
-        block_sum<MAXT, 1>(v, area, half);
-        mu = v[0] * inv_h;
-        v[0] = 0.f;
+    for (int i = 0; i < VPT; ++i) f[i] += 1.f;
+    if (a.weight) {
+        float w[VPT];
+        ld_row<float, VPT>(a.weight, h, w);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) f[i] *= 1.f + w[i];
     }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-        if (threadIdx.x + i * blockDim.x < h) v[0] = fmaf(r[i] - mu, r[i] - mu, v[0]);
-    float w[VPT], sh[VPT];
-    ld_mods<VPT>(a.scale, a.mod_f32, b * a.scale_sample, h, m);
-    ld_mods<VPT>(a.shift, a.mod_f32, b * a.shift_sample, h, sh);
-    if (a.weight) ld_row<float, VPT>(a.weight, h, w);
-    block_sum<MAXT, 1>(v, area, half);
-    const float s = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
-    if (threadIdx.x == 0 && a.rstd) {
-        a.rstd[row] = s;
-        if (a.layer) a.mean[row] = mu;
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) r[i] = fmaf((r[i] - mu) * s * (a.weight ? 1.f + w[i] : 1.f), 1.f + m[i], sh[i]);
-    st_row<T, VPT>((T*)a.z + row * h, h, r);
 }
 
 template <typename T, int VPT>
-__global__ void __launch_bounds__(512) resnorm_bwd_kernel(const Args a, const lq_residual_norm_grads g, int chunks, int64_t per,
-                                                          float* __restrict__ part) {
+__global__ void __launch_bounds__(512, VPT == 8 ? 2 : 1) resnorm_fwd_kernel(const Args a, int chunks, int64_t per) {
     constexpr int MAXT = 512;
+    constexpr bool KEEP = VPT == 8;
     __shared__ __align__(16) float area[2][2][kMaxWarps];
     int half = 0;
     const Rows rows(a.tokens, chunks, per);
     const int64_t b = rows.b;
     const int h = (int)a.h;
     const float inv_h = 1.f / (float)h;
-    float S[VPT], D1[VPT], G[VPT];
+    clear_area(area);
+    if (rows.t0 >= rows.t1) return;
+    float gate[VPT], mul[VPT], shift[VPT];
+    if (KEEP) {
+        if (a.y) ld_gate<VPT>(a, b, h, gate);
+        ld_mul<VPT>(a, b, h, mul);
+        ld_mods<VPT>(a.shift, a.mod_f32, b * a.shift_sample, h, shift);
+    }
+    const T* xp = (const T*)a.x + b * a.x_sample + rows.t0 * a.x_token;
+    const T* yp = (const T*)a.y + b * a.y_sample + rows.t0 * a.y_token;
+    Raw<T, VPT> xr, yr;
+    xr.ld(xp, h);
+    if (a.y) yr.ld(yp, h);
+    for (int64_t t = rows.t0; t < rows.t1; ++t) {
+        const int64_t row = b * a.tokens + t;
+        float r[VPT], y[VPT], v[1] = {0.f};
+        xr.get(h, r);
+        if (a.y) yr.get(h, y);
+        if (KEEP && t + 1 < rows.t1) {
+            xr.ld(xp += a.x_token, h);
+            if (a.y) yr.ld(yp += a.y_token, h);
+        }
+        if (a.y) {
+            if (!KEEP) ld_gate<VPT>(a, b, h, gate);
+            if (a.post_weight) {
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) v[0] = fmaf(y[i], y[i], v[0]);
+                block_sum<MAXT, 1>(v, area, half);
+                const float q = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
+                if (threadIdx.x == 0 && a.rstd) a.post_rstd[row] = q;
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) y[i] *= q;
+                v[0] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) r[i] = fmaf(gate[i], y[i], a.alpha * r[i]);
+            if (a.r) st_row<T, VPT>((T*)a.r + row * h, h, r);
+        }
+        float mu = 0.f;
+        if (a.layer) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) v[0] += r[i];
+            block_sum<MAXT, 1>(v, area, half);
+            mu = v[0] * inv_h;
+            v[0] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (threadIdx.x + i * blockDim.x < h) v[0] = fmaf(r[i] - mu, r[i] - mu, v[0]);
+        if (!KEEP) {
+            ld_mul<VPT>(a, b, h, mul);
+            ld_mods<VPT>(a.shift, a.mod_f32, b * a.shift_sample, h, shift);
+        }
+        block_sum<MAXT, 1>(v, area, half);
+        const float s = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
+        if (threadIdx.x == 0 && a.rstd) {
+            a.rstd[row] = s;
+            if (a.layer) a.mean[row] = mu;
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) r[i] = fmaf((r[i] - mu) * s, mul[i], shift[i]);
+        st_row<T, VPT>((T*)a.z + row * h, h, r);
+        if (!KEEP && t + 1 < rows.t1) {
+            xr.ld(xp += a.x_token, h);
+            if (a.y) yr.ld(yp += a.y_token, h);
+        }
+    }
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(512) resnorm_bwd_kernel(const Args a, const lq_residual_norm_grads g, int chunks, int64_t per,
+                                                          float* __restrict__ part) {
+    constexpr int MAXT = 512;
+    constexpr bool KEEP = VPT == 8;
+    __shared__ __align__(16) float area[2][2][kMaxWarps];
+    int half = 0;
+    const Rows rows(a.tokens, chunks, per);
+    const int64_t b = rows.b;
+    const int h = (int)a.h;
+    const float inv_h = 1.f / (float)h;
+    float S[VPT], D1[VPT], G[VPT], gate[VPT], mul[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) S[i] = D1[i] = G[i] = 0.f;
     clear_area(area);
+    const T* xp = (const T*)a.x + b * a.x_sample + rows.t0 * a.x_token;
+    const T* yp = (const T*)a.y + b * a.y_sample + rows.t0 * a.y_token;
+    const T* zp = (const T*)g.dz + b * g.dz_sample + rows.t0 * g.dz_token;
+    const T* rp = (const T*)g.dr + b * g.dr_sample + rows.t0 * g.dr_token;
+    Raw<T, VPT> xr, yr, zr, rr;
+    auto fetch = [&] {
+        xr.ld(xp, h);
+        if (g.dz) zr.ld(zp, h);
+        if (a.y) yr.ld(yp, h);
+        if (g.dr) rr.ld(rp, h);
+        xp += a.x_token, yp += a.y_token, zp += g.dz_token, rp += g.dr_token;
+    };
+    if (rows.t0 < rows.t1) {
+        if (KEEP) {
+            if (a.y) ld_gate<VPT>(a, b, h, gate);
+            ld_mul<VPT>(a, b, h, mul);
+        }
+        fetch();
+    }
     for (int64_t t = rows.t0; t < rows.t1; ++t) {
         const int64_t row = b * a.tokens + t;
-        float rh[VPT], gz[VPT], yh[VPT], d[VPT], m[VPT];
-        ld_row<T, VPT>((const T*)a.x + b * a.x_sample + t * a.x_token, h, rh);
+        float rh[VPT], gz[VPT], yh[VPT], d[VPT];
+        const float s = a.rstd[row], mu = a.layer ? a.mean[row] : 0.f, q = a.post_weight ? a.post_rstd[row] : 1.f;
+        xr.get(h, rh);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) gz[i] = yh[i] = d[i] = 0.f;
-        if (g.dz) ld_row<T, VPT>((const T*)g.dz + b * g.dz_sample + t * g.dz_token, h, gz);
-        if (a.y) ld_row<T, VPT>((const T*)a.y + b * a.y_sample + t * a.y_token, h, yh);
-        if (g.dr) ld_row<T, VPT>((const T*)g.dr + b * g.dr_sample + t * g.dr_token, h, d);
-        const float s = a.rstd[row], mu = a.layer ? a.mean[row] : 0.f, q = a.post_weight ? a.post_rstd[row] : 1.f;
+        if (g.dz) zr.get(h, gz);
+        if (a.y) yr.get(h, yh);
+        if (g.dr) rr.get(h, d);
+        if (KEEP && t + 1 < rows.t1) fetch();
+        if (!KEEP) {
+            if (a.y) ld_gate<VPT>(a, b, h, gate);
+            ld_mul<VPT>(a, b, h, mul);
+        }
         if (a.y) {
-            ld_mods<VPT>(a.gate, a.mod_f32, b * a.gate_sample, h, m);
-            if (a.post_weight) {
-                float pw[VPT];
-                ld_row<float, VPT>(a.post_weight, h, pw);
 #pragma unroll
-                for (int i = 0; i < VPT; ++i) {
-                    m[i] *= 1.f + pw[i];
-                    yh[i] *= q;
-                }
+            for (int i = 0; i < VPT; ++i) {
+                if (a.post_weight) yh[i] *= q;
+                rh[i] = fmaf(gate[i], yh[i], a.alpha * rh[i]);
             }
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) rh[i] = fmaf(m[i], yh[i], a.alpha * rh[i]);
         }
-        float v[2] = {0.f, 0.f}, mul[VPT];
-        ld_mods<VPT>(a.scale, a.mod_f32, b * a.scale_sample, h, mul);
-        if (a.weight) {
-            float w[VPT];
-            ld_row<float, VPT>(a.weight, h, w);
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) mul[i] = (1.f + mul[i]) * (1.f + w[i]) - 1.f;
-        }
+        float v[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             rh[i] = (rh[i] - mu) * s;  // gz is zero behind the row
             S[i] = fmaf(gz[i], rh[i], S[i]);
             D1[i] += gz[i];
-            gz[i] = fmaf(gz[i], mul[i], gz[i]);
+            gz[i] *= mul[i];
             v[0] = fmaf(gz[i], rh[i], v[0]);
             v[1] += gz[i];
         }
@@ -580,20 +646,22 @@ __global__ void __launch_bounds__(512) resnorm_bwd_kernel(const Args a, const lq
             d[i] = fmaf(s, gz[i] - c0 - rh[i] * c1, d[i]);
             if (a.y) {
                 G[i] = fmaf(d[i], yh[i], G[i]);
-                gz[i] = m[i] * d[i];
+                gz[i] = gate[i] * d[i];
                 p[0] = fmaf(gz[i], yh[i], p[0]);  // yh is zero behind the row
                 d[i] *= a.alpha;
             }
         }
         if (g.dx) st_row<T, VPT>((T*)g.dx + row * h, h, d);
-        if (!a.y || !g.dy) continue;
-        if (a.post_weight) {
-            block_sum<MAXT, 1>(p, area, half);
-            const float pm = p[0] * inv_h;
+        if (a.y && g.dy) {
+            if (a.post_weight) {
+                block_sum<MAXT, 1>(p, area, half);
+                const float pm = p[0] * inv_h;
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) gz[i] = q * (gz[i] - yh[i] * pm);
+                for (int i = 0; i < VPT; ++i) gz[i] = q * (gz[i] - yh[i] * pm);
+            }
+            st_row<T, VPT>((T*)g.dy + row * h, h, gz);
         }
-        st_row<T, VPT>((T*)g.dy + row * h, h, gz);
+        if (!KEEP && t + 1 < rows.t1) fetch();
     }
     if (!part) return;
     float* dst = part + (int64_t)blockIdx.x * 3 * h;
@@ -685,12 +753,22 @@ int threads_of(int64_t h) { return (int)((h + 255) / 256 * 32); }  // 8 columns 
 // Blocks of an SM: 1024 threads with the forward's 64 registers, 768 with the backward's 80 (the launch bounds below).
 int blocks_per_sm(int64_t h, bool backward) { return std::max(1, (backward ? 768 : 1024) / threads_of(h)); }
 
+int scalar_ept(int64_t h) { return h <= 4096 ? 8 : (h <= 8192 ? 16 : 32); }
+int scalar_threads(int64_t h) {
+    const int64_t e = scalar_ept(h);
+    return (int)(((h + e - 1) / e + 31) / 32 * 32);
+}
+// ... and of the kernels for any rows: 128 registers, 64 in the forward up to 4096 columns
+int scalar_blocks_per_sm(int64_t h, bool backward) {
+    return std::max(1, (backward || scalar_ept(h) > 8 ? 512 : 1024) / scalar_threads(h));
+}
+
 // Chunks of one sample, one block each: such that all blocks fill the SMs' places once, or w times where one round
 // would leave too many empty (a round beyond the last full one costs as much as a whole one: 448 blocks on 444 places took
 // 292 us where 440 take 256, 8 x 4096 x 2048 forward and backward), but four rows or more each where that still gives every
 // SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
-int chunks_of(int64_t samples, int64_t tokens, int64_t h, int sms, bool backward) {
-    const int64_t places = (int64_t)sms * blocks_per_sm(h, backward), one = (sms + samples - 1) / samples;
+int chunks_of(int64_t samples, int64_t tokens, int64_t places, int sms) {
+    const int64_t one = (sms + samples - 1) / samples;
     const int64_t most = std::max<int64_t>(1, std::min(tokens, std::max(tokens / 4, one)));
     int64_t best = 1, cost = -1;
     for (int64_t w = 1; w <= 4; ++w) {
@@ -782,45 +860,55 @@ void launch_ring(int dev, unsigned grid, int threads, size_t smem, cudaStream_t 
         else if (a.layer) DIR(T, false, true, __VA_ARGS__);            \
         else DIR(T, false, false, __VA_ARGS__);                        \
     } while (0)
-// 8 elements a thread up to 4096 columns, then 16, then 32: blocks of at most 512 threads, 128 registers each
-#define LQ_SCALAR(KERN, ...)                                                                                                        \
-    do {                                                                                                                           \
-        const int ept = a.h <= 4096 ? 8 : (a.h <= 8192 ? 16 : 32);                                                                  \
-        const int threads = (int)(((a.h + ept - 1) / ept + 31) / 32 * 32);                                                          \
-        if (a.dtype == LQ_F32) {                                                                                                    \
-            if (ept == 8) KERN<float, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);                                                    \
-            else if (ept == 16) KERN<float, 16><<<grid, threads, 0, st>>>(__VA_ARGS__);                                             \
-            else KERN<float, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);                                                            \
-        } else {                                                                                                                    \
-            if (ept == 8) KERN<__nv_bfloat16, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);                                            \
-            else if (ept == 16) KERN<__nv_bfloat16, 16><<<grid, threads, 0, st>>>(__VA_ARGS__);                                     \
-            else KERN<__nv_bfloat16, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);                                                    \
-        }                                                                                                                           \
+// 8 elements a thread up to 4096 columns, then 16, then 32: blocks of at most 512 threads.
+#define LQ_SCALAR(KERN, ...)                                                                \
+    do {                                                                                   \
+        const int ept = scalar_ept(a.h), threads = scalar_threads(a.h);                     \
+        if (a.dtype == LQ_F32) {                                                            \
+            if (ept == 8) KERN<float, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);            \
+            else if (ept == 16) KERN<float, 16><<<grid, threads, 0, st>>>(__VA_ARGS__);     \
+            else KERN<float, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);                    \
+        } else {                                                                            \
+            if (ept == 8) KERN<__nv_bfloat16, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);    \
+            else if (ept == 16) KERN<__nv_bfloat16, 16><<<grid, threads, 0, st>>>(__VA_ARGS__); \
+            else KERN<__nv_bfloat16, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);            \
+        }                                                                                   \
     } while (0)
 
 constexpr int64_t kRingMaxH = 8192;  // 1024 threads x 8 columns
 
 void forward(const Args& a, int dev, cudaStream_t st) {
     const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype, inputs, false) : 0;
+    const int sms = lq_tc_sm_count(dev);
+    const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, false) : scalar_blocks_per_sm(a.h, false)), sms);
+    const int64_t per = (a.tokens + chunks - 1) / chunks;
+    LQ_CHECK_ARG(a.samples * chunks < (int64_t)1 << 31, "too many samples");
+    const unsigned grid = (unsigned)(a.samples * chunks);
     LqProf prof(LQ_K_PREP, st);
     if (stages) {
-        const int chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev), false), threads = threads_of(a.h);
-        const int64_t per = (a.tokens + chunks - 1) / chunks;
-        const unsigned grid = (unsigned)(a.samples * chunks);
+        const int threads = threads_of(a.h);
         const size_t smem = (size_t)std::min<int64_t>(stages, per) * inputs * a.h * (a.dtype == LQ_F32 ? 4 : 2);
         int* status = lq_tc_status_word(dev);
         if (a.dtype == LQ_F32) LQ_RING(LQ_RING_FWD, float, a, chunks, per, stages, status);
         else LQ_RING(LQ_RING_FWD, __nv_bfloat16, a, chunks, per, stages, status);
     } else {
-        const unsigned grid = (unsigned)(a.samples * a.tokens);
-        LQ_SCALAR(resnorm_fwd_kernel, a);
+        LQ_SCALAR(resnorm_fwd_kernel, a, chunks, per);
     }
     LQ_CUDA(cudaGetLastError());
 }
 
-void backward(const Args& a, const lq_residual_norm_grads& g, int chunks, float* part, int dev, cudaStream_t st) {
+// Most chunks of the backward, whichever kernel the rows take: what the workspace is sized for.
+int most_chunks(int64_t samples, int64_t tokens, int64_t h, int sms) {
+    return std::max(chunks_of(samples, tokens, (int64_t)sms * blocks_per_sm(h, true), sms),
+                    chunks_of(samples, tokens, (int64_t)sms * scalar_blocks_per_sm(h, true), sms));
+}
+
+// Returns the chunks that it used.
+int backward(const Args& a, const lq_residual_norm_grads& g, float* part, int dev, cudaStream_t st) {
     const int inputs = 1 + (a.y ? 1 : 0) + (g.dz ? 1 : 0) + (g.dr ? 1 : 0);
     const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype, inputs, true) : 0;
+    const int sms = lq_tc_sm_count(dev);
+    const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, true) : scalar_blocks_per_sm(a.h, true)), sms);
     const int64_t per = (a.tokens + chunks - 1) / chunks;
     const unsigned grid = (unsigned)(a.samples * chunks);
     LqProf prof(LQ_K_PREP, st);
@@ -834,6 +922,7 @@ void backward(const Args& a, const lq_residual_norm_grads& g, int chunks, float*
         LQ_SCALAR(resnorm_bwd_kernel, a, g, chunks, per, part);
     }
     LQ_CUDA(cudaGetLastError());
+    return chunks;
 }
 
 }  // namespace
@@ -857,7 +946,7 @@ int lq_residual_norm_fwd(const lq_residual_norm_args* args, void* stream) {
 size_t lq_residual_norm_workspace_bytes(int64_t samples, int64_t tokens, int64_t h) {
     if (samples < 1 || tokens < 1 || h < 1 || h > kMaxH) return 0;
     size_t n = 0;
-    if (guarded_call([&] { n = ws_bytes_of(samples, chunks_of(samples, tokens, h, lq_tc_sm_count(current_device()), true), h); }) != LQ_OK) return 0;
+    if (guarded_call([&] { n = ws_bytes_of(samples, most_chunks(samples, tokens, h, lq_tc_sm_count(current_device())), h); }) != LQ_OK) return 0;
     return n;
 }
 
@@ -883,14 +972,14 @@ int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_no
         LQ_CHECK_ARG(!g.dpost_weight || a.post_weight, "dpost_weight needs post_weight");
         LQ_CHECK_ARG(!g.dweight || a.weight, "dweight needs weight");
         LQ_CHECK_ARG(a.rstd && (!a.layer || a.mean) && (!a.post_weight || a.post_rstd), "the forward's statistics are needed");
-        const int dev = current_device(), chunks = chunks_of(a.samples, a.tokens, a.h, lq_tc_sm_count(dev), true);
-        LQ_CHECK_ARG(a.samples * chunks < (int64_t)1 << 31, "too many samples");
-        if (sums && (!ws || ws_bytes < ws_bytes_of(a.samples, chunks, a.h)))
+        const int dev = current_device(), most = most_chunks(a.samples, a.tokens, a.h, lq_tc_sm_count(dev));
+        LQ_CHECK_ARG(a.samples * most < (int64_t)1 << 31, "too many samples");
+        if (sums && (!ws || ws_bytes < ws_bytes_of(a.samples, most, a.h)))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the residual-norm backward");
         LQ_CHECK_ARG(!sums || al16(ws), "the workspace must be 16-byte aligned");
         LQ_CHECK_ARG(!sums || a.samples < 65535, "at most 65534 samples with gradients of the vectors");
         float* part = sums ? (float*)ws : nullptr;
-        backward(a, g, chunks, part, dev, st);
+        const int chunks = backward(a, g, part, dev, st);
         if (sums) {
             LqProf prof(LQ_K_REDUCE, st);
             const unsigned cols = (unsigned)((a.h + 31) / 32), b = (unsigned)a.samples;
