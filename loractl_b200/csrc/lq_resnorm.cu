@@ -154,6 +154,50 @@ __device__ __forceinline__ void st8(float* p, const float (&f)[8]) {
     *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
     *(float4*)(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
 }
+// Pairs of f32 in one 64-bit register pair: one instruction for two products or sums, each rounded as its scalar form
+// is.  A row's arithmetic was two thirds of the issue slots of the backward.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ f2 both(float v) { return pack2(v, v); }
+__device__ __forceinline__ void unpack2(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float sum2(f2 v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    return lo + hi;
+}
+template <typename T>
+__device__ __forceinline__ f2 pair_of(const Raw8<T>& r, int k) { return pack2(r[2 * k], r[2 * k + 1]); }
+template <typename T>
+__device__ __forceinline__ void st8(T* p, const f2 (&v)[4]) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) unpack2(v[k], f[2 * k], f[2 * k + 1]);
+    st8(p, f);
+}
+__device__ __forceinline__ void pack8(const float (&f)[8], f2 (&v)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
+}
+
 __device__ __forceinline__ void ld_mod8(const void* p, int f32, int64_t i, float (&f)[8]) {
     if (f32) ld8<float>((const uint8_t*)p + i * 4, f);
     else ld8<__nv_bfloat16>((const uint8_t*)p + i * 2, f);
@@ -206,66 +250,81 @@ __global__ void __launch_bounds__(MAXT, MINB) resnorm_fwd_ring_kernel(const Args
             for (int s = 0; s < min(stages, n); ++s) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
     }
     clear_area(area);
-    float gate[8], shift[8], mul[8], pw[8];  // of this thread's columns; mul = (1 + w)(1 + scale)
+    f2 gate[4] = {0, 0, 0, 0}, shift[4] = {0, 0, 0, 0}, mul[4] = {0, 0, 0, 0};  // of this thread's columns; mul = (1 + w)(1 + scale)
     if (in) {
-        float w[8];
-        ld_mod8(a.shift, a.mod_f32, rows.b * a.shift_sample + c, shift);
-        ld_mod8(a.scale, a.mod_f32, rows.b * a.scale_sample + c, mul);
+        float f[8], w[8];
+        ld_mod8(a.shift, a.mod_f32, rows.b * a.shift_sample + c, f);
+        pack8(f, shift);
+        ld_mod8(a.scale, a.mod_f32, rows.b * a.scale_sample + c, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mul[e] += 1.f;
+        for (int e = 0; e < 8; ++e) f[e] += 1.f;
         if (a.weight) {
             ld_mod8(a.weight, 1, c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mul[e] *= 1.f + w[e];
+            for (int e = 0; e < 8; ++e) f[e] *= 1.f + w[e];
         }
-        if (a.y) ld_mod8(a.gate, a.mod_f32, rows.b * a.gate_sample + c, gate);
+        pack8(f, mul);
+        if (a.y) ld_mod8(a.gate, a.mod_f32, rows.b * a.gate_sample + c, f);
         if (POST) {
-            ld_mod8(a.post_weight, 1, c, pw);
+            ld_mod8(a.post_weight, 1, c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate[e] *= 1.f + pw[e];
+            for (int e = 0; e < 8; ++e) f[e] *= 1.f + w[e];
         }
+        pack8(f, gate);
     }
     int half = 0, s = 0;
     uint32_t phase = 0;
     const int64_t row0 = rows.b * a.tokens + rows.t0;
     T *rp = (T*)a.r + row0 * h + c, *zp = (T*)a.z + row0 * h + c;
+    const f2 alpha = both(a.alpha);
     for (int i = 0; i < n; ++i) {
         const int64_t row = row0 + i;
         // a wait that gives up marks the error word; the block goes through its remaining rows without waiting
         umma::mbar_wait(umma::smem_u32(&bars[s]), phase, &abort_flag, status, 81);
         const uint8_t* st = ring_smem + s * stage_bytes + threadIdx.x * 8 * sizeof(T);
-        float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        float v[1] = {0.f};
-        if (in) ld8<T>(st, r);
-        if (a.y) {
-            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (in) ld8<T>(st + row_bytes, y);
-            float q = 1.f;
-            if (POST) {
+        f2 r[4];
+        float v[1];
+        {
+            Raw8<T> x, y;
+            x.zero();
+            y.zero();
+            if (in) x.ld(st);
+            if (in && a.y) y.ld(st + row_bytes);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[0] = fmaf(y[e], y[e], v[0]);
-                block_sum<MAXT, 1>(v, area, half);
-                q = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
-                if (threadIdx.x == 0 && a.rstd) a.post_rstd[row] = q;
-                v[0] = 0.f;
-            }
-            if (in) {
+            for (int k = 0; k < 4; ++k) r[k] = pair_of(x, k);
+            if (a.y) {
+                f2 q = both(1.f);
+                if (POST) {
+                    f2 sq = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) r[e] = fmaf(gate[e], POST ? y[e] * q : y[e], a.alpha * r[e]);
+                    for (int k = 0; k < 4; ++k) sq = fma2(pair_of(y, k), pair_of(y, k), sq);
+                    v[0] = sum2(sq);
+                    block_sum<MAXT, 1>(v, area, half);
+                    const float qs = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
+                    if (threadIdx.x == 0 && a.rstd) a.post_rstd[row] = qs;
+                    q = both(qs);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r[k] = fma2(gate[k], POST ? mul2(pair_of(y, k), q) : pair_of(y, k), mul2(alpha, r[k]));
             }
         }
         float mu = 0.f;
+        f2 d[4];
         if (LAYER) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[0] += r[e];
+            v[0] = sum2(add2(add2(r[0], r[1]), add2(r[2], r[3])));
             block_sum<MAXT, 1>(v, area, half);
             mu = v[0] * inv_h;
-            v[0] = 0.f;
-        }
-        if (in) {
+            const f2 m = both(-mu);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[0] = fmaf(r[e] - mu, r[e] - mu, v[0]);
+            for (int k = 0; k < 4; ++k) d[k] = add2(r[k], m);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[k] = r[k];
         }
+        f2 sq = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sq = fma2(d[k], d[k], sq);
+        v[0] = in ? sum2(sq) : 0.f;
         block_sum<MAXT, 1>(v, area, half);  // every thread has read the stage
         if (threadIdx.x < inputs && i + stages < n) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
         const float rs = rsqrt_f32(fmaf(v[0], inv_h, a.eps));
@@ -275,9 +334,10 @@ __global__ void __launch_bounds__(MAXT, MINB) resnorm_fwd_ring_kernel(const Args
         }
         if (in) {
             if (a.r) st8(rp, r);
+            const f2 rs2 = both(rs);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = fmaf((r[e] - mu) * rs, mul[e], shift[e]);
-            st8(zp, r);
+            for (int k = 0; k < 4; ++k) d[k] = fma2(mul2(d[k], rs2), mul[k], shift[k]);
+            st8(zp, d);
             rp += h;
             zp += h;
         }
@@ -320,99 +380,118 @@ __global__ void __launch_bounds__(MAXT, MINB) resnorm_bwd_ring_kernel(const Args
             for (int s = 0; s < min(stages, n); ++s) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
     }
     clear_area(area);
-    float gate[8], mul[8], S[8], D1[8], G[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) gate[e] = mul[e] = S[e] = D1[e] = G[e] = 0.f;
+    f2 gate[4] = {0, 0, 0, 0}, mul[4] = {0, 0, 0, 0}, S[4] = {0, 0, 0, 0}, D1[4] = {0, 0, 0, 0}, G[4] = {0, 0, 0, 0};
     if (in) {
-        ld_mod8(a.scale, a.mod_f32, rows.b * a.scale_sample + c, mul);
+        float f[8], w[8];
+        ld_mod8(a.scale, a.mod_f32, rows.b * a.scale_sample + c, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mul[e] += 1.f;
+        for (int e = 0; e < 8; ++e) f[e] += 1.f;
         if (a.weight) {
-            float w[8];
             ld_mod8(a.weight, 1, c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mul[e] *= 1.f + w[e];
+            for (int e = 0; e < 8; ++e) f[e] *= 1.f + w[e];
         }
-        if (a.y) ld_mod8(a.gate, a.mod_f32, rows.b * a.gate_sample + c, gate);
+        pack8(f, mul);
+        if (a.y) ld_mod8(a.gate, a.mod_f32, rows.b * a.gate_sample + c, f);
         if (POST) {  // gate (1 + pw) is all that the row needs; dgate gets its (1 + pw) with the sums
-            float pw[8];
-            ld_mod8(a.post_weight, 1, c, pw);
+            ld_mod8(a.post_weight, 1, c, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) gate[e] *= 1.f + pw[e];
+            for (int e = 0; e < 8; ++e) f[e] *= 1.f + w[e];
         }
+        if (a.y) pack8(f, gate);
     }
     int half = 0, s = 0;
     uint32_t phase = 0;
     const int64_t row0 = rows.b * a.tokens + rows.t0;
     T *dxp = (T*)g.dx + row0 * h + c, *dyp = (T*)g.dy + row0 * h + c;
     float rs = n > 0 ? a.rstd[row0] : 0.f, mu = n > 0 && LAYER ? a.mean[row0] : 0.f, q = n > 0 && POST ? a.post_rstd[row0] : 1.f;
+    const f2 alpha = both(a.y ? a.alpha : 1.f);
     for (int i = 0; i < n; ++i) {
         const int64_t row = row0 + i;
         umma::mbar_wait(umma::smem_u32(&bars[s]), phase, &abort_flag, status, 82);
         const uint8_t* st = ring_smem + s * stage_bytes + threadIdx.x * 8 * sizeof(T);
-        float rh[8], gz[8];
+        f2 rh[4], gz[4];
         Raw8<T> yr, dr;
         yr.zero();
         dr.zero();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) rh[e] = gz[e] = 0.f;
-        float v[2] = {0.f, 0.f};
-        if (in) {
-            ld8<T>(st, rh);
-            if (g.dz) ld8<T>(st + at_dz, gz);
-            if (a.y) {
-                yr.ld(st + at_y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) rh[e] = fmaf(gate[e], POST ? yr[e] * q : yr[e], a.alpha * rh[e]);
+        {
+            Raw8<T> x, z;
+            x.zero();
+            z.zero();
+            if (in) {
+                x.ld(st);
+                if (g.dz) z.ld(st + at_dz);
+                if (g.dr) dr.ld(st + at_dr);
+                if (a.y) yr.ld(st + at_y);
             }
+            const f2 q2 = both(q), rs2 = both(rs), m = both(-mu);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                rh[e] = LAYER ? (rh[e] - mu) * rs : rh[e] * rs;
-                S[e] = fmaf(gz[e], rh[e], S[e]);
-                D1[e] += gz[e];
-                gz[e] *= mul[e];
-                v[0] = fmaf(gz[e], rh[e], v[0]);
-                if (LAYER) v[1] += gz[e];
+            for (int k = 0; k < 4; ++k) {
+                rh[k] = mul2(alpha, pair_of(x, k));
+                if (a.y) rh[k] = fma2(gate[k], POST ? mul2(pair_of(yr, k), q2) : pair_of(yr, k), rh[k]);
+                if (LAYER) rh[k] = add2(rh[k], m);
+                rh[k] = mul2(rh[k], rs2);
+                gz[k] = pair_of(z, k);
             }
-            if (g.dr) dr.ld(st + at_dr);
         }
+        f2 dot = 0, sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            S[k] = fma2(gz[k], rh[k], S[k]);
+            D1[k] = add2(D1[k], gz[k]);
+            gz[k] = mul2(gz[k], mul[k]);
+            dot = fma2(gz[k], rh[k], dot);
+            if (LAYER) sum = add2(sum, gz[k]);
+        }
+        float c0 = 0.f, c1;
         if (LAYER) {
+            float v[2] = {sum2(dot), sum2(sum)};
             block_sum<MAXT, 2>(v, area, half);
+            c1 = v[0] * inv_h, c0 = v[1] * inv_h;
         } else {
-            float v1[1] = {v[0]};
-            block_sum<MAXT, 1>(v1, area, half);
-            v[0] = v1[0];
+            float v[1] = {sum2(dot)};
+            block_sum<MAXT, 1>(v, area, half);
+            c1 = v[0] * inv_h;
         }
         // every thread has read the stage
         if (threadIdx.x < inputs && i + stages < n) feed.fill(umma::smem_u32(&bars[s]), ring + s * stage_bytes, row_bytes, stage_bytes);
-        const float c1 = v[0] * inv_h, c0 = LAYER ? v[1] * inv_h : 0.f;
+        {
+            const f2 m0 = both(-c0), m1 = both(-c1), rs2 = both(rs);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rh[e] = fmaf(rs, gz[e] - c0 - rh[e] * c1, dr[e]);  // D
-        const float q_row = q;
+            for (int k = 0; k < 4; ++k) {
+                f2 t = LAYER ? add2(gz[k], m0) : gz[k];
+                rh[k] = fma2(rs2, fma2(rh[k], m1, t), pair_of(dr, k));  // D
+            }
+        }
+        const f2 q2 = both(q);
         if (i + 1 < n) {  // the next row's statistics, behind the stores of this one
             rs = a.rstd[row + 1];
             if (LAYER) mu = a.mean[row + 1];
             if (POST) q = a.post_rstd[row + 1];
         }
-        float p[1] = {0.f};
-        if (a.y && in) {
+        f2 p2 = 0;
+        if (a.y) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float yh = POST ? yr[e] * q_row : yr[e];
-                G[e] = fmaf(rh[e], yh, G[e]);
-                gz[e] = gate[e] * rh[e];  // the gradient of yh
-                if (POST) p[0] = fmaf(gz[e], yh, p[0]);
-                rh[e] *= a.alpha;
+            for (int k = 0; k < 4; ++k) {
+                const f2 yh = POST ? mul2(pair_of(yr, k), q2) : pair_of(yr, k);
+                G[k] = fma2(rh[k], yh, G[k]);
+                gz[k] = mul2(gate[k], rh[k]);  // the gradient of yh
+                if (POST) p2 = fma2(gz[k], yh, p2);
             }
         }
-        if (g.dx && in) st8(dxp, rh);
+        if (g.dx && in) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) rh[k] = mul2(alpha, rh[k]);
+            st8(dxp, rh);
+        }
         dxp += h;
         if (a.y && g.dy) {
             if (POST) {
+                float p[1] = {sum2(p2)};
                 block_sum<MAXT, 1>(p, area, half);
-                const float pm = p[0] * inv_h;
+                const f2 pm = both(-p[0] * inv_h);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) gz[e] = q_row * (gz[e] - yr[e] * q_row * pm);
+                for (int k = 0; k < 4; ++k) gz[k] = mul2(q2, fma2(mul2(pair_of(yr, k), q2), pm, gz[k]));
             }
             if (in) st8(dyp, gz);
             dyp += h;
