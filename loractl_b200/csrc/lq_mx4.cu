@@ -242,6 +242,7 @@ struct ProductParams {
     int m, n, kb;             // d_out, tokens, k-blocks of 256
     int w_tiles, x_tiles;     // 128 weight rows; BN tokens, which is 128 (a whole scale tile) when there are several
     int splits;               // blocks of a tile: ranges of the reduction, one cluster
+    int early_w;              // the launch before this one is known not to write the weight (it quantises x)
     const float* bias;
     void* y;
     int y_f32;
@@ -335,11 +336,12 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
                 tma_load_2d(smem_u32(smem_a + (size_t)st * C::A_BYTES), &tmW, bar, kb * 128, wt * 128);
                 bulk_load(smem_u32(smem_s + (size_t)st * 2 * C::S_BYTES), p.w_scales + ((int64_t)wt * kt + 2 * kb) * kTile, C::S_BYTES, bar);
             };
-            // the weight does not depend on the launch before this one (the quantisation of x): its first stages
-            // are fetched while that runs
+            // behind the quantisation of x, the weight's first stages are fetched while that runs; behind any other
+            // launch (which may be the weight's own quantisation) nothing is read before it has ended
+            if (!p.early_w) lqstream::pdl_wait();
             const int ahead = min(STAGES, k1 - k0);
             for (int i = 0; i < ahead; ++i) load_w(i, k0 + i);
-            lqstream::pdl_wait();
+            if (p.early_w) lqstream::pdl_wait();
             int s = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -867,7 +869,7 @@ void quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, voi
 }
 
 void product(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
-             const float* bias, void* y, int y_dtype, int dev, cudaStream_t st) {
+             const float* bias, void* y, int y_dtype, bool early_w, int dev, cudaStream_t st) {
     const int sms = lq_tc_sm_count(dev), bn = bn_of(n);
     ProductParams p;
     p.w_scales = (const uint8_t*)w_scales;
@@ -878,6 +880,7 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
     p.w_tiles = (int)((m + 127) / 128);
     p.x_tiles = (int)((n + bn - 1) / bn);
     p.splits = splits_of((int64_t)p.w_tiles * p.x_tiles, p.kb, sms);
+    p.early_w = early_w;
     p.bias = bias;
     p.y = y;
     p.y_f32 = y_dtype == LQ_F32;
@@ -939,7 +942,7 @@ int lq_mx4_matmul(const void* x_codes, const void* x_scales, int64_t n, const vo
         check_tensor(x_codes, x_scales);
         check_tensor(w_codes, w_scales);
         LQ_CHECK_ARG(y != nullptr, "NULL argument");
-        product(x_codes, x_scales, n, w_codes, w_scales, m, k, bias, y, y_dtype, current_device(), (cudaStream_t)stream);
+        product(x_codes, x_scales, n, w_codes, w_scales, m, k, bias, y, y_dtype, false, current_device(), (cudaStream_t)stream);
     });
 }
 
@@ -965,7 +968,7 @@ int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* 
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled linear");
         uint8_t* codes = (uint8_t*)ws;
         quantize(x, dtype, n, k, ldx, codes, codes + cb, dev, (cudaStream_t)stream);
-        product(codes, codes + cb, n, w_codes, w_scales, m, k, bias, y, dtype, dev, (cudaStream_t)stream);
+        product(codes, codes + cb, n, w_codes, w_scales, m, k, bias, y, dtype, true, dev, (cudaStream_t)stream);
     });
 }
 

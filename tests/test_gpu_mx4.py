@@ -231,6 +231,61 @@ def test_two_streams_capture_and_determinism():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_operands_of_the_launch_before(n):
+    """A product right behind the quantisation of its weight, and a linear right behind it, read what that wrote: the
+    product's launch may start early, its reads may not."""
+    import loractl_b200 as lb
+
+    x = sample(n, 4096, BF, seed=8)
+    xq = lb.mx4_quantize(x)
+    for seed in range(4):
+        w = sample(6000, 4096, BF, seed=10 + seed)
+        lb.mx4_quantize(sample(6000, 4096, BF, seed=20 + seed))  # leaves other codes where the next allocation may lie
+        torch.cuda.synchronize()
+        wq = lb.mx4_quantize(w)
+        y = lb.mx4_matmul_t(xq, wq)
+        wq2 = lb.mx4_quantize(w)
+        z = lb.Mx4Linear(wq2)(x)
+        torch.cuda.synchronize()
+        want = lb.mx4_matmul_t(xq, wq)
+        assert torch.equal(y, want) and torch.equal(z, want)
+
+
+CAPTURE_BESIDE_EAGER = """
+import torch
+import loractl_b200 as lb
+from loractl_b200.block_ops import gated_residual_norm
+x = torch.randn(2, 8, 64, device="cuda", requires_grad=True)
+mods = [torch.randn(2, 1, 64, device="cuda", requires_grad=True) for _ in range(3)]
+layer = lb.Mx4Linear(lb.mx4_quantize(torch.randn(32, 64, device="cuda")))
+for op in (lambda: gated_residual_norm(x, mods[0], x, mods[1], mods[2])[1], lambda: layer(x)):
+    living = op()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            op().sum().backward()
+    except RuntimeError as e:
+        assert "capture" in str(e), e
+    torch.cuda.synchronize()
+    assert torch.isfinite(op()).all() and torch.isfinite(torch.autograd.grad(living.sum(), x)[0]).all()
+print("usable")
+"""
+
+
+@pytest.mark.gpu
+def test_capture_beside_a_living_eager_graph_ends_in_an_error():
+    """A backward pass captured while an eager graph of the same leaves lives is torch's error about the capture, as with
+    torch's own operators: the process, the context and the eager graph stay usable."""
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+
+    r = subprocess.run([sys.executable, "-c", CAPTURE_BESIDE_EAGER], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "usable" in r.stdout, r.stdout[-1000:] + r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_gpu():
     import loractl_b200 as lb
 
