@@ -298,7 +298,8 @@ int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* 
 
 /* dX[n, k] = dY[n, m] . W[m, k]: the gradient through the frozen weight (that of crates/loractl-core/src/
  * quant.rs:221-235), with the quantisation of x taken as the identity.  dy, dx contiguous, 16-byte aligned, LQ_BF16
- * (W is exact in bf16) or LQ_F32 (f32 arithmetic).  `ws`: lq_mx4_matmul_dx_workspace_bytes() bytes, 256-byte aligned. */
+ * (W is exact in bf16) or LQ_F32 (dy as three bf16 terms whose sum it is, each multiplied with f32 accumulation: products
+ * are exact, so this is an f32 product).  `ws`: lq_mx4_matmul_dx_workspace_bytes() bytes, 256-byte aligned. */
 size_t lq_mx4_matmul_dx_workspace_bytes(int64_t n, int64_t m, int64_t k, int dtype);
 int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
                      int64_t k, void* dx, void* ws, size_t ws_bytes, void* stream);

@@ -229,6 +229,8 @@ def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, sh
     vector); `weight`, `post_weight`: `[h]` or None; h <= 16384.  `norm`: "zrms" (mmdit.rs:282-330) or "layer".
     Arithmetic is f32, `z` comes from the unrounded `r`, each output is rounded once; one kernel forward, one plus a
     fixed-order sum over tokens backward, gradients to every tensor argument that asks for one."""
+    if gate is None or y is None:
+        raise ValueError("gate and y are needed: modulated_zrmsnorm is the norm alone")
     if norm not in ("zrms", "layer"):
         raise ValueError(f"norm must be zrms or layer, got {norm!r}")
     eps = ZRMS_EPS if norm == "zrms" else LN_EPS

@@ -739,6 +739,30 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __nv_bfloat16* __re
     }
 }
 
+// [n, m] f32 as three stacked bf16 matrices [3, n, ld] whose sum it is: each takes the eight leading bits of what the one
+// before left, cut and not rounded, so nothing overflows and the third is exact too.  An Inf or a NaN goes to the first.
+__global__ void __launch_bounds__(256) split3_kernel(const float* __restrict__ in, int64_t n, int64_t m, int64_t ld,
+                                                     __nv_bfloat16* __restrict__ out) {
+    const int64_t total = n * ld;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / ld, c = i - r * ld;
+        const float v = c < m ? in[r * m + c] : 0.f;
+        float rest = v;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            float part = __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
+            if (k == 0 && isnan(v)) part = v;
+            out[k * total + i] = __float2bfloat16(part);
+            rest = isfinite(v) ? rest - part : 0.f;
+        }
+    }
+}
+// out = c[0] + (c[1] + c[2]), [3, n] f32 in.
+__global__ void __launch_bounds__(256) join3_kernel(const float* __restrict__ c, int64_t n, float* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+        out[i] = c[i] + (c[n + i] + c[2 * n + i]);
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 
 template <typename F>
@@ -854,6 +878,21 @@ void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int6
 }
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// The backward's workspace: the weight in bf16, dy's rows where they have to be copied (f32: three bf16 terms), and the
+// f32 products of those terms.
+struct DxSpace {
+    int64_t ld;  // of the copied rows: the tensor maps want 16 bytes
+    size_t rows, three, bytes;
+};
+DxSpace dx_space(int64_t n, int64_t m, int64_t k, int dtype) {
+    DxSpace s;
+    s.ld = (m + 7) / 8 * 8;
+    s.rows = al256((size_t)m * k * 2);
+    s.three = s.rows + (dtype == LQ_F32 ? al256((size_t)3 * n * s.ld * 2) : (s.ld != m ? al256((size_t)n * s.ld * 2) : 0));
+    s.bytes = s.three + (dtype == LQ_F32 ? (size_t)3 * n * k * 4 : 0);
+    return s;
+}
 
 void quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, void* codes, void* scales, int dev, cudaStream_t st) {
     const int64_t pad = row_tiles(rows) * 128;
@@ -974,8 +1013,7 @@ int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* 
 
 size_t lq_mx4_matmul_dx_workspace_bytes(int64_t n, int64_t m, int64_t k, int dtype) {
     if (n < 1 || m < 1 || k < 32) return 0;
-    const size_t w = (size_t)m * k * (dtype == LQ_F32 ? 4 : 2);
-    return al256(w) + (dtype == LQ_BF16 && m % 8 ? (size_t)n * ((m + 7) / 8 * 8) * 2 : 0);
+    return dx_space(n, m, k, dtype).bytes;
 }
 
 int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k, void* dx,
@@ -996,28 +1034,33 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
         LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
         if (ws_bytes < lq_mx4_matmul_dx_workspace_bytes(n, m, k, dtype))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled backward");
-        if (lq_mx4_dequantize(w_codes, w_scales, m, k, ws, dtype, stream) != LQ_OK) throw LqError(LQ_ERR_CUDA, lq_last_error());
+        if (lq_mx4_dequantize(w_codes, w_scales, m, k, ws, LQ_BF16, stream) != LQ_OK) throw LqError(LQ_ERR_CUDA, lq_last_error());
+        const DxSpace sp = dx_space(n, m, k, dtype);
+        const int sms = lq_tc_sm_count(current_device());
+        __nv_bfloat16* rows = (__nv_bfloat16*)((uint8_t*)ws + sp.rows);
         if (dtype == LQ_F32) {
-            LqSimtArgs a{};
-            a.A = dy, a.a_dtype = LQ_F32, a.sa_i = m, a.sa_k = 1;
-            a.b_mode = 0, a.Bp = ws, a.b_dtype = LQ_F32, a.sb_k = k, a.sb_j = 1;
-            a.C = dx, a.c_dtype = LQ_F32, a.ldc = k;
-            a.I = n, a.J = k, a.Kred = m, a.alpha = 1.f, a.beta = 0;
-            lq_launch_simt_gemm(a, st);
+            float* three = (float*)((uint8_t*)ws + sp.three);
+            {
+                LqProf prof(LQ_K_PREP, st);
+                split3_kernel<<<grid_of((n * sp.ld + 255) / 256, sms, 16), 256, 0, st>>>((const float*)dy, n, m, sp.ld, rows);
+                LQ_CUDA(cudaGetLastError());
+            }
+            lq_tc_gemm_nn(rows, sp.ld, ws, k, three, LQ_F32, 3 * n, k, m, st);
+            LqProf prof(LQ_K_REDUCE, st);
+            join3_kernel<<<grid_of((n * k + 255) / 256, sms, 16), 256, 0, st>>>(three, n * k, (float*)dx);
+            LQ_CUDA(cudaGetLastError());
             return;
         }
         const void* src = dy;
-        const int64_t ld = (m + 7) / 8 * 8;
-        if (ld != m || !al16(dy)) {
-            LQ_CHECK_ARG(ld != m, "dy must be 16-byte aligned");
-            __nv_bfloat16* padded = (__nv_bfloat16*)((uint8_t*)ws + al256((size_t)m * k * 2));
+        if (sp.ld != m) {
             LqProf prof(LQ_K_PREP, st);
-            pad_rows_kernel<<<grid_of((n * ld + 255) / 256, lq_tc_sm_count(current_device()), 16), 256, 0, st>>>(
-                (const __nv_bfloat16*)dy, n, m, ld, padded);
+            pad_rows_kernel<<<grid_of((n * sp.ld + 255) / 256, sms, 16), 256, 0, st>>>((const __nv_bfloat16*)dy, n, m, sp.ld, rows);
             LQ_CUDA(cudaGetLastError());
-            src = padded;
+            src = rows;
+        } else {
+            LQ_CHECK_ARG(al16(dy), "dy must be 16-byte aligned");
         }
-        lq_tc_gemm_nn(src, ld, ws, k, dx, n, k, m, st);
+        lq_tc_gemm_nn(src, sp.ld, ws, k, dx, LQ_BF16, n, k, m, st);
     });
 }
 

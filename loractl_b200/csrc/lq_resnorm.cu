@@ -1056,17 +1056,18 @@ int lq_residual_norm_bwd(const lq_residual_norm_args* args, const lq_residual_no
         if (sums && (!ws || ws_bytes < ws_bytes_of(a.samples, most, a.h)))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the residual-norm backward");
         LQ_CHECK_ARG(!sums || al16(ws), "the workspace must be 16-byte aligned");
-        LQ_CHECK_ARG(!sums || a.samples < 65535, "at most 65534 samples with gradients of the vectors");
         float* part = sums ? (float*)ws : nullptr;
         const int chunks = backward(a, g, part, dev, st);
         if (sums) {
             LqProf prof(LQ_K_REDUCE, st);
-            const unsigned cols = (unsigned)((a.h + 31) / 32), b = (unsigned)a.samples;
+            const unsigned cols = (unsigned)((a.h + 31) / 32);
             const bool weights = a.samples > 1 && (g.dweight || g.dpost_weight);
             // the weights' sums over many partial rows would be one block's work per 32 columns: over the samples' totals instead
             float* totals = weights && a.samples * chunks > 64 ? part + (size_t)a.samples * chunks * 3 * a.h : nullptr;
-            resnorm_final_kernel<<<dim3(cols, b + (weights && !totals ? 1 : 0)), 512, 0, st>>>(a, g, chunks, part, totals, 0);
-            if (totals) resnorm_final_kernel<<<dim3(cols, 1), 512, 0, st>>>(a, g, 1, totals, nullptr, (int)b);
+            const int64_t places = a.samples + (weights && !totals ? 1 : 0);
+            for (int64_t first = 0; first < places; first += 65535)  // the grid's second axis
+                resnorm_final_kernel<<<dim3(cols, (unsigned)std::min<int64_t>(65535, places - first)), 512, 0, st>>>(a, g, chunks, part, totals, (int)first);
+            if (totals) resnorm_final_kernel<<<dim3(cols, 1), 512, 0, st>>>(a, g, 1, totals, nullptr, (int)a.samples);
             LQ_CUDA(cudaGetLastError());
         }
     });

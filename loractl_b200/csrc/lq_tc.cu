@@ -787,8 +787,20 @@ DevCtx& dev_ctx(int dev) {
     DevCtx& c = ctx[dev];
     if (!c.status) {
         LQ_CUDA(cudaDeviceGetAttribute(&c.sm_count, cudaDevAttrMultiProcessorCount, dev));
-        LQ_CUDA(cudaMalloc((void**)&c.status, sizeof(int)));
-        LQ_CUDA(cudaMemset(c.status, 0, sizeof(int)));
+        // on a stream of its own and with the thread's capture mode relaxed, so that a first call made under a
+        // stream capture works
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        LQ_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        int* word = nullptr;
+        cudaStream_t own = nullptr;
+        cudaError_t e = cudaMalloc((void**)&word, sizeof(int));
+        if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+        if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), own);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+        if (own) cudaStreamDestroy(own);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) throw LqError(LQ_ERR_CUDA, std::string("device context: ") + cudaGetErrorString(e));
+        c.status = word;
     }
     return c;
 }
@@ -1975,12 +1987,14 @@ void lq_tc_gemm_bf16(const void* A, int a_mn, int64_t lda, const void* B, int b_
     throw LqError(LQ_ERR_UNSUPPORTED, "gemm: this (block_n, operand major) combination is not built");
 }
 
-void lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int64_t Mg, int64_t Ng, int64_t Kg,
-                   cudaStream_t st) {
+void lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int c_dtype, int64_t Mg, int64_t Ng,
+                   int64_t Kg, cudaStream_t st) {
     int dev;
     LQ_CUDA(cudaGetDevice(&dev));
     const Operand a{A, false, lda}, b{B, true, ldb};
-    if (pair_enabled() && Mg >= 256 && Ng > 192 && dev_ctx(dev).sm_count >= 2)
+    if (c_dtype == LQ_F32)
+        launch_gemm<128, false, true, float>(a, b, Kg, nullptr, nullptr, 0, (float*)C, Ng, 0, Mg, Ng, 1, nullptr, st);
+    else if (pair_enabled() && Mg >= 256 && Ng > 192 && dev_ctx(dev).sm_count >= 2)
         launch_gemm_pair<256, false, true>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, Mg, Ng, nullptr, st);
     else
         launch_gemm<128, false, true, __nv_bfloat16>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, 0, Mg, Ng, 1, nullptr, st);

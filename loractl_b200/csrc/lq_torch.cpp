@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
@@ -53,10 +54,14 @@ inline bool wants_grad(std::initializer_list<const Tensor*> inputs) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
-inline void once(const variable_list& grads, const char* name) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor& g : grads)
-        TORCH_CHECK(!g.defined() || !g.requires_grad(), name, " is differentiable once only");
+// Gradients that are themselves to be differentiated (create_graph) fail when that is tried, as torch's
+// once_differentiable does.
+variable_list once(variable_list&& grads, const char* name) {
+    if (!at::GradMode::is_enabled()) return std::move(grads);
+    variable_list marked;
+    for (const Tensor& g : grads) marked.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once only", (int64_t)grads.size());
+    return (*error)(std::move(marked));
 }
 
 // ---- residual norm ----------------------------------------------------------------------------------
@@ -106,7 +111,9 @@ struct ResidualNormBackward : public Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         TORCH_CHECK(!released, "Trying to backward through the graph a second time: specify retain_graph=True");
-        once(grads, "gated_residual_norm");
+        return once(gradients(std::move(grads)), "gated_residual_norm");
+    }
+    variable_list gradients(variable_list&& grads) {
         variable_list out(7);
         Tensor dr = two ? grads[0] : Tensor(), dz = grads[two ? 1 : 0];
         if (!dr.defined() && !dz.defined()) return out;
@@ -175,6 +182,7 @@ std::vector<Tensor> residual_norm(const Tensor& x_, const std::optional<Tensor>&
                          " of gate, shift or scale: f32 or bf16");
         if (v->scalar_type() != type) type = at::kFloat;
     }
+    TORCH_CHECK_VALUE(y0.defined() == gate0.defined(), "gate and y go together");
     const bool grad = wants_grad({&x_, &gate0, &y0, &shift_, &scale_, &weight0, &post0});
     Tensor x, y, gate, shift, scale, w, pw, r, z, stats;
     c10::cuda::OptionalCUDAGuard guard(x_.device());
@@ -372,8 +380,8 @@ std::pair<Tensor, Tensor> mx4_quantize(const Tensor& x_) {
 }
 
 Tensor mx4_dequantize(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t k, at::ScalarType dtype) {
-    c10::cuda::OptionalCUDAGuard guard(codes.device());
     require_cuda(codes, "codes");
+    c10::cuda::OptionalCUDAGuard guard(codes.device());
     Tensor out = at::empty({rows, k}, codes.options().dtype(dtype));
     check(lq_mx4_dequantize(ptr(codes), ptr(scales), rows, k, mut(out), dtype_code(out), stream_of(codes)));
     return out;
@@ -422,10 +430,13 @@ struct Mx4LinearBackward : public Node {
 
     std::string name() const override { return "Mx4LinearBackward"; }
     variable_list apply(variable_list&& grads) override {
-        once(grads, "Mx4Linear");
+        const bool asked = at::GradMode::is_enabled();
         if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+        at::NoGradGuard no_grad_in_here;
         const Tensor dy = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, m});
-        return {mx4_matmul_dx(dy, codes, scales, m, k).view(shape)};
+        variable_list out = {mx4_matmul_dx(dy, codes, scales, m, k).view(shape)};
+        at::AutoGradMode as_asked(asked);
+        return once(std::move(out), "Mx4Linear");
     }
 };
 

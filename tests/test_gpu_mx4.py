@@ -5,7 +5,7 @@ Tolerances.  Quantisation is exact arithmetic and one rounding: equal.  Products
 exact; the tensor core adds 64 of them at a time onto an f32 accumulator, and each such step may round (or cut) the
 sum twice by 2^-23 of what has been added up, so (2 k / 64 + 8) 2^-23 of sum |x w| bounds the f32 result, joined ranges
 included; a bf16 output adds half a step, 2^-8 of its value.  The bf16 gradient's reduction runs over d_out in steps
-of 16 with the same reasoning; the f32 gradient adds one product at a time: d_out 2^-24 of sum |dy w|."""
+of 16 with the same reasoning; the f32 gradient has the bound of adding one product at a time, d_out 2^-24 of sum |dy w|."""
 import pytest
 import torch
 
@@ -250,6 +250,72 @@ def test_operands_of_the_launch_before(n):
         torch.cuda.synchronize()
         want = lb.mx4_matmul_t(xq, wq)
         assert torch.equal(y, want) and torch.equal(z, want)
+
+
+@pytest.mark.gpu
+def test_f32_gradient_over_the_whole_range():
+    """dy from the smallest normal numbers to the largest, cut into three bf16 terms without overflow; Inf and NaN stay in
+    their rows."""
+    import loractl_b200 as lb
+
+    w = lb.mx4_quantize(sample(96, 64, F, seed=30).clamp(-1, 1) * 2.0 ** -8)
+    dy = torch.randn(6, 96, device="cuda")
+    dy[0] *= 1e30
+    dy[1, ::2], dy[1, 1::2] = 3.4e38, -3.3e38
+    dy[2] *= 1e-30
+    dy[3, 5], dy[4, 7] = float("inf"), float("nan")
+    dx = lb.mx4_matmul_dx(dy, w)
+    wd = w.dequantize().double()
+    ref, mag = dy.double() @ wd, dy.double().abs() @ wd.abs()
+    ok = [0, 1, 2, 5]
+    assert bool(((dx.double() - ref)[ok].abs() <= 100 * 2.0 ** -24 * mag[ok]).all())
+    assert torch.equal(torch.isnan(dx[4]), torch.isnan(ref[4])) and not torch.isfinite(dx[3]).any()
+
+
+@pytest.mark.gpu
+def test_layer_is_differentiable_once():
+    import loractl_b200 as lb
+
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    layer = lb.Mx4Linear(lb.mx4_quantize(torch.randn(32, 64, device="cuda")))
+    (dx,) = torch.autograd.grad(layer(x).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dx.sum().backward()
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+import loractl_b200 as lb
+from loractl_b200.block_ops import gated_residual_norm
+torch.manual_seed(0)
+x = torch.randn(2, 8, 256, device="cuda")
+mods = [torch.randn(2, 1, 256, device="cuda") for _ in range(3)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    r, z = gated_residual_norm(x, mods[0], x, mods[1], mods[2])
+    y = lb.Mx4Linear(lb.mx4_quantize(z[0]))(z)
+    norm = lb.clip_grad_norm([y, r], 1.0)
+graph.replay()
+torch.cuda.synchronize()
+r2, z2 = gated_residual_norm(x, mods[0], x, mods[1], mods[2])
+y2 = lb.Mx4Linear(lb.mx4_quantize(z2[0]))(z2)
+norm2 = lb.clip_grad_norm([y2, r2], 1.0)
+assert torch.equal(z, z2) and torch.equal(y, y2) and torch.equal(r, r2) and torch.equal(norm, norm2)
+lb.check_device_status()
+print("same")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout[-1000:] + r.stderr[-2000:]
 
 
 CAPTURE_BESIDE_EAGER = """

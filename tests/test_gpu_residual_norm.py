@@ -53,7 +53,8 @@ def close(ours, ref, dtype, summed=None, what=""):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,t,h", SHAPES)
-@pytest.mark.parametrize("dtype,mod", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("dtype,mod", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                       (torch.float32, torch.bfloat16)])
 @pytest.mark.parametrize("norm,post,alpha", [("zrms", False, 1.0), ("layer", False, 0.5), ("zrms", True, 0.8125), ("layer", True, 1.0)])
 def test_values_and_gradients_match_the_formulas(b, t, h, dtype, mod, norm, post, alpha):
     from loractl_b200.block_ops import gated_residual_norm
@@ -238,6 +239,49 @@ def test_captured_forward_and_backward_replay():
 
 
 @pytest.mark.gpu
+def test_many_samples():
+    """More samples than a grid's second axis has places, one token each: every sample's own sums, and the weight's over all."""
+    from loractl_b200.block_ops import modulated_zrmsnorm
+
+    b, h = 70_001, 8
+    v = make(b, 1, h, torch.float32, torch.float32, seed=8)
+    xs = [v[n].detach().requires_grad_(True) for n in ("x", "weight", "shift", "scale")]
+    z = modulated_zrmsnorm(*xs)
+    dx, dw, dshift, dscale = torch.autograd.grad(z, xs, v["dz"])
+    ref = {n: v[n].detach().double().requires_grad_(True) for n in ("x", "weight", "shift", "scale")}
+    _, rz = formula(ref, "zrms", False, 1.0, two=False)
+    rdx, rdw, rdshift, rdscale = torch.autograd.grad(rz, [ref[n] for n in ("x", "weight", "shift", "scale")], v["dz"].double())
+    close(z.detach(), rz.detach(), torch.float32, what="z")
+    close(dx, rdx, torch.float32, rdx.abs().max() * 4, "x")
+    assert torch.equal(dshift, v["dz"])
+    close(dscale, rdscale, torch.float32, rdscale.abs().max(), "scale")
+    c = v["x"].double()
+    rh = (c / (c.square().mean(-1, keepdim=True) + EPS).sqrt()).abs()
+    terms = (v["dz"].double().abs() * rh * (1 + v["scale"].detach().double()).abs()).sum((0, 1))
+    close(dw, rdw, torch.float32, terms, "weight")
+
+
+@pytest.mark.gpu
+def test_differentiable_once():
+    from loractl_b200.block_ops import gated_residual_norm
+
+    v = make(1, 4, 64, torch.float32, torch.float32)
+    x = v["x"].requires_grad_(True)
+    _, z = gated_residual_norm(x, v["gate"], v["y"], v["shift"], v["scale"])
+    (dx,) = torch.autograd.grad(z.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dx.sum().backward()
+    _, z = gated_residual_norm(x, v["gate"], v["y"], v["shift"], v["scale"])
+    z.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        z.sum().backward()
+    _, z = gated_residual_norm(x, v["gate"], v["y"], v["shift"], v["scale"])
+    v["y"].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+
+
+@pytest.mark.gpu
 def test_refusals():
     from loractl_b200 import _lib as L
     from loractl_b200.block_ops import gated_residual_norm, modulated_zrmsnorm
@@ -246,6 +290,8 @@ def test_refusals():
     args = [v[n] for n in ("x", "gate", "y", "shift", "scale")]
     with pytest.raises(ValueError, match="norm must be"):
         gated_residual_norm(*args, norm="batch")
+    with pytest.raises(ValueError, match="gate and y are needed"):
+        gated_residual_norm(args[0], args[1], None, *args[3:])
     with pytest.raises(ValueError, match="agree in shape and dtype"):
         gated_residual_norm(args[0], args[1], args[2].bfloat16(), *args[3:])
     with pytest.raises(ValueError, match="gate must be"):
