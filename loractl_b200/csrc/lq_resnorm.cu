@@ -844,11 +844,11 @@ int scalar_blocks_per_sm(int64_t h, bool backward) {
 
 // Chunks of one sample, one block each: such that all blocks fill the SMs' places once, or w times where one round
 // would leave too many empty (a round beyond the last full one costs as much as a whole one: 448 blocks on 444 places took
-// 292 us where 440 take 256, 8 x 4096 x 2048 forward and backward), but four rows or more each where that still gives every
-// SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
-int chunks_of(int64_t samples, int64_t tokens, int64_t places, int sms) {
+// 292 us where 440 take 256, 8 x 4096 x 2048 forward and backward); in the backward four rows or more each where that still
+// gives every SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
+int chunks_of(int64_t samples, int64_t tokens, int64_t places, int sms, bool backward) {
     const int64_t one = (sms + samples - 1) / samples;
-    const int64_t most = std::max<int64_t>(1, std::min(tokens, std::max(tokens / 4, one)));
+    const int64_t most = std::max<int64_t>(1, backward ? std::min(tokens, std::max(tokens / 4, one)) : tokens);
     int64_t best = 1, cost = -1;
     for (int64_t w = 1; w <= 4; ++w) {
         const int64_t c = std::min(most, std::max<int64_t>(1, places * w / samples));
@@ -959,7 +959,7 @@ constexpr int64_t kRingMaxH = 8192;  // 1024 threads x 8 columns
 void forward(const Args& a, int dev, cudaStream_t st) {
     const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype, inputs, false) : 0;
     const int sms = lq_tc_sm_count(dev);
-    const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, false) : scalar_blocks_per_sm(a.h, false)), sms);
+    const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, false) : scalar_blocks_per_sm(a.h, false)), sms, false);
     const int64_t per = (a.tokens + chunks - 1) / chunks;
     LQ_CHECK_ARG(a.samples * chunks < (int64_t)1 << 31, "too many samples");
     const unsigned grid = (unsigned)(a.samples * chunks);
@@ -978,8 +978,8 @@ void forward(const Args& a, int dev, cudaStream_t st) {
 
 // Most chunks of the backward, whichever kernel the rows take: what the workspace is sized for.
 int most_chunks(int64_t samples, int64_t tokens, int64_t h, int sms) {
-    return std::max(chunks_of(samples, tokens, (int64_t)sms * blocks_per_sm(h, true), sms),
-                    chunks_of(samples, tokens, (int64_t)sms * scalar_blocks_per_sm(h, true), sms));
+    return std::max(chunks_of(samples, tokens, (int64_t)sms * blocks_per_sm(h, true), sms, true),
+                    chunks_of(samples, tokens, (int64_t)sms * scalar_blocks_per_sm(h, true), sms, true));
 }
 
 // Returns the chunks that it used.
@@ -987,7 +987,7 @@ int backward(const Args& a, const lq_residual_norm_grads& g, float* part, int de
     const int inputs = 1 + (a.y ? 1 : 0) + (g.dz ? 1 : 0) + (g.dr ? 1 : 0);
     const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype, inputs, true) : 0;
     const int sms = lq_tc_sm_count(dev);
-    const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, true) : scalar_blocks_per_sm(a.h, true)), sms);
+    const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, true) : scalar_blocks_per_sm(a.h, true)), sms, true);
     const int64_t per = (a.tokens + chunks - 1) / chunks;
     const unsigned grid = (unsigned)(a.samples * chunks);
     LqProf prof(LQ_K_PREP, st);
