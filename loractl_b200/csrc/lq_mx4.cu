@@ -429,6 +429,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
             }
         }
     }
+    __syncwarp();  // the single-lane roles rejoin their warps before the aligned barriers
     if (p.splits > 1) {
         cluster_sync_all();
         const uint32_t part = smem_u32(smem);
@@ -723,6 +724,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         }
         if (lane == 0) bulk_wait0();
     }
+    __syncwarp();  // the single-lane roles rejoin their warps before the aligned barrier
     tc_fence_before();
     cluster_sync_all();
     if (warp == 1) {

@@ -88,11 +88,11 @@ __device__ __forceinline__ void clear_area(float (*area)[2][kMaxWarps]) {
     __syncthreads();
 }
 
-// 1 / sqrt(v): the hardware's estimate and one Newton step (the IEEE square root and quotient are forty
-// instructions that every thread of a row would run).
+// 1 / sqrt(v) for v >= eps: the hardware's estimate and one Newton step (the IEEE square root and quotient are forty
+// instructions that every thread of a row would run).  0 for a sum of squares that overflowed.
 __device__ __forceinline__ float rsqrt_f32(float v) {
     const float y = rsqrtf(v);
-    return y * fmaf(-0.5f * v * y, y, 1.5f);
+    return y == 0.f ? y : y * fmaf(-0.5f * v * y, y, 1.5f);
 }
 
 // The rows of one block: chunk `blockIdx.x % chunks` of a sample.

@@ -152,7 +152,7 @@ def _tensors(grads) -> Sequence[torch.Tensor]:
 def global_grad_norm(grads: Sequence[torch.Tensor], grad_scale: float = 1.0) -> torch.Tensor:
     """The 2-norm of all `grads` (f32 and bf16 tensors of any shape on one device) taken as one vector, times
     `|grad_scale|`, as an f32 device scalar: two launches for up to 128 tensors, no host synchronisation.  Squares and
-    sums are 64-bit; the norm is NaN or Inf exactly when some gradient is."""
+    sums are 64-bit: it is NaN or Inf when some gradient is, and otherwise only above the largest f32."""
     return L.ext().global_grad_norm(_tensors(grads), grad_scale)
 
 

@@ -239,6 +239,22 @@ def test_captured_forward_and_backward_replay():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("h", [64, 65])
+def test_rows_whose_squares_overflow(h):
+    """A row above 1.8e19 has an infinite sum of squares in f32: it normalises to zero, as the f32 tensor ops have it, and
+    touches no other row."""
+    from loractl_b200.block_ops import modulated_zrmsnorm
+
+    v = make(1, 5, h, torch.float32, torch.float32, seed=9)
+    v["x"][0, 2] *= 1e25
+    z = modulated_zrmsnorm(v["x"], v["weight"], v["shift"], v["scale"])
+    x = v["x"]
+    ref = x / (x.square().mean(-1, keepdim=True) + EPS).sqrt() * (1 + v["weight"]) * (1 + v["scale"]) + v["shift"]
+    assert torch.equal(z[0, 2], v["shift"][0, 0]) and torch.equal(ref[0, 2], z[0, 2])
+    assert float((z - ref).abs().max()) <= 1e-5 * float(ref.abs().max())
+
+
+@pytest.mark.gpu
 def test_many_samples():
     """More samples than a grid's second axis has places, one token each: every sample's own sums, and the weight's over all."""
     from loractl_b200.block_ops import modulated_zrmsnorm
