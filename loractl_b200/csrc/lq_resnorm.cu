@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(MAXT, MINB) resnorm_bwd_ring_kernel(const Args
 // Single elements, for rows that do not all start on 16 bytes (an odd width, an odd offset) and for rows too wide
 // for the ring: thread t owns the columns t, t + blockDim, ...  All of a row's loads are issued before the first is
 // used, whatever columns the thread has (a place behind the row reads column 0 and counts as zero).  Up to 4096 columns
-// (VPT = 8) the modulation stays in registers over the rows of a chunk and the next row is fetched into registers behind
+// (512 threads) the modulation stays in registers over the rows of a chunk and the next row is fetched into registers behind
 // the current one's arithmetic; wider rows have no registers for either.  Bound by instructions, two accesses and a dozen
 // of arithmetic an element: 8000 rows of 4001 f32 columns 152 us forward and 166 us backward (51 % and 71 % of HBM),
 // 24000 rows of 1155 bf16 columns 110 us and 153 us (31 % and 33 %; 1152 columns by the ring: 41 us and 69 us).
@@ -576,10 +576,9 @@ __device__ __forceinline__ void ld_mul(const Args& a, int64_t b, int h, float (&
     }
 }
 
-template <typename T, int VPT>
-__global__ void __launch_bounds__(512, VPT == 8 ? 2 : 1) resnorm_fwd_kernel(const Args a, int chunks, int64_t per) {
-    constexpr int MAXT = 512;
-    constexpr bool KEEP = VPT == 8;
+template <typename T, int VPT, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == 512 ? 2 : 1) resnorm_fwd_kernel(const Args a, int chunks, int64_t per) {
+    constexpr bool KEEP = MAXT == 512;
     __shared__ __align__(16) float area[2][2][kMaxWarps];
     int half = 0;
     const Rows rows(a.tokens, chunks, per);
@@ -655,11 +654,10 @@ __global__ void __launch_bounds__(512, VPT == 8 ? 2 : 1) resnorm_fwd_kernel(cons
     }
 }
 
-template <typename T, int VPT>
-__global__ void __launch_bounds__(512) resnorm_bwd_kernel(const Args a, const lq_residual_norm_grads g, int chunks, int64_t per,
-                                                          float* __restrict__ part) {
-    constexpr int MAXT = 512;
-    constexpr bool KEEP = VPT == 8;
+template <typename T, int VPT, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) resnorm_bwd_kernel(const Args a, const lq_residual_norm_grads g, int chunks, int64_t per,
+                                                              float* __restrict__ part) {
+    constexpr bool KEEP = MAXT == 512;
     __shared__ __align__(16) float area[2][2][kMaxWarps];
     int half = 0;
     const Rows rows(a.tokens, chunks, per);
@@ -810,7 +808,7 @@ __global__ void __launch_bounds__(512) resnorm_final_kernel(const Args a, const 
 
 // ---- host ---------------------------------------------------------------------------------------
 
-constexpr int64_t kMaxH = 16384;  // 512 threads x 32 elements
+constexpr int64_t kMaxH = 16384;  // 1024 threads x 16 elements
 constexpr size_t kRingBytes = 216 * 1024;  // shared memory of an SM for the rings of its blocks
 
 inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -836,15 +834,13 @@ int threads_of(int64_t h) { return (int)((h + 255) / 256 * 32); }  // 8 columns 
 // Blocks of an SM: 1024 threads with the forward's 64 registers, 768 with the backward's 80 (the launch bounds below).
 int blocks_per_sm(int64_t h, bool backward) { return std::max(1, (backward ? 768 : 1024) / threads_of(h)); }
 
-int scalar_ept(int64_t h) { return h <= 4096 ? 8 : (h <= 8192 ? 16 : 32); }
+// ... and of the kernels for any rows: 8 elements a thread in up to 512 threads (128 registers; 64 in the forward), then
+// up to 1024 threads, then 16 elements.
 int scalar_threads(int64_t h) {
-    const int64_t e = scalar_ept(h);
+    const int64_t e = h <= 8192 ? 8 : 16;
     return (int)(((h + e - 1) / e + 31) / 32 * 32);
 }
-// ... and of the kernels for any rows: 128 registers, 64 in the forward up to 4096 columns
-int scalar_blocks_per_sm(int64_t h, bool backward) {
-    return std::max(1, (backward || scalar_ept(h) > 8 ? 512 : 1024) / scalar_threads(h));
-}
+int scalar_blocks_per_sm(int64_t h, bool backward) { return std::max(1, (backward ? 512 : 1024) / scalar_threads(h)); }
 
 // Chunks of one sample, one block each: such that all blocks fill the SMs' places once, or w times where one round
 // would leave too many empty (a round beyond the last full one costs as much as a whole one: 448 blocks on 444 places took
@@ -943,19 +939,17 @@ void launch_ring(int dev, unsigned grid, int threads, size_t smem, cudaStream_t 
         else if (a.layer) DIR(T, false, true, __VA_ARGS__);            \
         else DIR(T, false, false, __VA_ARGS__);                        \
     } while (0)
-// 8 elements a thread up to 4096 columns, then 16, then 32: blocks of at most 512 threads.
-#define LQ_SCALAR(KERN, ...)                                                                \
-    do {                                                                                   \
-        const int ept = scalar_ept(a.h), threads = scalar_threads(a.h);                     \
-        if (a.dtype == LQ_F32) {                                                            \
-            if (ept == 8) KERN<float, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);            \
-            else if (ept == 16) KERN<float, 16><<<grid, threads, 0, st>>>(__VA_ARGS__);     \
-            else KERN<float, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);                    \
-        } else {                                                                            \
-            if (ept == 8) KERN<__nv_bfloat16, 8><<<grid, threads, 0, st>>>(__VA_ARGS__);    \
-            else if (ept == 16) KERN<__nv_bfloat16, 16><<<grid, threads, 0, st>>>(__VA_ARGS__); \
-            else KERN<__nv_bfloat16, 32><<<grid, threads, 0, st>>>(__VA_ARGS__);            \
-        }                                                                                   \
+#define LQ_SCALAR_T(KERN, T, ...)                                                              \
+    do {                                                                                      \
+        if (a.h <= 4096) KERN<T, 8, 512><<<grid, threads, 0, st>>>(__VA_ARGS__);               \
+        else if (a.h <= 8192) KERN<T, 8, 1024><<<grid, threads, 0, st>>>(__VA_ARGS__);         \
+        else KERN<T, 16, 1024><<<grid, threads, 0, st>>>(__VA_ARGS__);                         \
+    } while (0)
+#define LQ_SCALAR(KERN, ...)                                                                  \
+    do {                                                                                      \
+        const int threads = scalar_threads(a.h);                                              \
+        if (a.dtype == LQ_F32) LQ_SCALAR_T(KERN, float, __VA_ARGS__);                          \
+        else LQ_SCALAR_T(KERN, __nv_bfloat16, __VA_ARGS__);                                    \
     } while (0)
 
 constexpr int64_t kRingMaxH = 8192;  // 1024 threads x 8 columns
