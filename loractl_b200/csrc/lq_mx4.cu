@@ -74,6 +74,18 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __uint_as_float(bits);
 }
 
+// Two products an instruction, each rounded as its scalar form is.
+__device__ __forceinline__ void scale8(float (&f)[8], float s) {
+    asm("{\n\t.reg .b64 s, p;\n\t"
+        "mov.b64 s, {%8, %8};\n\t"
+        "mov.b64 p, {%0, %1};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {%0, %1}, p;\n\t"
+        "mov.b64 p, {%2, %3};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {%2, %3}, p;\n\t"
+        "mov.b64 p, {%4, %5};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {%4, %5}, p;\n\t"
+        "mov.b64 p, {%6, %7};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {%6, %7}, p;\n\t}"
+        : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7])
+        : "f"(s));
+}
+
 // Eight elements as they are stored, zeros where `in` is false; `vec`: they start on 16 bytes.
 template <typename T>
 struct In8 {
@@ -110,13 +122,14 @@ struct In8 {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (sizeof(T) == 4) {
-                    f[4 * i + j] = __uint_as_float(w[j]) * s;
+                    f[4 * i + j] = __uint_as_float(w[j]);
                 } else {
-                    f[2 * j] = __uint_as_float(w[j] << 16) * s;
-                    f[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u) * s;
+                    f[2 * j] = __uint_as_float(w[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
                 }
             }
         }
+        scale8(f, s);
     }
 };
 
@@ -192,8 +205,7 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint32_t* __r
             const float s = scale_value(byte[i]);
             float v[8];
             unpack_e2m1(w[i], v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= s;
+            scale8(v, s);
             T* o = out + at + i * 256;
             if (sizeof(T) == 4) {
                 ((float4*)o)[0] = make_float4(v[0], v[1], v[2], v[3]);
