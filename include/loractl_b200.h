@@ -304,6 +304,21 @@ size_t lq_mx4_matmul_dx_workspace_bytes(int64_t n, int64_t m, int64_t k, int dty
 int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
                      int64_t k, void* dx, void* ws, size_t ws_bytes, void* stream);
 
+/* A LoRA adapter on such a weight (crates/loractl-core/src/mmdit.rs:526-536), bf16 activations:
+ *   H = X . A,   Y = quant(X) . W^T + bias + scaling * H . B,
+ *   dX = dY . W + scaling * dY . B^T . A^T,   dA = scaling * X^T . dY . B^T,   dB = scaling * H^T . dY,
+ * the adapter reading X itself.  `mirror`: lq_lora_mirror_update() of the factors (A [k, rank], B [rank, m]); m a multiple of
+ * 8, rank <= 256; x, dy, y and dx contiguous, 16-byte aligned.  `h_out` / `h`: f32 [n, rank], may be NULL (the backward then
+ * computes it again).  dX, dA and dB may be NULL; `accumulate` adds to dA and dB.  `ws`: lq_mx4_lora_workspace_bytes() bytes,
+ * 256-byte aligned, of the forward or the backward; calls that can overlap need one each. */
+size_t lq_mx4_lora_workspace_bytes(int64_t n, int64_t m, int64_t k, int rank, int backward);
+int lq_mx4_lora_fwd(const void* x, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
+                    const float* bias, const void* mirror, int rank, float scaling, void* y, float* h_out, void* ws,
+                    size_t ws_bytes, void* stream);
+int lq_mx4_lora_bwd(const void* dy, const void* x, const float* h, int64_t n, const void* w_codes, const void* w_scales,
+                    int64_t m, int64_t k, const void* mirror, int rank, float scaling, void* dx, float* dA, float* dB,
+                    int accumulate, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- step glue on the flat LoRA buffers ---------------------------------------- */
 
 /* crates/loractl-core/src/diffusion_trainer.rs:1708-1725 (the finite check over every adapter

@@ -97,6 +97,9 @@ SIGNATURES = {
     "lq_mx4_linear": (_I, [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
     "lq_mx4_matmul_dx_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "lq_mx4_matmul_dx": (_I, [_P, _I, _I64, _P, _P, _I64, _I64, _P, _P, _SZ, _P]),
+    "lq_mx4_lora_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I]),
+    "lq_mx4_lora_fwd": (_I, [_P, _I64, _P, _P, _I64, _I64, _P, _P, _I, _F, _P, _P, _P, _SZ, _P]),
+    "lq_mx4_lora_bwd": (_I, [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I, _F, _P, _P, _P, _I, _P, _SZ, _P]),
     "lq_grad_nonfinite_flag": (_I, [_P, _I64, _P, _P]),
     "lq_adamw_step": (_I, [_P, _P, _P, _P, _I64, _F, _F, _F, _F, _F, _I64, _F, _P, _P]),
     "lq_adamw_step_clipped": (_I, [_P, _P, _P, _P, _I64, _F, _F, _F, _F, _F, _I64, _F, _P, _P, _P]),

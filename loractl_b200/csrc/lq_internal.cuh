@@ -39,7 +39,12 @@ struct lq_weight {
     size_t packed_bytes = 0, scale_bytes = 0;
     void* packed_t = nullptr;  // fp8 only: the bytes transposed to [d_in, d_out], built on first use
     const void* bf16_copy = nullptr;  // optional caller-owned bf16 [d_out, d_in] copy of the dequantised weight
+    const void* mx4_scales = nullptr;  // kSchemeMx4 only (`packed` holds the codes)
 };
+
+// A microscaled 4-bit weight passed to the tensor-core backward (lq_mx4.cu): no handle of the C ABI has this scheme.
+constexpr int kSchemeMx4 = 100;
+void lq_mx4_launch_dequant(const void* codes, const void* scales, int64_t rows, int64_t k, void* out, int out_dtype, cudaStream_t st);
 
 // Device-side view passed to kernels by value.
 struct LqWView {

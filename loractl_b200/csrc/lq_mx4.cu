@@ -254,6 +254,7 @@ struct ProductParams {
     int m, n, kb;             // d_out, tokens, k-blocks of 256
     int w_tiles, x_tiles;     // 128 weight rows; BN tokens, which is 128 (a whole scale tile) when there are several
     int splits;               // blocks of a tile: ranges of the reduction, one cluster
+    int lora;                 // k-blocks of 64 bf16 after those (pairs only): s * H against B^T
     int early_w;              // the launch before this one is known not to write the weight (it quantises x)
     const float* bias;
     void* y;
@@ -525,7 +526,8 @@ __device__ __forceinline__ void tile2(const ProductParams& p, int item, int& xt,
 template <bool TMA_OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmXs,
-                const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmY, ProductParams p) {
+                const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmH,
+                const __grid_constant__ CUtensorMap tmB, ProductParams p) {
     using C = Cfg2;
     constexpr int STAGES = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -573,6 +575,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int items = p.x_tiles * p.w_tiles, cid = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+    const int blocks = p.kb + p.lora;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -583,16 +586,22 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             for (int item = cid; ok && item < items; item += pairs) {
                 int xt, wt;
                 tile2(p, item, xt, wt);
-                for (int kb = 0; kb < p.kb; ++kb) {
+                for (int kb = 0; kb < blocks; ++kb) {
                     if (!mbar_wait(smem_u32(&empty[s]), phase ^ 1u, abort_flag, p.status, 75)) { ok = false; break; }
-                    const uint32_t bar = smem_u32(&full[s]);
+                    const uint32_t bar = smem_u32(&full[s]), sbar = smem_u32(&sfull[s]);
+                    const uint32_t sa = smem_u32(smem_a + (size_t)s * C::A_BYTES), sb = smem_u32(smem_b + (size_t)s * C::B_BYTES);
                     if (leader) mbar_expect_tx(bar, 2 * (C::A_BYTES + C::B_BYTES));
-                    tma_load_2d_pair(smem_u32(smem_a + (size_t)s * C::A_BYTES), &tmX, bar, kb * 128, xt * 256 + (int)rank * 128);
-                    tma_load_2d_pair(smem_u32(smem_b + (size_t)s * C::B_BYTES), &tmW, bar, kb * 128, wt * 256 + (int)rank * 128);
-                    const uint32_t sbar = smem_u32(&sfull[s]);
-                    mbar_expect_tx(sbar, C::SA_BYTES + C::SB_BYTES);
-                    tma_load_2d(smem_u32(smem_sa + (size_t)s * C::SA_BYTES), &tmXs, sbar, kb * 256, xt * 2 + (int)rank);
-                    tma_load_2d(smem_u32(smem_sb + (size_t)s * C::SB_BYTES), &tmWs, sbar, kb * 256, wt * 2);
+                    if (kb < p.kb) {
+                        tma_load_2d_pair(sa, &tmX, bar, kb * 128, xt * 256 + (int)rank * 128);
+                        tma_load_2d_pair(sb, &tmW, bar, kb * 128, wt * 256 + (int)rank * 128);
+                        mbar_expect_tx(sbar, C::SA_BYTES + C::SB_BYTES);
+                        tma_load_2d(smem_u32(smem_sa + (size_t)s * C::SA_BYTES), &tmXs, sbar, kb * 256, xt * 2 + (int)rank);
+                        tma_load_2d(smem_u32(smem_sb + (size_t)s * C::SB_BYTES), &tmWs, sbar, kb * 256, wt * 2);
+                    } else {  // 64 columns of s * H and of B^T: rows of 128 bytes as well
+                        tma_load_2d_pair(sa, &tmH, bar, (kb - p.kb) * 64, xt * 256 + (int)rank * 128);
+                        tma_load_2d_pair(sb, &tmB, bar, (kb - p.kb) * 64, wt * 256 + (int)rank * 128);
+                        mbar_arrive(sbar);
+                    }
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
@@ -609,17 +618,24 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 if (!mbar_wait(smem_u32(tempty), acc_phase ^ 1u, abort_flag, p.status, 76)) { ok = false; break; }
                 acc_phase ^= 1u;
                 tc_fence_after();
-                for (int kb = 0; kb < p.kb; ++kb) {
+                for (int kb = 0; kb < blocks; ++kb) {
                     if (!mbar_wait(smem_u32(&full[s]), phase, abort_flag, p.status, 77) ||
                         !mbar_wait(smem_u32(&scaled[s]), phase, abort_flag, p.status, 83)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 24, sfb = sfa + 8;
                     const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
                     const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
+                    if (kb < p.kb) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
-                        mma2_mxf4(tmem, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi), idesc_mxf4(256, 256, k & 1),
-                                  sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
+                        for (uint32_t k = 0; k < 4; ++k)
+                            mma2_mxf4(tmem, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi), idesc_mxf4(256, 256, k & 1),
+                                      sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
+                    } else {
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)  // 16 bf16 an instruction: 32 bytes along the row, as 64 codes are
+                            mma2_f16(tmem, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi),
+                                     make_idesc(1, 1, false, false, 256, 256), 1u);
+                    }
                     mma2_commit_mc(smem_u32(&empty[s]), 3);
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
@@ -633,17 +649,19 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         uint32_t phase = 0;
         bool ok = true;
         for (int item = cid; ok && item < items; item += pairs) {
-            for (int kb = 0; kb < p.kb; ++kb) {
+            for (int kb = 0; kb < blocks; ++kb) {
                 if (!mbar_wait(smem_u32(&sfull[s]), phase, abort_flag, p.status, 84)) { ok = false; break; }
                 const uint8_t *sa = smem_sa + (size_t)s * C::SA_BYTES, *sb = smem_sb + (size_t)s * C::SB_BYTES;
                 const uint32_t sfa = lanes + (uint32_t)s * 24, sfb = sfa + 8;
+                if (kb < p.kb) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {  // tiles of 128 elements; B's rows 0-127 and 128-255
-                    stage_scales(sfa + 4 * j, sa + j * kTile, lane);
-                    stage_scales(sfb + 8 * j, sb + j * kTile, lane);
-                    stage_scales(sfb + 8 * j + 4, sb + (2 + j) * kTile, lane);
+                    for (int j = 0; j < 2; ++j) {  // tiles of 128 elements; B's rows 0-127 and 128-255
+                        stage_scales(sfa + 4 * j, sa + j * kTile, lane);
+                        stage_scales(sfb + 8 * j, sb + j * kTile, lane);
+                        stage_scales(sfb + 8 * j + 4, sb + (2 + j) * kTile, lane);
+                    }
+                    tmem_st_wait();
                 }
-                tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -857,6 +875,12 @@ void launch_stream(const ProductParams& p, const void* w_codes, const void* x_co
     LQ_CUDA(cudaLaunchKernelEx(&cfg, mx4_stream_kernel<BN>, tw, tx, p));
 }
 
+// Of a LoRA product that the pair kernel adds: s * H [n, ext] and B^T [m, ext] in bf16, zero beyond the rank.
+struct LoraOperands {
+    const __nv_bfloat16 *h, *bt;
+    int ext;
+};
+
 // Pairs that can be resident at once, asked once per device.
 int resident_pairs(int dev, int sms) {
     static std::mutex mu;
@@ -875,12 +899,16 @@ int resident_pairs(int dev, int sms) {
     return known[dev & 63];
 }
 
-void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int64_t k, int dev, int sms, cudaStream_t st) {
+void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int64_t k, const LoraOperands* lora, int dev, int sms,
+                 cudaStream_t st) {
     const CUtensorMap tx = lq_tc_make_map_u8(x_codes, k / 2, p.n, k / 2, 128);
     const CUtensorMap tw = lq_tc_make_map_u8(w_codes, k / 2, p.m, k / 2, 128);
     const CUtensorMap txs = lq_tc_make_map_u32(p.x_scales, k_tiles(k) * (kTile / 4), row_tiles(p.n), 256, 1);
     const CUtensorMap tws = lq_tc_make_map_u32(p.w_scales, k_tiles(k) * (kTile / 4), row_tiles(p.m), 256, 2);
     const int tma_store = !p.y_f32 && p.m % 8 == 0 && al16(p.y);
+    const CUtensorMap th = lora ? lq_tc_make_map(lora->h, lora->ext, p.n, lora->ext, 128) : tx;
+    const CUtensorMap tb = lora ? lq_tc_make_map(lora->bt, lora->ext, p.m, lora->ext, 128) : tx;
+    p.lora = lora ? lora->ext / 64 : 0;
     const CUtensorMap ty = tma_store ? lq_tc_make_store_map(p.y, p.m, p.n, p.m) : tx;
     p.x_tiles = (p.n + 255) / 256;
     p.w_tiles = (p.m + 255) / 256;
@@ -889,7 +917,7 @@ void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int6
     auto kern = tma_store ? mx4_pair_kernel<true> : mx4_pair_kernel<false>;
     LQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
     LqProf prof(LQ_K_GEMM_MAIN, st);
-    lqstream::launch_pdl(kern, dim3(2 * pairs), dim3(kThreads2), Cfg2::SMEM, st, tx, tw, txs, tws, ty, p);
+    lqstream::launch_pdl(kern, dim3(2 * pairs), dim3(kThreads2), Cfg2::SMEM, st, tx, tw, txs, tws, ty, th, tb, p);
     LQ_CUDA(cudaGetLastError());
 }
 
@@ -924,7 +952,7 @@ void quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t ld, voi
 }
 
 void product(const void* x_codes, const void* x_scales, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k,
-             const float* bias, void* y, int y_dtype, bool early_w, int dev, cudaStream_t st) {
+             const float* bias, void* y, int y_dtype, bool early_w, int dev, cudaStream_t st, const LoraOperands* lora = nullptr) {
     const int sms = lq_tc_sm_count(dev), bn = bn_of(n);
     ProductParams p;
     p.w_scales = (const uint8_t*)w_scales;
@@ -935,19 +963,94 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
     p.w_tiles = (int)((m + 127) / 128);
     p.x_tiles = (int)((n + bn - 1) / bn);
     p.splits = splits_of((int64_t)p.w_tiles * p.x_tiles, p.kb, sms);
+    p.lora = 0;
     p.early_w = early_w;
     p.bias = bias;
     p.y = y;
     p.y_f32 = y_dtype == LQ_F32;
     p.status = lq_tc_status_word(dev);
-    if (use_pair(n, m, sms)) launch_pair(p, w_codes, x_codes, k, dev, sms, st);
+    if (use_pair(n, m, sms)) launch_pair(p, w_codes, x_codes, k, lora, dev, sms, st);
     else if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, st);
     else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, st);
     else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, st);
     else launch_stream<128>(p, w_codes, x_codes, k, st);
 }
 
+// ---- with an adapter ------------------------------------------------------------------------------
+// y += h . B for few tokens (or few outputs): h = s * H [n, ext] and B [r, m] in bf16, the sum in f32, y rounded once more.
+// A thread owns two columns of eight rows; 77 x 6144, rank 16: 3 us, launch and latency.
+constexpr int kDeltaRows = 8;
+__global__ void __launch_bounds__(256) mx4_add_delta_kernel(__nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
+                                                            const __nv_bfloat16* __restrict__ b, int64_t n, int64_t m, int r, int ext) {
+    extern __shared__ float hs[];  // [rank][row]
+    const int64_t row0 = (int64_t)blockIdx.y * kDeltaRows, col = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 2;
+    for (int i = threadIdx.x; i < r * kDeltaRows; i += 256) {
+        const int row = i / r, j = i - row * r;
+        hs[j * kDeltaRows + row] = row0 + row < n ? __bfloat162float(h[(row0 + row) * ext + j]) : 0.f;
+    }
+    __syncthreads();
+    if (col >= m) return;  // m is even
+    float2 acc[kDeltaRows] = {};
+#pragma unroll 4
+    for (int j = 0; j < r; ++j) {
+        const float2 w = __bfloat1622float2(*(const __nv_bfloat162*)(b + j * m + col));
+#pragma unroll
+        for (int i = 0; i < kDeltaRows; ++i) {
+            acc[i].x = fmaf(hs[j * kDeltaRows + i], w.x, acc[i].x);
+            acc[i].y = fmaf(hs[j * kDeltaRows + i], w.y, acc[i].y);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kDeltaRows; ++i)
+        if (row0 + i < n) {
+            __nv_bfloat162* at = (__nv_bfloat162*)(y + (row0 + i) * m + col);
+            const float2 v = __bfloat1622float2(*at);
+            *at = __floats2bfloat162_rn(v.x + acc[i].x, v.y + acc[i].y);
+        }
+}
+
+// The forward's workspace: the quantised x, s * H, H where the caller does not keep it, and the partial sums of H.
+struct LoraSpace {
+    size_t ext, h, part, bytes;
+};
+LoraSpace lora_space(int64_t n, int64_t k, int r) {
+    LoraSpace s;
+    s.ext = al256(lq_mx4_linear_workspace_bytes(n, k));
+    s.h = s.ext + al256((size_t)n * lq_tc_ext_width(r) * 2);
+    s.part = s.h + al256((size_t)n * r * 4);
+    s.bytes = s.part + lq_tc_lora_down_bytes(n, r);
+    return s;
+}
+lq_weight lora_weight(const void* codes, const void* scales, int64_t m, int64_t k, int dev) {
+    lq_weight w;
+    w.device = dev;
+    w.scheme = kSchemeMx4;
+    w.M = m;
+    w.K = k;
+    w.packed = const_cast<void*>(codes);
+    w.mx4_scales = scales;
+    return w;
+}
+void check_lora(int64_t n, int64_t m, int64_t k, int r, const void* mirror) {
+    check_dims(n, k);
+    check_dims(m, k);
+    LQ_CHECK_ARG(r >= 1 && r <= 256, "LoRA rank must be in [1, 256]");
+    LQ_CHECK_ARG(m >= 8 && m % 8 == 0, "with an adapter d_out must be a positive multiple of 8");
+    LQ_CHECK_ARG(mirror && ((uintptr_t)mirror & 255) == 0, "a 256-byte aligned mirror of the factors is needed");
+}
+
 }  // namespace
+
+void lq_mx4_launch_dequant(const void* codes, const void* scales, int64_t rows, int64_t k, void* out, int out_dtype, cudaStream_t st) {
+    const unsigned grid = grid_of((rows * runs_of(k) + 7) / 8, lq_tc_sm_count(current_device()), 16);
+    LqProf prof(LQ_K_DEQUANT, st);
+    if (out_dtype == LQ_F32)
+        mx4_dequantize_kernel<float><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, (int)k, (float*)out);
+    else
+        mx4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, (int)k,
+                                                                   (__nv_bfloat16*)out);
+    LQ_CUDA(cudaGetLastError());
+}
 
 extern "C" {
 
@@ -975,15 +1078,7 @@ int lq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64
         if (rows == 0) return;
         check_tensor(codes, scales);
         LQ_CHECK_ARG(out && al16(out), "the output must be 16-byte aligned");
-        cudaStream_t st = (cudaStream_t)stream;
-        const unsigned grid = grid_of((rows * runs_of(k) + 7) / 8, lq_tc_sm_count(current_device()), 16);
-        LqProf prof(LQ_K_DEQUANT, st);
-        if (out_dtype == LQ_F32)
-            mx4_dequantize_kernel<float><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, (int)k, (float*)out);
-        else
-            mx4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const uint32_t*)codes, (const uint8_t*)scales, rows, (int)k,
-                                                                       (__nv_bfloat16*)out);
-        LQ_CUDA(cudaGetLastError());
+        lq_mx4_launch_dequant(codes, scales, rows, k, out, out_dtype, (cudaStream_t)stream);
     });
 }
 
@@ -1050,7 +1145,7 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
         LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
         if (ws_bytes < lq_mx4_matmul_dx_workspace_bytes(n, m, k, dtype))
             throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled backward");
-        if (lq_mx4_dequantize(w_codes, w_scales, m, k, ws, LQ_BF16, stream) != LQ_OK) throw LqError(LQ_ERR_CUDA, lq_last_error());
+        lq_mx4_launch_dequant(w_codes, w_scales, m, k, ws, LQ_BF16, st);
         const DxSpace sp = dx_space(n, m, k, dtype);
         const int sms = lq_tc_sm_count(current_device());
         __nv_bfloat16* rows = (__nv_bfloat16*)((uint8_t*)ws + sp.rows);
@@ -1077,6 +1172,63 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
             LQ_CHECK_ARG(al16(dy), "dy must be 16-byte aligned");
         }
         lq_tc_gemm_nn(src, sp.ld, ws, k, dx, LQ_BF16, n, k, m, st);
+    });
+}
+
+size_t lq_mx4_lora_workspace_bytes(int64_t n, int64_t m, int64_t k, int rank, int backward) {
+    if (n < 1 || m < 1 || k < 32 || rank < 1 || rank > 256) return 0;
+    if (!backward) return lora_space(n, k, rank).bytes;
+    const lq_weight w = lora_weight(nullptr, nullptr, m, k, 0);
+    return lq_tc_workspace_bytes(&w, n, rank);
+}
+
+int lq_mx4_lora_fwd(const void* x, int64_t n, const void* w_codes, const void* w_scales, int64_t m, int64_t k, const float* bias,
+                    const void* mirror, int rank, float scaling, void* y, float* h_out, void* ws, size_t ws_bytes, void* stream) {
+    return guarded_call([&] {
+        check_lora(n, m, k, rank, mirror);
+        if (n == 0) return;
+        check_tensor(w_codes, w_scales);
+        LQ_CHECK_ARG(x && y && al16(x) && al16(y), "x and y must be 16-byte aligned");
+        LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
+        const LoraSpace sp = lora_space(n, k, rank);
+        if (ws_bytes < sp.bytes) throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled linear with an adapter");
+        cudaStream_t st = (cudaStream_t)stream;
+        const int dev = current_device(), sms = lq_tc_sm_count(dev), ext = lq_tc_ext_width(rank);
+        const LqMirrorView mv = lq_tc_mirror_view(k, m, rank, mirror);
+        uint8_t *codes = (uint8_t*)ws, *scales = codes + al256((size_t)n * k / 2);
+        __nv_bfloat16* sh = (__nv_bfloat16*)(codes + sp.ext);
+        lq_tc_lora_down(x, n, k, k, mv.At, rank, scaling, h_out ? h_out : (float*)(codes + sp.h), sh, codes + sp.part, sms, st);
+        quantize(x, LQ_BF16, n, k, k, codes, scales, dev, st);
+        const LoraOperands lora{sh, mv.Bt, ext};
+        product(codes, scales, n, w_codes, w_scales, m, k, bias, y, LQ_BF16, true, dev, st, &lora);
+        if (!use_pair(n, m, sms)) {
+            LqProf prof(LQ_K_REDUCE, st);
+            const int64_t rows = (n + kDeltaRows - 1) / kDeltaRows;
+            for (int64_t first = 0; first < rows; first += 65535) {
+                const int64_t part = std::min<int64_t>(65535, rows - first), at = first * kDeltaRows;
+                mx4_add_delta_kernel<<<dim3((unsigned)((m + 511) / 512), (unsigned)part), 256, (size_t)rank * kDeltaRows * 4, st>>>(
+                    (__nv_bfloat16*)y + at * m, sh + at * ext, mv.Bb, n - at, m, rank, ext);
+                LQ_CUDA(cudaGetLastError());
+            }
+        }
+    });
+}
+
+int lq_mx4_lora_bwd(const void* dy, const void* x, const float* h, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
+                    int64_t k, const void* mirror, int rank, float scaling, void* dx, float* dA, float* dB, int accumulate, void* ws,
+                    size_t ws_bytes, void* stream) {
+    return guarded_call([&] {
+        check_lora(n, m, k, rank, mirror);
+        cudaStream_t st = (cudaStream_t)stream;
+        if (n == 0) {  // sums over nothing
+            if (dA && !accumulate) LQ_CUDA(cudaMemsetAsync(dA, 0, sizeof(float) * (size_t)k * rank, st));
+            if (dB && !accumulate) LQ_CUDA(cudaMemsetAsync(dB, 0, sizeof(float) * (size_t)m * rank, st));
+            return;
+        }
+        check_tensor(w_codes, w_scales);
+        LQ_CHECK_ARG(dy && x && al16(dy) && al16(x) && al16(dx), "dy, x and dx must be 16-byte aligned");
+        const lq_weight w = lora_weight(w_codes, w_scales, m, k, current_device());
+        lq_tc_bwd(&w, dy, x, h, n, nullptr, nullptr, rank, scaling, dx, dA, dB, accumulate, ws, ws_bytes, st, mirror);
     });
 }
 

@@ -492,6 +492,11 @@ void lq_launch_unpack(const lq_weight* w, int8_t* codes, float* scales, cudaStre
 }
 
 void lq_launch_dequant(const lq_weight* w, void* out, int out_dtype, int64_t ld, int transpose, cudaStream_t st) {
+    if (w->scheme == kSchemeMx4) {
+        LQ_CHECK_ARG(!transpose && ld == w->K, "a microscaled weight is dequantised in its own orientation");
+        lq_mx4_launch_dequant(w->packed, w->mx4_scales, w->M, w->K, out, out_dtype, st);
+        return;
+    }
     LqProf prof(LQ_K_DEQUANT, st);
     const bool aligned = (ld % 8 == 0) && (((uintptr_t)out & 15) == 0) && (w->M % 8 == 0) &&
                          (w->scheme != LQ_FP8_E4M3 || w->K % 16 == 0);

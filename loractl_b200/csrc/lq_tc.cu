@@ -1578,6 +1578,20 @@ int lq_tc_read_status(int device, cudaStream_t st) {
     return v != 0 ? v : v2;
 }
 
+int lq_tc_ext_width(int r) { return ext_width(r); }
+
+LqMirrorView lq_tc_mirror_view(int64_t K, int64_t M, int r, const void* mirror) {
+    const LoraMirror m = carve_mirror(K, M, r, const_cast<void*>(mirror));
+    return {m.At, m.Bt, m.Bb};
+}
+
+size_t lq_tc_lora_down_bytes(int64_t N, int r) { return (size_t)16 * N * ext_width(r) * 4; }
+
+void lq_tc_lora_down(const void* X, int64_t N, int64_t K, int64_t ldx, const __nv_bfloat16* At, int r, float s, float* H,
+                     __nv_bfloat16* ext, void* part, int sm_count, cudaStream_t st) {
+    skinny_down(X, N, K, ldx, At, K, r, 1.f, H, ext, s, (float*)part, sm_count, st);
+}
+
 size_t lq_tc_mirror_bytes(int64_t K, int64_t M, int r) { return r > 0 ? carve_mirror(K, M, r, nullptr).bytes : 0; }
 
 bool lq_tc_option_set(const char* name, int value) {
@@ -1735,7 +1749,9 @@ void lq_tc_bwd(const lq_weight* w, const void* dY, const void* X, const float* H
     // without a resident copy the same operand form serves the per-call scratch: the weight is
     // dequantised in its own [M, K] orientation (the cheaper pass: full output lines per warp, no
     // staging) and the dX GEMM reads the scratch MN-major
-    const bool mn_scratch = mn_ok && !cached && !w4 && g_bwd_mn.load() != 0 && K % 8 == 0;
+    const bool mx4 = w->scheme == kSchemeMx4;  // has its own orientation only; always with a mirror
+    const bool mn_scratch = mn_ok && !cached && !w4 && (mx4 || g_bwd_mn.load() != 0) && K % 8 == 0;
+    const bool mn_single = dX && mx4 && !mn_scratch;  // the same operand form below the CTA-pair kernel's sizes
     Operand bmn{cached ? (const void*)w->bf16_copy : (const void*)t.wscr, true, K};
     if (r == 0) {
         if (dX && w4) {
@@ -1764,7 +1780,7 @@ void lq_tc_bwd(const lq_weight* w, const void* dY, const void* X, const float* H
     skinny_down(dY, N, M, M, t.pdown, M, r, s, t.dHf, t.ext_a, 1.f, t.part, ctx.sm_count, st);
     // side: what the dX GEMM needs besides dH: W^T [K, M] and A [K, EXT] in bf16
     if (dX) {
-        if (mn_scratch) lq_launch_dequant(w, t.wscr, LQ_BF16, K, 0, fj.side());       // W [M, K]
+        if (mn_scratch || mn_single) lq_launch_dequant(w, t.wscr, LQ_BF16, K, 0, fj.side());  // W [M, K]
         else if (!w4 && !cached) lq_launch_dequant(w, t.wscr, LQ_BF16, M, 1, fj.side());  // W^T [K, M]
         if (!mirror) cast_pad(A, r, 1, t.pext, EXT, K, r, EXT, 1.f, fj.side());
     }
@@ -1791,6 +1807,9 @@ void lq_tc_bwd(const lq_weight* w, const void* dY, const void* X, const float* H
             Operand a1{t.ext_a, false, EXT}, b1{t.pext, false, EXT};
             launch_gemm_pair<256, false, true>(a0, bmn, M, &a1, &b1, EXT, (__nv_bfloat16*)dX, K, N, K, nullptr, st,
                                                EpiScales(), t.tail);
+        } else if (mn_single) {  // the extension's B operand is A^T [r, K]: MN-major too
+            Operand a1{t.ext_a, false, EXT}, b1{t.pdown2, true, K};
+            launch_gemm<128, false, true, __nv_bfloat16>(a0, bmn, M, &a1, &b1, r, (__nv_bfloat16*)dX, K, 0, N, K, 1, nullptr, st);
         } else {
             Operand a1{t.ext_a, false, EXT}, b1{t.pext, false, EXT};
             main_gemm<__nv_bfloat16>(a0, b0, M, &a1, &b1, EXT, (__nv_bfloat16*)dX, K, N, K, nullptr, ctx.sm_count, st, t.tail);

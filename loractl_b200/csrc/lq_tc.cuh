@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_bf16.h>
 
 #include "lq_internal.cuh"
 
@@ -20,6 +21,18 @@ void lq_tc_bwd(const lq_weight* w, const void* dY, const void* X, const float* H
 size_t lq_tc_mirror_bytes(int64_t K, int64_t M, int r);
 void lq_tc_mirror_build(const float* A, const float* B, int64_t K, int64_t M, int r, void* mirror, cudaStream_t st);
 void lq_tc_mirror_build_batch(const lq_mirror_job* jobs, int n, cudaStream_t st);
+
+// The pieces of a LoRA product for a kernel that extends its own reduction by it (lq_mx4.cu): the mirror's arrays
+// A^T [r, K], B^T [M, EXT], B [r, M]; EXT = r rounded up to 64; and H = X . A (f32 [N, r]) with ext = s * H (bf16
+// [N, EXT], zero padded), `part` being lq_tc_lora_down_bytes() of partial sums.
+struct LqMirrorView {
+    const __nv_bfloat16 *At, *Bt, *Bb;
+};
+LqMirrorView lq_tc_mirror_view(int64_t K, int64_t M, int r, const void* mirror);
+int lq_tc_ext_width(int r);
+size_t lq_tc_lora_down_bytes(int64_t N, int r);
+void lq_tc_lora_down(const void* X, int64_t N, int64_t K, int64_t ldx, const __nv_bfloat16* At, int r, float s, float* H,
+                     __nv_bfloat16* ext, void* part, int sm_count, cudaStream_t st);
 
 // Plain bf16 GEMM entry used by tests and probes: C[Mg,Ng] = A . B^T with either operand
 // K-major ([rows, Kg], Kg contiguous) or MN-major ([Kg, rows], rows contiguous).

@@ -468,6 +468,99 @@ Tensor mx4_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int64_t 
     return y;
 }
 
+// With an adapter on the same input: quant(x) . W^T + bias + scaling * (x . A) . B in bf16.
+struct Mx4LoraBackward : public Node {
+    Tensor codes, scales, mirror, h;   // state, never graph parents
+    Tensor bucket_a, bucket_b;         // views of a flat gradient buffer, or undefined
+    SavedVariable x, a, b;
+    int64_t m = 0, k = 0;
+    double scaling = 1.0;
+    std::vector<int64_t> shape;
+    bool released = false;
+
+    std::string name() const override { return "Mx4LoraBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* v : {&x, &a, &b}) v->reset_data();
+        h.reset();
+        released = true;
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        TORCH_CHECK(!released, "Trying to backward through the graph a second time: specify retain_graph=True");
+        return once(gradients(std::move(grads)), "the microscaled linear with an adapter");
+    }
+    variable_list gradients(variable_list&& grads) {
+        variable_list out(3);
+        if (!grads[0].defined()) return out;
+        const Tensor xs = x.unpack(), as = a.unpack(), bs = b.unpack();
+        at::NoGradGuard no_grad;
+        c10::cuda::OptionalCUDAGuard guard(xs.device());
+        Tensor dy = grads[0].reshape({-1, m}).contiguous();
+        if ((uintptr_t)ptr(dy) % 16) dy = dy.clone();
+        const int64_t n = dy.size(0), rank = as.size(1);
+        // straight into the flat buffer only while the factors' .grad are its views: whoever reset them expects autograd's
+        auto lives = [](const Tensor& p, const Tensor& view) {
+            return view.defined() && p.grad().defined() && p.grad().const_data_ptr() == view.const_data_ptr();
+        };
+        const bool direct = lives(as, bucket_a) && lives(bs, bucket_b);
+        const auto opts = xs.options().requires_grad(false);
+        Tensor da, db;
+        if (task_should_compute_output(0)) out[0] = at::empty({n, k}, opts);
+        if (task_should_compute_output(1)) da = direct ? bucket_a : at::empty({k, rank}, opts.dtype(at::kFloat));
+        if (task_should_compute_output(2)) db = direct ? bucket_b : at::empty({rank, m}, opts.dtype(at::kFloat));
+        // of this call alone: from the pool of the current stream, or of the graph being captured
+        Tensor space = at::empty({(int64_t)lq_mx4_lora_workspace_bytes(n, m, k, (int)rank, 1)}, opts.dtype(at::kByte));
+        check(lq_mx4_lora_bwd(ptr(dy), ptr(xs), (const float*)ptr(h), n, ptr(codes), ptr(scales), m, k, ptr(mirror), (int)rank, (float)scaling,
+                              mut(out[0]), (float*)mut(da), (float*)mut(db), direct, mut(space), space.numel(), stream_of(xs)));
+        if (out[0].defined()) out[0] = out[0].view(shape);
+        if (!direct) out[1] = da, out[2] = db;
+        return out;
+    }
+};
+
+Tensor mx4_lora_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int64_t m, int64_t k, const std::optional<Tensor>& bias_,
+                       const Tensor& a, const Tensor& b, double scaling, const Tensor& mirror, const std::optional<Tensor>& bucket_a,
+                       const std::optional<Tensor>& bucket_b) {
+    require_cuda(x_, "x");
+    TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) == k, "last dim ", x_.dim() ? x_.size(-1) : 0, " != d_in ", k);
+    TORCH_CHECK_TYPE(x_.scalar_type() == at::kBFloat16, "the fused adapter takes bf16 activations, got ", x_.scalar_type());
+    const std::pair<const char*, const Tensor*> named[] = {{"w", &wc}, {"lora_a", &a}, {"lora_b", &b}, {"the mirror", &mirror}};
+    for (const auto& [name, v] : named) TORCH_CHECK(v->device() == x_.device(), name, " is on ", v->device(), ", x on ", x_.device());
+    const int64_t rank = a.dim() == 2 ? a.size(1) : 0;
+    TORCH_CHECK_VALUE(rank > 0 && a.size(0) == k && b.dim() == 2 && b.size(0) == rank && b.size(1) == m, "lora_a must be [", k,
+                      ", rank], lora_b [rank, ", m, "], got ", a.sizes(), " and ", b.sizes());
+    TORCH_CHECK_VALUE(mirror.is_contiguous() && mirror.nbytes() >= lq_lora_mirror_bytes(k, m, (int)rank), "the mirror is too small");
+    c10::cuda::OptionalCUDAGuard guard(x_.device());
+    const bool grad = wants_grad({&x_, &a, &b});
+    Tensor x, y, h;
+    {
+        at::NoGradGuard no_grad;
+        x = x_.reshape({-1, k}).contiguous();
+        if ((uintptr_t)ptr(x) % 16) x = x.clone();
+        const Tensor bias = bias_of(bias_, wc, m);
+        const int64_t n = x.size(0);
+        auto shape = x_.sizes().vec();
+        shape.back() = m;
+        const auto opts = x.options().requires_grad(false);
+        y = at::empty(shape, opts);
+        if (grad) h = at::empty({n, rank}, opts.dtype(at::kFloat));
+        Tensor space = at::empty({(int64_t)lq_mx4_lora_workspace_bytes(n, m, k, (int)rank, 0)}, wc.options());
+        check(lq_mx4_lora_fwd(ptr(x), n, ptr(wc), ptr(ws), m, k, (const float*)ptr(bias), ptr(mirror), (int)rank, (float)scaling, mut(y),
+                              (float*)mut(h), mut(space), space.numel(), stream_of(x)));
+    }
+    if (grad) {
+        auto node = std::shared_ptr<Mx4LoraBackward>(new Mx4LoraBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x_, a, b));
+        node->x = SavedVariable(x, false), node->a = SavedVariable(a, false), node->b = SavedVariable(b, false);
+        node->codes = wc, node->scales = ws, node->mirror = mirror, node->h = h;
+        node->bucket_a = defined(bucket_a), node->bucket_b = defined(bucket_b);
+        node->m = m, node->k = k, node->scaling = scaling, node->shape = x_.sizes().vec();
+        torch::autograd::set_history(y, node);
+    }
+    return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_lq_torch, mod) {
@@ -489,4 +582,5 @@ PYBIND11_MODULE(_lq_torch, mod) {
     mod.def("mx4_matmul", &mx4_matmul);
     mod.def("mx4_matmul_dx", &mx4_matmul_dx);
     mod.def("mx4_linear", &mx4_linear);
+    mod.def("mx4_lora_linear", &mx4_lora_linear);
 }

@@ -53,7 +53,7 @@ class QuantLinear(nn.Module):
 
 class BaseLinear(nn.Module):
     """crates/loractl-core/src/mmdit.rs:451-520: `Plain(Linear)` or `Quant(QuantLinear)`; here also
-    `Mx4(Mx4Linear)`, whose adapter delta is added outside the kernel as a plain linear's is."""
+    `Mx4(Mx4Linear)`, whose adapter is part of its call in bf16 and added outside as a plain linear's in f32."""
 
     def __init__(self, inner: nn.Module):
         super().__init__()
@@ -227,9 +227,17 @@ def site_group(adapters: Optional[LoraAdapters], sites, x: torch.Tensor):
     return [y.reshape(*lead, base.d_out) for y, (_, base) in zip(ys, sites)]
 
 
+def _mx4_fuses(q: Mx4Linear, delta: LoraDelta, x: torch.Tensor) -> bool:
+    """What `lq_mx4_lora_fwd` takes; the rest adds the delta in plain tensor ops (f32 activations keep an f32 delta)."""
+    return (x.is_cuda and delta.lora_a.is_cuda and x.dtype == torch.bfloat16 and q.d_out % 8 == 0 and delta.rank <= 256
+            and not (delta.dropout > 0.0 and delta.training))
+
+
 def apply_site(base: BaseLinear, delta: Optional[LoraDelta], x: torch.Tensor) -> torch.Tensor:
     if base.is_quant:
         return _fused(base.inner.weight, x, delta)
+    if base.is_mx4 and delta is not None and _mx4_fuses(base.inner, delta, x):
+        return base.inner.forward_adapted(x, delta)
     out = base(x)
     return out if delta is None else out + delta(x)
 

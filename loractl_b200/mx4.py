@@ -103,3 +103,11 @@ class Mx4Linear(nn.Module):
         `dy . dequant(w)`: the quantisation of x is taken as the identity, the weight is state (quant.rs:217-219)."""
         w = self.weight
         return L.ext().mx4_linear(x, w.codes, w.scales, w.rows, w.k, self.bias)
+
+    def forward_adapted(self, x: torch.Tensor, delta) -> torch.Tensor:
+        """`forward(x) + scaling * (x . lora_a) . lora_b` of a `LoraDelta` in one call, x in bf16 and d_out a multiple of 8: the
+        adapter reads x itself, its factors rounded to bf16; the backward gives dx and both factors' gradients, into the
+        flat gradient buffer where the factors live in one."""
+        w, bucket = self.weight, delta.bucket_grads or (None, None)
+        return L.ext().mx4_lora_linear(x, w.codes, w.scales, w.rows, w.k, self.bias, delta.lora_a, delta.lora_b, delta.scaling,
+                                       delta.operand_mirror(), *bucket)
