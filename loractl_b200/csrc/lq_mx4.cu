@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
 // the stage they came with, so that a stage's release covers them.  The accumulator has one buffer (256 columns; two
 // would leave no room for scales): the epilogue empties it into registers at once and converts and stores
 // while the next tile's products run.  4096 x 6144 -> 16384: 167 us, 4.9 PFLOP/s (single CTAs with 128 x 128 tiles: 343 us);
-// for seconds on end 4.3 PFLOP/s, at the card's power cap.
+// for seconds on end 4.3 PFLOP/s, at the card's power cap.  An adapter's product is one more k-block of bf16 for each 64 of
+// rank (the ring's stages fit: 64 bf16 are 128 bytes a row too): 180 us with rank 16.
 struct Cfg2 {
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = 128 * 128, SA_BYTES = 2 * kTile, SB_BYTES = 4 * kTile;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
@@ -978,20 +979,28 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
 
 // ---- with an adapter ------------------------------------------------------------------------------
 // y += h . B for few tokens (or few outputs): h = s * H [n, ext] and B [r, m] in bf16, the sum in f32, y rounded once more.
-// A thread owns two columns of eight rows; 77 x 6144, rank 16: 3 us, launch and latency.
+// A thread owns two columns of eight rows; launch and latency bound it: 77 x 6144, rank 16 (240 blocks of 128 threads, y
+// fetched ahead) 4.6 us, with 120 blocks of 256 and y last 6.9.
 constexpr int kDeltaRows = 8;
-__global__ void __launch_bounds__(256) mx4_add_delta_kernel(__nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
+constexpr int kDeltaThreads = 128;
+__global__ void __launch_bounds__(kDeltaThreads) mx4_add_delta_kernel(__nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
                                                             const __nv_bfloat16* __restrict__ b, int64_t n, int64_t m, int r, int ext) {
     extern __shared__ float hs[];  // [rank][row]
-    const int64_t row0 = (int64_t)blockIdx.y * kDeltaRows, col = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 2;
-    for (int i = threadIdx.x; i < r * kDeltaRows; i += 256) {
+    const int64_t row0 = (int64_t)blockIdx.y * kDeltaRows, col = ((int64_t)blockIdx.x * kDeltaThreads + threadIdx.x) * 2;
+    __nv_bfloat162 base[kDeltaRows] = {};  // fetched ahead of the sums
+    if (col < m) {  // m is even
+#pragma unroll
+        for (int i = 0; i < kDeltaRows; ++i)
+            if (row0 + i < n) base[i] = *(const __nv_bfloat162*)(y + (row0 + i) * m + col);
+    }
+    for (int i = threadIdx.x; i < r * kDeltaRows; i += kDeltaThreads) {
         const int row = i / r, j = i - row * r;
         hs[j * kDeltaRows + row] = row0 + row < n ? __bfloat162float(h[(row0 + row) * ext + j]) : 0.f;
     }
     __syncthreads();
-    if (col >= m) return;  // m is even
+    if (col >= m) return;
     float2 acc[kDeltaRows] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < r; ++j) {
         const float2 w = __bfloat1622float2(*(const __nv_bfloat162*)(b + j * m + col));
 #pragma unroll
@@ -1003,9 +1012,8 @@ __global__ void __launch_bounds__(256) mx4_add_delta_kernel(__nv_bfloat16* __res
 #pragma unroll
     for (int i = 0; i < kDeltaRows; ++i)
         if (row0 + i < n) {
-            __nv_bfloat162* at = (__nv_bfloat162*)(y + (row0 + i) * m + col);
-            const float2 v = __bfloat1622float2(*at);
-            *at = __floats2bfloat162_rn(v.x + acc[i].x, v.y + acc[i].y);
+            const float2 v = __bfloat1622float2(base[i]);
+            *(__nv_bfloat162*)(y + (row0 + i) * m + col) = __floats2bfloat162_rn(v.x + acc[i].x, v.y + acc[i].y);
         }
 }
 
@@ -1206,7 +1214,8 @@ int lq_mx4_lora_fwd(const void* x, int64_t n, const void* w_codes, const void* w
             const int64_t rows = (n + kDeltaRows - 1) / kDeltaRows;
             for (int64_t first = 0; first < rows; first += 65535) {
                 const int64_t part = std::min<int64_t>(65535, rows - first), at = first * kDeltaRows;
-                mx4_add_delta_kernel<<<dim3((unsigned)((m + 511) / 512), (unsigned)part), 256, (size_t)rank * kDeltaRows * 4, st>>>(
+                const dim3 grid((unsigned)((m + 2 * kDeltaThreads - 1) / (2 * kDeltaThreads)), (unsigned)part);
+                mx4_add_delta_kernel<<<grid, kDeltaThreads, (size_t)rank * kDeltaRows * 4, st>>>(
                     (__nv_bfloat16*)y + at * m, sh + at * ext, mv.Bb, n - at, m, rank, ext);
                 LQ_CUDA(cudaGetLastError());
             }
