@@ -524,7 +524,8 @@ __device__ __forceinline__ void tile2(const ProductParams& p, int item, int& xt,
     wt = r / rows;
 }
 
-template <bool TMA_OUT>
+// LORA: an adapter's k-blocks follow (a variant of its own: the branches in every role cost the plain product 2-4 %).
+template <bool TMA_OUT, bool LORA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads2, 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmXs,
                 const __grid_constant__ CUtensorMap tmWs, const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmH,
@@ -576,7 +577,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int items = p.x_tiles * p.w_tiles, cid = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
-    const int blocks = p.kb + p.lora;
+    const int blocks = LORA ? p.kb + p.lora : p.kb;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -592,7 +593,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     const uint32_t bar = smem_u32(&full[s]), sbar = smem_u32(&sfull[s]);
                     const uint32_t sa = smem_u32(smem_a + (size_t)s * C::A_BYTES), sb = smem_u32(smem_b + (size_t)s * C::B_BYTES);
                     if (leader) mbar_expect_tx(bar, 2 * (C::A_BYTES + C::B_BYTES));
-                    if (kb < p.kb) {
+                    if (!LORA || kb < p.kb) {
                         tma_load_2d_pair(sa, &tmX, bar, kb * 128, xt * 256 + (int)rank * 128);
                         tma_load_2d_pair(sb, &tmW, bar, kb * 128, wt * 256 + (int)rank * 128);
                         mbar_expect_tx(sbar, C::SA_BYTES + C::SB_BYTES);
@@ -626,7 +627,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     const uint32_t sfa = tmem + C::SCALE_COL + (uint32_t)s * 24, sfb = sfa + 8;
                     const uint32_t a_lo = desc_lo(smem_u32(smem_a + (size_t)s * C::A_BYTES), 16);
                     const uint32_t b_lo = desc_lo(smem_u32(smem_b + (size_t)s * C::B_BYTES), 16);
-                    if (kb < p.kb) {
+                    if (!LORA || kb < p.kb) {
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k)
                             mma2_mxf4(tmem, desc_join(a_lo + 2 * k, d_hi), desc_join(b_lo + 2 * k, d_hi), idesc_mxf4(256, 256, k & 1),
@@ -654,7 +655,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 if (!mbar_wait(smem_u32(&sfull[s]), phase, abort_flag, p.status, 84)) { ok = false; break; }
                 const uint8_t *sa = smem_sa + (size_t)s * C::SA_BYTES, *sb = smem_sb + (size_t)s * C::SB_BYTES;
                 const uint32_t sfa = lanes + (uint32_t)s * 24, sfb = sfa + 8;
-                if (kb < p.kb) {
+                if (!LORA || kb < p.kb) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {  // tiles of 128 elements; B's rows 0-127 and 128-255
                         stage_scales(sfa + 4 * j, sa + j * kTile, lane);
@@ -888,13 +889,13 @@ int resident_pairs(int dev, int sms) {
     static int known[64] = {};
     std::lock_guard<std::mutex> lk(mu);
     if (known[dev & 63] == 0) {
-        LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
+        LQ_CUDA(cudaFuncSetAttribute(mx4_pair_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(sms & ~1);
         cfg.blockDim = dim3(kThreads2);
         cfg.dynamicSmemBytes = Cfg2::SMEM;
         int n = 0;
-        LQ_CUDA(cudaOccupancyMaxActiveClusters(&n, mx4_pair_kernel<true>, &cfg));
+        LQ_CUDA(cudaOccupancyMaxActiveClusters(&n, mx4_pair_kernel<true, false>, &cfg));
         known[dev & 63] = std::max(1, std::min(n, sms / 2));
     }
     return known[dev & 63];
@@ -910,12 +911,13 @@ void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int6
     const CUtensorMap th = lora ? lq_tc_make_map(lora->h, lora->ext, p.n, lora->ext, 128) : tx;
     const CUtensorMap tb = lora ? lq_tc_make_map(lora->bt, lora->ext, p.m, lora->ext, 128) : tx;
     p.lora = lora ? lora->ext / 64 : 0;
+    LQ_CHECK_ARG(!lora || tma_store, "with an adapter the output is bf16 in rows of 16 bytes");
     const CUtensorMap ty = tma_store ? lq_tc_make_store_map(p.y, p.m, p.n, p.m) : tx;
     p.x_tiles = (p.n + 255) / 256;
     p.w_tiles = (p.m + 255) / 256;
     LQ_CHECK_ARG((int64_t)p.x_tiles * p.w_tiles < (int64_t)1 << 31, "too many tiles");
     const int pairs = std::min(resident_pairs(dev, sms), p.x_tiles * p.w_tiles);
-    auto kern = tma_store ? mx4_pair_kernel<true> : mx4_pair_kernel<false>;
+    auto kern = lora ? mx4_pair_kernel<true, true> : (tma_store ? mx4_pair_kernel<true, false> : mx4_pair_kernel<false, false>);
     LQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
     LqProf prof(LQ_K_GEMM_MAIN, st);
     lqstream::launch_pdl(kern, dim3(2 * pairs), dim3(kThreads2), Cfg2::SMEM, st, tx, tw, txs, tws, ty, th, tb, p);
