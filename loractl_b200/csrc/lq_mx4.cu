@@ -793,10 +793,18 @@ __global__ void __launch_bounds__(256) split3_kernel(const float* __restrict__ i
         }
     }
 }
-// out = c[0] + (c[1] + c[2]), [3, n] f32 in.
-__global__ void __launch_bounds__(256) join3_kernel(const float* __restrict__ c, int64_t n, float* __restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-        out[i] = c[i] + (c[n + i] + c[2 * n + i]);
+// out = c[0] + (c[1] + c[2]) of the terms, each the sum of its ranges: [ranges, 3, n] f32 in, n4 = n / 4.
+__global__ void __launch_bounds__(256) join3_kernel(const float4* __restrict__ c, int64_t n4, int ranges, float4* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
+        float4 t[3] = {};
+        for (int z = 0; z < ranges; ++z)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+                const float4 v = c[(3 * z + j) * n4 + i];
+                t[j].x += v.x, t[j].y += v.y, t[j].z += v.z, t[j].w += v.w;
+            }
+        out[i] = make_float4(t[0].x + (t[1].x + t[2].x), t[0].y + (t[1].y + t[2].y), t[0].z + (t[1].z + t[2].z), t[0].w + (t[1].w + t[2].w));
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -927,17 +935,17 @@ void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int6
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 // The backward's workspace: the weight in bf16, dy's rows where they have to be copied (f32: three bf16 terms), and the
-// f32 products of those terms.
+// product's partial sums (f32: the products of those terms).
 struct DxSpace {
     int64_t ld;  // of the copied rows: the tensor maps want 16 bytes
-    size_t rows, three, bytes;
+    size_t rows, part, bytes;
 };
 DxSpace dx_space(int64_t n, int64_t m, int64_t k, int dtype) {
     DxSpace s;
     s.ld = (m + 7) / 8 * 8;
     s.rows = al256((size_t)m * k * 2);
-    s.three = s.rows + (dtype == LQ_F32 ? al256((size_t)3 * n * s.ld * 2) : (s.ld != m ? al256((size_t)n * s.ld * 2) : 0));
-    s.bytes = s.three + (dtype == LQ_F32 ? (size_t)3 * n * k * 4 : 0);
+    s.part = s.rows + (dtype == LQ_F32 ? al256((size_t)3 * n * s.ld * 2) : (s.ld != m ? al256((size_t)n * s.ld * 2) : 0));
+    s.bytes = s.part + (dtype == LQ_F32 ? lq_tc_gemm_nn_part_bytes(3 * n, k, m, false) : lq_tc_gemm_nn_part_bytes(n, k, m, true));
     return s;
 }
 
@@ -1159,16 +1167,17 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
         const DxSpace sp = dx_space(n, m, k, dtype);
         const int sms = lq_tc_sm_count(current_device());
         __nv_bfloat16* rows = (__nv_bfloat16*)((uint8_t*)ws + sp.rows);
+        float* part = (float*)((uint8_t*)ws + sp.part);
+        const size_t part_bytes = sp.bytes - sp.part;
         if (dtype == LQ_F32) {
-            float* three = (float*)((uint8_t*)ws + sp.three);
             {
                 LqProf prof(LQ_K_PREP, st);
                 split3_kernel<<<grid_of((n * sp.ld + 255) / 256, sms, 16), 256, 0, st>>>((const float*)dy, n, m, sp.ld, rows);
                 LQ_CUDA(cudaGetLastError());
             }
-            lq_tc_gemm_nn(rows, sp.ld, ws, k, three, LQ_F32, 3 * n, k, m, st);
+            const int ranges = lq_tc_gemm_nn(rows, sp.ld, ws, k, nullptr, part, part_bytes, 3 * n, k, m, st);
             LqProf prof(LQ_K_REDUCE, st);
-            join3_kernel<<<grid_of((n * k + 255) / 256, sms, 16), 256, 0, st>>>(three, n * k, (float*)dx);
+            join3_kernel<<<grid_of((n * k / 4 + 255) / 256, sms, 16), 256, 0, st>>>((const float4*)part, n * k / 4, ranges, (float4*)dx);
             LQ_CUDA(cudaGetLastError());
             return;
         }
@@ -1181,7 +1190,7 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
         } else {
             LQ_CHECK_ARG(al16(dy), "dy must be 16-byte aligned");
         }
-        lq_tc_gemm_nn(src, sp.ld, ws, k, dx, LQ_BF16, n, k, m, st);
+        lq_tc_gemm_nn(src, sp.ld, ws, k, dx, part, part_bytes, n, k, m, st);
     });
 }
 

@@ -1728,6 +1728,45 @@ void lq_tc_fwd(const lq_weight* w, const void* X, int64_t N, const float* A, con
     main_gemm<__nv_bfloat16>(a0, b0, K, &a1, &b1, EXT, (__nv_bfloat16*)Y, M, N, M, w->bias, ctx.sm_count, st, t.tail);
 }
 
+// C[Mg, Ng] = A[Mg, K] . B[K, Ng] with B read MN-major: by the CTA pairs where they have rows enough, else in 128 x 128 tiles,
+// cut along K into f32 partial tiles where those leave SMs idle (the MXFP4 gradient, dequantisation included: 77 x 6144 -> 6144,
+// 48 tiles or 144 ranges of them, 44 or 33 us; one token 52 or 36; 200 tokens, 96 tiles either way, 45).
+namespace {
+constexpr int kSizingSms = 148;  // workspaces are sized without a device; what does not fit is cut less often
+bool nn_pair(int64_t Mg, int64_t Ng, int sms) { return pair_enabled() && Mg >= 256 && Ng > 192 && sms >= 2; }
+int nn_splits(int64_t Mg, int64_t Ng, int64_t k_blocks, int sms, size_t part_bytes = ~(size_t)0) {
+    const int s = choose_splits(((Mg + BM - 1) / BM) * ((Ng + 127) / 128), k_blocks, sms);
+    return (int)std::max<size_t>(1, std::min<size_t>((size_t)s, part_bytes / ((size_t)Mg * Ng * 4)));
+}
+__global__ void __launch_bounds__(256) sum_ranges_kernel(const float4* __restrict__ part, long long stride, int splits, long long n4,
+                                                         uint2* __restrict__ out) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    float4 v = part[i];
+    for (int z = 1; z < splits; ++z) {
+        const float4 a = part[z * stride + i];
+        v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+    }
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    out[i] = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+}
+// Ng a multiple of 4; (a1, b1): an extension of the reduction, b1 MN-major as well.
+void gemm_nn_single(const Operand& a0, const Operand& b0, int64_t K0, const Operand* a1, const Operand* b1, int64_t K1, __nv_bfloat16* C,
+                    int64_t Mg, int64_t Ng, float* part, size_t part_bytes, int sms, cudaStream_t st) {
+    const int64_t kb = (K0 + BK - 1) / BK + (a1 ? (K1 + BK - 1) / BK : 0);
+    const int splits = nn_splits(Mg, Ng, kb, sms, part_bytes);
+    if (splits == 1) {
+        launch_gemm<128, false, true, __nv_bfloat16>(a0, b0, K0, a1, b1, K1, C, Ng, 0, Mg, Ng, 1, nullptr, st);
+        return;
+    }
+    launch_gemm<128, false, true, float>(a0, b0, K0, a1, b1, K1, part, Ng, Mg * Ng, Mg, Ng, splits, nullptr, st);
+    LqProf prof(LQ_K_REDUCE, st);
+    const long long n4 = Mg * Ng / 4;
+    sum_ranges_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>((const float4*)part, n4, splits, n4, (uint2*)C);
+    LQ_CUDA(cudaGetLastError());
+}
+}  // namespace
+
 void lq_tc_bwd(const lq_weight* w, const void* dY, const void* X, const float* H, int64_t N, const float* A,
                const float* B, int r, float s, void* dX, float* dA, float* dB, int accumulate, void* ws,
                size_t ws_bytes, cudaStream_t st, const void* mirror) {
@@ -1809,7 +1848,8 @@ void lq_tc_bwd(const lq_weight* w, const void* dY, const void* X, const float* H
                                                EpiScales(), t.tail);
         } else if (mn_single) {  // the extension's B operand is A^T [r, K]: MN-major too
             Operand a1{t.ext_a, false, EXT}, b1{t.pdown2, true, K};
-            launch_gemm<128, false, true, __nv_bfloat16>(a0, bmn, M, &a1, &b1, r, (__nv_bfloat16*)dX, K, 0, N, K, 1, nullptr, st);
+            // `part` is free between dH and dA
+            gemm_nn_single(a0, bmn, M, &a1, &b1, r, (__nv_bfloat16*)dX, N, K, t.part, (size_t)16 * std::max(N, std::max(M, K)) * EXT * 4, ctx.sm_count, st);
         } else {
             Operand a1{t.ext_a, false, EXT}, b1{t.pext, false, EXT};
             main_gemm<__nv_bfloat16>(a0, b0, M, &a1, &b1, EXT, (__nv_bfloat16*)dX, K, N, K, nullptr, ctx.sm_count, st, t.tail);
@@ -2006,17 +2046,29 @@ void lq_tc_gemm_bf16(const void* A, int a_mn, int64_t lda, const void* B, int b_
     throw LqError(LQ_ERR_UNSUPPORTED, "gemm: this (block_n, operand major) combination is not built");
 }
 
-void lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int c_dtype, int64_t Mg, int64_t Ng,
-                   int64_t Kg, cudaStream_t st) {
+size_t lq_tc_gemm_nn_part_bytes(int64_t Mg, int64_t Ng, int64_t Kg, bool bf16_out) {
+    if (bf16_out && nn_pair(Mg, Ng, kSizingSms)) return kTailWsBytes;
+    const int splits = nn_splits(Mg, Ng, (Kg + BK - 1) / BK, kSizingSms);
+    return bf16_out && splits == 1 ? 0 : (size_t)splits * Mg * Ng * 4;
+}
+
+int lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part, size_t part_bytes, int64_t Mg, int64_t Ng,
+                  int64_t Kg, cudaStream_t st) {
     int dev;
     LQ_CUDA(cudaGetDevice(&dev));
+    const int sms = dev_ctx(dev).sm_count;
     const Operand a{A, false, lda}, b{B, true, ldb};
-    if (c_dtype == LQ_F32)
-        launch_gemm<128, false, true, float>(a, b, Kg, nullptr, nullptr, 0, (float*)C, Ng, 0, Mg, Ng, 1, nullptr, st);
-    else if (pair_enabled() && Mg >= 256 && Ng > 192 && dev_ctx(dev).sm_count >= 2)
-        launch_gemm_pair<256, false, true>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, Mg, Ng, nullptr, st);
+    if (!C) {
+        const int splits = nn_splits(Mg, Ng, (Kg + BK - 1) / BK, sms, part_bytes);
+        launch_gemm<128, false, true, float>(a, b, Kg, nullptr, nullptr, 0, part, Ng, Mg * Ng, Mg, Ng, splits, nullptr, st);
+        return splits;
+    }
+    if (nn_pair(Mg, Ng, sms))
+        launch_gemm_pair<256, false, true>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, Mg, Ng, nullptr, st, EpiScales(),
+                                           part_bytes >= kTailWsBytes ? part : nullptr);
     else
-        launch_gemm<128, false, true, __nv_bfloat16>(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Ng, 0, Mg, Ng, 1, nullptr, st);
+        gemm_nn_single(a, b, Kg, nullptr, nullptr, 0, (__nv_bfloat16*)C, Mg, Ng, part, part_bytes, sms, st);
+    return 1;
 }
 
 // =========================================================================================

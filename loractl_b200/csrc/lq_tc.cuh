@@ -40,9 +40,11 @@ void lq_tc_gemm_bf16(const void* A, int a_mn, int64_t lda, const void* B, int b_
                      int64_t ldc, int64_t Mg, int64_t Ng, int64_t Kg, int block_n, int splits, float* partial_ws,
                      const float* bias, cudaStream_t st);
 
-// C[Mg, Ng] (bf16 or f32, contiguous) = A[Mg, Kg] . B[Kg, Ng], both bf16 and row-major: B is read MN-major.
-void lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, int c_dtype, int64_t Mg, int64_t Ng,
-                   int64_t Kg, cudaStream_t st);
+// C[Mg, Ng] (bf16, contiguous) = A[Mg, Kg] . B[Kg, Ng], both bf16 and row-major: B is read MN-major.  Ng a multiple of 8.
+// With C = NULL the f32 sums of ranges of the reduction go to `part`, whole matrices one after the other: returns how many.
+size_t lq_tc_gemm_nn_part_bytes(int64_t Mg, int64_t Ng, int64_t Kg, bool bf16_out);
+int lq_tc_gemm_nn(const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part, size_t part_bytes, int64_t Mg,
+                  int64_t Ng, int64_t Kg, cudaStream_t st);
 
 // Per-device error word written by kernels whose bounded waits gave up.  Synchronises `st`.
 int lq_tc_read_status(int device, cudaStream_t st);

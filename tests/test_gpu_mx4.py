@@ -200,6 +200,25 @@ def test_layer_and_gradient(n, m, k, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,m,k", [(1, 4104, 512), (3, 5000, 96), (130, 2056, 1024), (64, 8192, 32), (600, 6152, 512), (2600, 6152, 2048)])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_gradient_over_many_outputs(n, m, k, dtype):
+    """Reductions that are cut into ranges: few rows, few columns, a last round of pairs."""
+    import loractl_b200 as lb
+
+    g = torch.Generator(device="cuda").manual_seed(n + m)
+    w = lb.mx4_quantize(torch.randn(m, k, generator=g, device="cuda"))
+    dy = (torch.randn(n, m, generator=g, device="cuda") * torch.exp(torch.randn(n, 1, generator=g, device="cuda"))).to(dtype)
+    dx = lb.mx4_matmul_dx(dy, w)
+    wd, d = w.dequantize().double(), dy.double()
+    ref, mag = d @ wd, d.abs() @ wd.abs()
+    lim = ((2 * m / 16 + 8) * 2.0 ** -23 * mag + 2.0 ** -8 * ref.abs()) if dtype == BF else (m + 4) * 2.0 ** -24 * mag
+    assert dx.dtype == dtype and bool(((dx.double() - ref).abs() <= lim).all())
+    assert torch.equal(lb.mx4_matmul_dx(dy, w), dx)
+    lb.check_device_status()
+
+
+@pytest.mark.gpu
 def test_two_streams_capture_and_determinism():
     """Two products at once on two streams with their own workspaces, two captured graphs replayed in turn."""
     import loractl_b200 as lb

@@ -67,7 +67,7 @@ def check(lin, lora, x, dy, y, dx, da, db):
 
 # few tokens and outputs (a kernel of its own adds the delta), then pairs of SMs (two to five k-blocks, ragged edges);
 # backward below 256 tokens, at an input of at most 192 and above; ranks of one to four k-blocks
-SITES = [(1, 8, 32, 1), (5, 304, 96, 4), (33, 72, 1184, 2), (77, 512, 288, 16), (129, 520, 64, 3), (256, 512, 512, 16), (300, 1000, 160, 8),
+SITES = [(1, 8, 32, 1), (33, 4104, 512, 4), (1, 6152, 64, 100), (5, 304, 96, 4), (33, 72, 1184, 2), (77, 512, 288, 16), (129, 520, 64, 3), (256, 512, 512, 16), (300, 1000, 160, 8),
          (301, 64, 1024, 64), (1000, 8, 224, 5), (2000, 2048, 288, 16), (1801, 1928, 544, 72), (2050, 1544, 32, 256), (1793, 2056, 1312, 128)]
 
 
