@@ -83,7 +83,7 @@ class LoraLinear(nn.Module):
     """crates/loractl-core/src/lora.rs:34-111: a frozen base plus a LoRA adapter,
     `y = base(x) + (alpha / rank) * B(A(dropout(x)))`.  The base may be a plain `nn.Linear`
     or a quantized `QuantLinear`; with the latter the whole forward/backward is one fused
-    call into the CUDA library.  An `Mx4Linear` base runs its own kernels, with the delta added to them."""
+    call into the CUDA library.  So it is with an `Mx4Linear` in bf16; in f32 the delta is added to its call."""
 
     def __init__(self, base: nn.Module, rank: int, alpha: float, dropout_prob: float = 0.0, device=None):
         super().__init__()
