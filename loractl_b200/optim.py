@@ -182,6 +182,9 @@ class AdamW:
         f = self.flat
         if not f.params.is_cuda:
             raise RuntimeError("the b200 backend has no CPU path")
+        if clip_coef is not None and (clip_coef.dtype != torch.float32 or clip_coef.device != f.params.device or clip_coef.numel() != 1):
+            raise ValueError(f"clip_coef must be one f32 value on {f.params.device}, got {list(clip_coef.shape)} {clip_coef.dtype} "
+                             f"on {clip_coef.device}")
         if count:
             self.steps += 1
         with torch.cuda.device(f.params.device):

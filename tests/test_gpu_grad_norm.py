@@ -231,6 +231,19 @@ def test_refusals_on_the_gpu():
     assert float(lb.global_grad_norm(torch.full((4,), 2.0, device="cuda"))) == 4.0
 
 
+@pytest.mark.gpu
+def test_step_refuses_a_coefficient_that_it_cannot_read():
+    import loractl_b200 as lb
+
+    delta = lb.LoraDelta(8, 8, 2, 4.0, device="cuda")
+    flat = lb.FlatAdapters(lb.LoraAdapters([delta], ["site"]), "cuda")
+    opt, before = lb.AdamW(flat, weight_decay=0.0), flat.params.clone()
+    for bad in (torch.ones(()), torch.ones((), device="cuda", dtype=torch.float64), torch.ones(2, device="cuda")):
+        with pytest.raises(ValueError, match="clip_coef must be one f32 value"):
+            opt.step(1e-3, clip_coef=bad)
+    assert opt.steps == 0 and torch.equal(flat.params, before)
+
+
 def test_refusals_without_a_gpu():
     import loractl_b200 as lb
     from loractl_b200._lib import ext
