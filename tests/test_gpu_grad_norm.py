@@ -87,6 +87,35 @@ def test_unaligned_and_strided_tensors():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,starts", [(BF, 8), (F, 4)])
+@pytest.mark.parametrize("size", [1, 6, 33, 8200, 33_000])
+def test_every_start_of_source_and_output(dtype, starts, size):
+    """Values unscaled (a bound above the norm) and halved (exact): each output is its gradient, its surroundings stay."""
+    import loractl_b200 as lb
+
+    room = size + 2 * starts
+    src = torch.randn(starts * starts, room, device="cuda").to(dtype)
+    dst = torch.full_like(src, 7.0)
+    pairs = [(i, i // starts, i % starts) for i in range(starts * starts)]
+    grads = [src[i].narrow(0, a, size) for i, a, _ in pairs]
+    outs = [dst[i].narrow(0, b, size) for i, _, b in pairs]
+    norm = torch.cat(grads).double().norm()
+    for factor in (1.0, 0.5):
+        got = lb.clip_grad_norm(grads, 1e30, out=outs, grad_scale=factor)
+        assert near(got, float(norm) * factor, 2.0 ** -23)
+        want = torch.full_like(src, 7.0)
+        for i, a, b in pairs:
+            want[i].narrow(0, b, size).copy_(grads[i] * factor)
+        assert torch.equal(dst, want)
+    copy = src.clone()
+    lb.clip_grad_norm([copy[i].narrow(0, a, size) for i, a, _ in pairs], 1e30, grad_scale=0.5)
+    want = src.clone()
+    for i, a, _ in pairs:
+        want[i].narrow(0, a, size).mul_(0.5)
+    assert torch.equal(copy, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [1e-42, 1e-30, 1e30, 3e38])
 def test_extreme_magnitudes(size):
     """Squares outside the f32 range; a norm above the largest f32 is Inf and the clip still finite."""
