@@ -151,7 +151,7 @@ def _tensors(grads) -> Sequence[torch.Tensor]:
 
 def global_grad_norm(grads: Sequence[torch.Tensor], grad_scale: float = 1.0) -> torch.Tensor:
     """The 2-norm of all `grads` (f32 and bf16 tensors of any shape on one device) taken as one vector, times
-    `|grad_scale|`, as an f32 device scalar: two launches for up to 128 tensors, no host synchronisation.  Squares and
+    `|grad_scale|`, as an f32 device scalar: two launches for up to 1024 tensors, no host synchronisation.  Squares and
     sums are 64-bit: it is NaN or Inf when some gradient is, and otherwise only above the largest f32."""
     return L.ext().global_grad_norm(_tensors(grads), grad_scale)
 
@@ -159,7 +159,7 @@ def global_grad_norm(grads: Sequence[torch.Tensor], grad_scale: float = 1.0) -> 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
                    grad_scale: float = 1.0) -> torch.Tensor:
     """Scales every gradient by `grad_scale * min(1, max_norm / (norm + 1e-6))`, where `norm` is their
-    `global_grad_norm` (with `grad_scale`), and returns that norm: two launches for up to 128 tensors, no host
+    `global_grad_norm` (with `grad_scale`), and returns that norm: two launches for up to 1024 tensors, no host
     synchronisation.  `grads` are scaled in place (they must be contiguous and must not overlap), or written to `out`:
     contiguous tensors of the same shapes and types that overlap nothing but their own gradient.  A norm that is not
     finite gives what the formula gives: zeros and NaN for Inf, NaN for NaN."""
