@@ -91,7 +91,7 @@ struct Like {
         there = t.defined();
         if (there) shape = t.sizes().vec(), type = t.scalar_type();
     }
-    Tensor back(const Tensor& g) const { return (g.scalar_type() == type ? g : g.to(type)).view(shape); }
+    Tensor back(const Tensor& g) const { return g.scalar_type() == type ? g : g.to(type); }
 };
 
 struct ResidualNormBackward : public Node {
@@ -137,7 +137,7 @@ struct ResidualNormBackward : public Node {
         for (int i = 0; i < 5; ++i) {
             if (!like[i].there || !task_should_compute_output(places[i])) continue;
             sums = true;
-            out[places[i]] = i < 3 ? at::empty({b, h}, opts.dtype(args.mod_f32 ? at::kFloat : at::kBFloat16)) : at::empty({h}, opts.dtype(at::kFloat));
+            out[places[i]] = at::empty(like[i].shape, opts.dtype(i >= 3 || args.mod_f32 ? at::kFloat : at::kBFloat16));  // b * h or h values
         }
         if (dr.defined()) {
             dr = rows_of(dr);
