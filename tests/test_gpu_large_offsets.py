@@ -50,6 +50,43 @@ def test_product(n, m):
     lb.check_device_status()
 
 
+@pytest.mark.parametrize("n,m", [(70_001, 32_768), (100, 22_000_000)])
+def test_adapter(n, m):
+    """The same with an adapter, and for the first its gradients: bounds as in tests/test_gpu_mx4_lora.py, for a corner."""
+    import loractl_b200 as lb
+
+    k, r, half = 64, 4, 2.0 ** -8
+    steps = lambda length: (length / 16 + 16) * 2.0 ** -22
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(n, k, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    layer = lb.Mx4Linear(lb.mx4_quantize(torch.randn(m, k, generator=g, device="cuda").bfloat16()))
+    lora = lb.LoraLinear(layer, r, 2.0 * r, device="cuda")
+    d = lora.delta
+    with torch.no_grad():
+        d.lora_a.normal_(generator=g), d.lora_b.normal_(generator=g)
+    y = lora(x)
+    assert y.numel() > 2 ** 31
+    a, b = d.lora_a.detach().bfloat16().double(), d.lora_b.detach().bfloat16().double()
+    few = layer.weight.dequantize(torch.bfloat16)[-5:].double()
+    xs, xq = x.detach()[-3:].double(), lb.mx4_quantize(x[-3:]).dequantize().double()
+    base, h = xq @ few.t(), 2.0 * (xs @ a)
+    ref = base + h @ b[:, -5:]
+    lim = half * (base.abs() + ref.abs() + h.abs() @ b[:, -5:].abs()) + steps(k) * (xq.abs() @ few.abs().t() + 2 * (xs.abs() @ a.abs()) @ b[:, -5:].abs())
+    assert bool(((y.detach()[-3:, -5:].double() - ref).abs() <= 1.02 * lim).all())
+    if n > m:
+        dy = torch.empty(n, m, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+        dx, db = torch.autograd.grad(y, [x, d.lora_b], dy)
+        w, dys = layer.weight.dequantize().double(), dy[-3:].double()
+        dh, dhm = 2.0 * (dys @ b.t()), 2.0 * (dys.abs() @ b.t().abs())
+        ref = dys @ w + dh @ a.t()
+        lim = half * (ref.abs() + dh.abs() @ a.t().abs()) + steps(m) * (dys.abs() @ w.abs() + 2 * (dhm @ a.t().abs()))
+        assert bool(((dx[-3:].double() - ref).abs() <= 1.02 * lim).all())
+        h, hm, last = 2.0 * (x.detach().double() @ a), 2.0 * (x.detach().double().abs() @ a.abs()), dy[:, -5:].double()
+        lim = half * (h.abs().t() @ last.abs()) + (steps(k) + steps(n)) * (hm.t() @ last.abs())
+        assert bool(((db[:, -5:].double() - h.t() @ last).abs() <= 1.02 * lim).all())
+    lb.check_device_status()
+
+
 def test_gradient_norm():
     import loractl_b200 as lb
 
