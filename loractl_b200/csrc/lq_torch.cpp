@@ -49,6 +49,15 @@ inline Tensor defined(const std::optional<Tensor>& t) { return t ? *t : Tensor()
 // The last axis contiguous (any other strides), a copy otherwise.
 inline Tensor rows_of(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
+// A saved tensor as unpacking gave it back.  Under saved-tensor hooks (checkpointing, offloading) that is another tensor than the
+// forward's, of any strides and at any address; so it is after a swap of `.data`.
+Tensor restored(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, at::Device device, const char* name) {
+    if (!t.defined()) return t;
+    TORCH_CHECK(t.sizes() == sizes && t.scalar_type() == type && t.device() == device, "the saved ", name, " came back as ", t.sizes(), " ",
+                t.scalar_type(), " on ", t.device(), ", it was ", sizes, " ", type, " on ", device);
+    return rows_of(t);
+}
+
 inline bool wants_grad(std::initializer_list<const Tensor*> inputs) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : inputs)
@@ -94,10 +103,20 @@ struct Like {
     Tensor back(const Tensor& g) const { return g.scalar_type() == type ? g : g.to(type); }
 };
 
+// What a call reads, with contiguous rows: x, y [b, t, h], vectors [b, h], weights f32 [h]; y, gate and weights may be undefined.
+struct ResidualNormInputs {
+    Tensor x, y, gate, shift, scale, weight, post_weight;
+    void put(lq_residual_norm_args& a) const {
+        a.x = ptr(x), a.x_sample = x.stride(0), a.x_token = x.stride(1);
+        if (y.defined()) a.y = ptr(y), a.y_sample = y.stride(0), a.y_token = y.stride(1), a.gate = ptr(gate), a.gate_sample = gate.stride(0);
+        a.shift = ptr(shift), a.shift_sample = shift.stride(0), a.scale = ptr(scale), a.scale_sample = scale.stride(0);
+        a.weight = (const float*)ptr(weight), a.post_weight = (const float*)ptr(post_weight);
+    }
+};
+
 struct ResidualNormBackward : public Node {
-    lq_residual_norm_args args;
-    // the addresses in `args` are those of these (r and z are not read by the backward)
-    SavedVariable x, y, gate, shift, scale, weight, post_weight;
+    lq_residual_norm_args args;  // of the inputs, only which there are: their addresses are those of what unpacking gives
+    SavedVariable x, y, gate, shift, scale, weight, post_weight;  // r and z are not read by the backward
     Tensor stats;
     Like like[5];  // gate, shift, scale, weight, post_weight
     bool two = false, released = false;
@@ -120,11 +139,20 @@ struct ResidualNormBackward : public Node {
         if (!dr.defined() && !dz.defined()) return out;
         // unpacking checks that none was changed in place; the tensors keep their memory through the launch
         const Tensor tensors[7] = {x.unpack(), y.unpack(), gate.unpack(), shift.unpack(), scale.unpack(), weight.unpack(), post_weight.unpack()};
-        const Tensor& xs = tensors[0];
         at::NoGradGuard no_grad;
-        c10::cuda::OptionalCUDAGuard guard(xs.device());
+        const auto device = stats.device();
+        c10::cuda::OptionalCUDAGuard guard(device);
         const int64_t b = args.samples, h = args.h;
+        const auto type = args.dtype == LQ_F32 ? at::kFloat : at::kBFloat16, mod = args.mod_f32 ? at::kFloat : at::kBFloat16;
+        const std::vector<int64_t> rows = {b, args.tokens, h}, vectors = {b, h}, columns = {h};
+        const ResidualNormInputs in = {restored(tensors[0], rows, type, device, "x"), restored(tensors[1], rows, type, device, "y"),
+                                       restored(tensors[2], vectors, mod, device, "gate"), restored(tensors[3], vectors, mod, device, "shift"),
+                                       restored(tensors[4], vectors, mod, device, "scale"), restored(tensors[5], columns, at::kFloat, device, "weight"),
+                                       restored(tensors[6], columns, at::kFloat, device, "post_weight")};
+        const Tensor& xs = in.x;
         const auto opts = xs.options().requires_grad(false);
+        lq_residual_norm_args args = this->args;
+        in.put(args);
         lq_residual_norm_grads g = {};
         auto token = [&](int i) {
             if (!task_should_compute_output(i)) return Tensor();
@@ -185,35 +213,35 @@ std::vector<Tensor> residual_norm(const Tensor& x_, const std::optional<Tensor>&
     }
     TORCH_CHECK_VALUE(y0.defined() == gate0.defined(), "gate and y go together");
     const bool grad = wants_grad({&x_, &gate0, &y0, &shift_, &scale_, &weight0, &post0});
-    Tensor x, y, gate, shift, scale, w, pw, r, z, stats;
+    ResidualNormInputs in;
+    Tensor r, z, stats;
     c10::cuda::OptionalCUDAGuard guard(x_.device());
     {
         at::NoGradGuard no_grad;
-        x = rows_of(x_), shift = vector_of(shift_, b, h, type, "shift"), scale = vector_of(scale_, b, h, type, "scale");
-        w = weight_of(weight0, h, "weight"), pw = weight_of(post0, h, "post_weight");
-        const auto opts = x.options().requires_grad(false);
+        in.x = rows_of(x_), in.shift = vector_of(shift_, b, h, type, "shift"), in.scale = vector_of(scale_, b, h, type, "scale");
+        in.weight = weight_of(weight0, h, "weight"), in.post_weight = weight_of(post0, h, "post_weight");
+        const auto opts = x_.options().requires_grad(false);
         z = at::empty({b, t, h}, opts);
         if (y0.defined()) {
-            y = rows_of(y0), gate = vector_of(gate0, b, h, type, "gate"), r = at::empty({b, t, h}, opts);
-            a.y = ptr(y), a.y_sample = y.stride(0), a.y_token = y.stride(1), a.gate = ptr(gate), a.gate_sample = gate.stride(0), a.r = mut(r);
+            in.y = rows_of(y0), in.gate = vector_of(gate0, b, h, type, "gate"), r = at::empty({b, t, h}, opts);
+            a.r = mut(r);
         }
         if (grad) {
             stats = at::empty({3, b * t}, opts.dtype(at::kFloat));
             a.mean = stats.data_ptr<float>(), a.rstd = a.mean + b * t, a.post_rstd = a.rstd + b * t;
         }
-        a.x = ptr(x), a.x_sample = x.stride(0), a.x_token = x.stride(1);
-        a.shift = ptr(shift), a.shift_sample = shift.stride(0), a.scale = ptr(scale), a.scale_sample = scale.stride(0);
-        a.weight = (const float*)ptr(w), a.post_weight = (const float*)ptr(pw), a.z = mut(z);
+        in.put(a);
+        a.z = mut(z);
         a.samples = b, a.tokens = t, a.h = h, a.mod_f32 = type == at::kFloat, a.layer = layer, a.alpha = (float)alpha, a.eps = (float)eps;
-        check(lq_residual_norm_fwd(&a, stream_of(x)));
+        check(lq_residual_norm_fwd(&a, stream_of(x_)));
     }
     if (grad) {
         auto node = std::shared_ptr<ResidualNormBackward>(new ResidualNormBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x_, gate0, y0, shift_, scale_, weight0, post0));
         node->args = a;
-        node->x = SavedVariable(x, false), node->y = SavedVariable(y, false), node->gate = SavedVariable(gate, false);
-        node->shift = SavedVariable(shift, false), node->scale = SavedVariable(scale, false);
-        node->weight = SavedVariable(w, false), node->post_weight = SavedVariable(pw, false);
+        node->x = SavedVariable(in.x, false), node->y = SavedVariable(in.y, false), node->gate = SavedVariable(in.gate, false);
+        node->shift = SavedVariable(in.shift, false), node->scale = SavedVariable(in.scale, false);
+        node->weight = SavedVariable(in.weight, false), node->post_weight = SavedVariable(in.post_weight, false);
         node->stats = stats;
         node->two = r.defined();
         const Tensor* vectors[5] = {&gate0, &shift_, &scale_, &weight0, &post0};
