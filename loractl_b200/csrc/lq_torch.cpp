@@ -49,6 +49,12 @@ inline Tensor defined(const std::optional<Tensor>& t) { return t ? *t : Tensor()
 // The last axis contiguous (any other strides), a copy otherwise.
 inline Tensor rows_of(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
+// Contiguous and on 16 bytes, a copy if it is not.
+inline Tensor whole(const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return (uintptr_t)ptr(c) % 16 ? c.clone() : c;
+}
+
 // A saved tensor as unpacking gave it back.  Under saved-tensor hooks (checkpointing, offloading) that is another tensor than the
 // forward's, of any strides and at any address; so it is after a swap of `.data`.
 Tensor restored(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, at::Device device, const char* name) {
@@ -471,8 +477,7 @@ Tensor mx4_matmul_dx(const Tensor& dy_, const Tensor& wc, const Tensor& ws, int6
     TORCH_CHECK(dy_.device() == wc.device(), "dy is on ", dy_.device(), ", w on ", wc.device());
     const int type = dtype_code(dy_);
     c10::cuda::OptionalCUDAGuard guard(dy_.device());
-    Tensor dy = dy_.contiguous();
-    if ((uintptr_t)ptr(dy) % 16) dy = dy.clone();
+    const Tensor dy = whole(dy_);
     const int64_t n = dy.size(0);
     Tensor dx = at::empty({n, k}, dy.options().requires_grad(false));
     // of this call alone: from the pool of the current stream, or of the graph being captured
@@ -530,8 +535,8 @@ Tensor mx4_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int64_t 
 struct Mx4LoraBackward : public Node {
     Tensor codes, scales, mirror, h;   // state, never graph parents
     Tensor bucket_a, bucket_b;         // views of a flat gradient buffer, or undefined
-    SavedVariable x, a, b;
-    int64_t m = 0, k = 0;
+    SavedVariable x, a, b;             // a and b for their versions and .grad: the mirror holds their values
+    int64_t n = 0, m = 0, k = 0, rank = 0;
     double scaling = 1.0;
     std::vector<int64_t> shape;
     bool released = false;
@@ -551,12 +556,10 @@ struct Mx4LoraBackward : public Node {
     variable_list gradients(variable_list&& grads) {
         variable_list out(3);
         if (!grads[0].defined()) return out;
-        const Tensor xs = x.unpack(), as = a.unpack(), bs = b.unpack();
+        const Tensor saved = x.unpack(), as = a.unpack(), bs = b.unpack();
         at::NoGradGuard no_grad;
-        c10::cuda::OptionalCUDAGuard guard(xs.device());
-        Tensor dy = grads[0].reshape({-1, m}).contiguous();
-        if ((uintptr_t)ptr(dy) % 16) dy = dy.clone();
-        const int64_t n = dy.size(0), rank = as.size(1);
+        c10::cuda::OptionalCUDAGuard guard(codes.device());
+        const Tensor xs = whole(restored(saved, {n, k}, at::kBFloat16, codes.device(), "x")), dy = whole(grads[0].reshape({n, m}));
         // straight into the flat buffer only while the factors' .grad are its views: whoever reset them expects autograd's
         auto lives = [](const Tensor& p, const Tensor& view) {
             return view.defined() && p.grad().defined() && p.grad().const_data_ptr() == view.const_data_ptr();
@@ -594,8 +597,7 @@ Tensor mx4_lora_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int
     Tensor x, y, h;
     {
         at::NoGradGuard no_grad;
-        x = x_.reshape({-1, k}).contiguous();
-        if ((uintptr_t)ptr(x) % 16) x = x.clone();
+        x = whole(x_.reshape({-1, k}));
         const Tensor bias = bias_of(bias_, wc, m);
         const int64_t n = x.size(0);
         auto shape = x_.sizes().vec();
@@ -613,7 +615,7 @@ Tensor mx4_lora_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int
         node->x = SavedVariable(x, false), node->a = SavedVariable(a, false), node->b = SavedVariable(b, false);
         node->codes = wc, node->scales = ws, node->mirror = mirror, node->h = h;
         node->bucket_a = defined(bucket_a), node->bucket_b = defined(bucket_b);
-        node->m = m, node->k = k, node->scaling = scaling, node->shape = x_.sizes().vec();
+        node->n = x.size(0), node->m = m, node->k = k, node->rank = rank, node->scaling = scaling, node->shape = x_.sizes().vec();
         torch::autograd::set_history(y, node);
     }
     return y;

@@ -138,6 +138,50 @@ def test_seam_refuses_what_a_hook_must_not_give_back():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,m,k,r", [(1, 64, 96, 4), (40, 136, 160, 16), (300, 520, 256, 16)])
+def test_adapter_under_hooks(n, m, k, r):
+    """The microscaled linear with an adapter: every copy has the rows of the original again before the kernels read it."""
+    from tests.test_gpu_mx4_lora import site
+
+    _, lora, x, dy = site(n, m, k, r)
+    x = x.detach().requires_grad_(True)
+    args = [x, lora.delta.lora_a, lora.delta.lora_b]
+    want = torch.autograd.grad(lora(x * 1), args, dy)
+    copies = lambda t: t.clone()
+    for unpack in (copies, padded, turned):
+        with torch.autograd.graph.saved_tensors_hooks(copies, unpack):
+            y = lora(x * 1)
+        junk = overwrite([x])
+        for ours, ref in zip(torch.autograd.grad(y, args, dy), want):
+            assert torch.equal(ours, ref)
+        del junk
+    y = checkpoint(lambda t: lora(t * 1), x, use_reentrant=False)
+    for ours, ref in zip(torch.autograd.grad(y, args, dy), want):
+        assert torch.equal(ours, ref)
+    for unpack in (lambda t: t.float(), lambda t: t[..., :-1]):
+        with torch.autograd.graph.saved_tensors_hooks(copies, unpack):
+            y = lora(x * 1)
+        with pytest.raises(RuntimeError, match="came back as"):
+            torch.autograd.grad(y, args, dy)
+
+
+@pytest.mark.gpu
+def test_adapter_adds_into_the_flat_buffer_under_a_checkpoint():
+    """The unpacked factors are other tensors than the leaves, so autograd accumulates: into the same views, the same sums."""
+    import loractl_b200 as lb
+    from tests.test_gpu_mx4_lora import site
+
+    _, lora, x, dy = site(40, 136, 160, 16)
+    d = lora.delta
+    want = torch.autograd.grad(lora(x), [d.lora_a, d.lora_b], dy)
+    flat = lb.FlatAdapters(lb.LoraAdapters([d], ["site"]), "cuda")
+    flat.zero_grad()
+    checkpoint(lora, x, use_reentrant=False).backward(dy)
+    for i, p in enumerate((d.lora_a, d.lora_b)):
+        assert p.grad.data_ptr() == flat.grad_views(0)[i].data_ptr() and torch.equal(p.grad, want[i])
+
+
+@pytest.mark.gpu
 def test_trunk_block_under_a_checkpoint():
     """A trunk block in bf16 on MXFP4 with adapters and the fused norms, recomputed.  The recomputed forward is the same; the
     gradient of torch's attention may add up in another order, and what it rounds to bf16 then differs by a step of 2^-7 of an element at
