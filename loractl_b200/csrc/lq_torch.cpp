@@ -70,6 +70,11 @@ inline bool wants_grad(std::initializer_list<const Tensor*> inputs) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// A forward-mode tangent that the node would drop is refused, as torch.autograd.Function does without a jvp.
+void no_tangents(std::initializer_list<const Tensor*> inputs, const char* name) {
+    for (const Tensor* t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), name, " has no forward-mode derivative");
+}
 // Gradients that are themselves to be differentiated (create_graph) fail when that is tried, as torch's
 // once_differentiable does.
 variable_list once(variable_list&& grads, const char* name) {
@@ -143,6 +148,7 @@ struct ResidualNormBackward : public Node {
         variable_list out(7);
         Tensor dr = two ? grads[0] : Tensor(), dz = grads[two ? 1 : 0];
         if (!dr.defined() && !dz.defined()) return out;
+        no_tangents({&dr, &dz}, "the residual norm's backward");
         // unpacking checks that none was changed in place; the tensors keep their memory through the launch
         const Tensor tensors[7] = {x.unpack(), y.unpack(), gate.unpack(), shift.unpack(), scale.unpack(), weight.unpack(), post_weight.unpack()};
         at::NoGradGuard no_grad;
@@ -197,6 +203,7 @@ std::vector<Tensor> residual_norm(const Tensor& x_, const std::optional<Tensor>&
                                   const Tensor& scale_, const std::optional<Tensor>& weight_, const std::optional<Tensor>& post_weight_,
                                   bool layer, double alpha, double eps) {
     const Tensor gate0 = defined(gate_), y0 = defined(y_), weight0 = defined(weight_), post0 = defined(post_weight_);
+    no_tangents({&x_, &gate0, &y0, &shift_, &scale_, &weight0, &post0}, "the residual norm");
     require_cuda(x_, "x");
     TORCH_CHECK_VALUE(x_.dim() == 3, "expected [b, tokens, h], got ", x_.sizes());
     const int64_t b = x_.size(0), t = x_.size(1), h = x_.size(2);
@@ -495,6 +502,7 @@ struct Mx4LinearBackward : public Node {
     variable_list apply(variable_list&& grads) override {
         const bool asked = at::GradMode::is_enabled();
         if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+        no_tangents({&grads[0]}, "Mx4Linear's backward");
         at::NoGradGuard no_grad_in_here;
         const Tensor dy = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, m});
         variable_list out = {mx4_matmul_dx(dy, codes, scales, m, k).view(shape)};
@@ -505,6 +513,8 @@ struct Mx4LinearBackward : public Node {
 
 // dequant(quant(x)) . dequant(w)^T + bias over the last axis of x; backward dy . dequant(w).
 Tensor mx4_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int64_t m, int64_t k, const std::optional<Tensor>& bias_) {
+    const Tensor bias0 = defined(bias_);
+    no_tangents({&x_, &bias0}, "Mx4Linear");
     require_cuda(x_, "x");
     TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) == k, "last dim ", x_.dim() ? x_.size(-1) : 0, " != d_in ", k);
     TORCH_CHECK(x_.device() == wc.device(), "x is on ", x_.device(), ", w on ", wc.device());
@@ -556,6 +566,7 @@ struct Mx4LoraBackward : public Node {
     variable_list gradients(variable_list&& grads) {
         variable_list out(3);
         if (!grads[0].defined()) return out;
+        no_tangents({&grads[0]}, "the backward of the microscaled linear with an adapter");
         const Tensor saved = x.unpack(), as = a.unpack(), bs = b.unpack();
         at::NoGradGuard no_grad;
         c10::cuda::OptionalCUDAGuard guard(codes.device());
@@ -583,6 +594,8 @@ struct Mx4LoraBackward : public Node {
 Tensor mx4_lora_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int64_t m, int64_t k, const std::optional<Tensor>& bias_,
                        const Tensor& a, const Tensor& b, double scaling, const Tensor& mirror, const std::optional<Tensor>& bucket_a,
                        const std::optional<Tensor>& bucket_b) {
+    const Tensor bias0 = defined(bias_);
+    no_tangents({&x_, &a, &b, &bias0}, "the microscaled linear with an adapter");
     require_cuda(x_, "x");
     TORCH_CHECK_VALUE(x_.dim() >= 1 && x_.size(-1) == k, "last dim ", x_.dim() ? x_.size(-1) : 0, " != d_in ", k);
     TORCH_CHECK_TYPE(x_.scalar_type() == at::kBFloat16, "the fused adapter takes bf16 activations, got ", x_.scalar_type());
