@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const Norm q) {
 }
 
 // The factor as m * p: p = 1 and m the factor rounded to f32, except where that would be subnormal (a norm
-// above 2^126 max_norm): there m is in [0.5, 1) and p the power of two, so that m keeps all its bits.
+// above 2^126 max_norm): there m is in [0.5, 1], rounded up to 1 from just below, and p the power of two, so that m keeps all its bits.
 struct Factor {
     float m, p;
     __device__ __forceinline__ float operator()(float v) const { return v * m * p; }
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
     const int chunks = l.first[l.count];
     for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         const int i = tensor_of(l, c);
-        if (f.m == 1.f && l.out[i] == l.g[i]) continue;  // in place and nothing to scale: every value stays as it is
+        if (f.m == 1.f && f.p == 1.f && l.out[i] == l.g[i]) continue;  // in place and nothing to scale: every value stays as it is
         const bool bf = l.n[i] < 0;
         const int esz = bf ? 2 : 4;
         const int64_t e0 = (int64_t)(c - l.first[i]) * (kChunkBytes / esz);
