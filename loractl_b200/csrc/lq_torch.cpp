@@ -344,14 +344,24 @@ Spans spans_of(const std::vector<const void*>& at, const std::vector<int64_t>& b
     return s;
 }
 
-// Outputs may be the gradients themselves, one for one, and share no byte with anything else.
-void check_outputs(const std::vector<const void*>& at, const std::vector<const void*>& out, const std::vector<int64_t>& bytes) {
+// The bytes from a tensor's first element to the end of its last; a strided one counts with the gaps between.
+int64_t extent_of(const Tensor& t) {
+    if (t.numel() == 0 || t.is_contiguous()) return t.nbytes();
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * t.element_size();
+}
+
+// Outputs (contiguous, `bytes` each) may be the gradients themselves, one for one, and share no byte with anything else;
+// `extents` are those of the gradients.
+void check_outputs(const std::vector<const void*>& at, const std::vector<int64_t>& extents, const std::vector<const void*>& out,
+                   const std::vector<int64_t>& bytes) {
     const Spans o = spans_of(out, bytes);
     for (size_t i = 1; i < o.size(); ++i)
         TORCH_CHECK_VALUE(o[i - 1].second <= o[i].first, "the clipped tensors overlap one another (the same tensor twice?)");
     if (&at == &out) return;
     // the usual call, whose outputs are all apart from the gradients: one walk along both
-    const Spans g = spans_of(at, bytes);
+    const Spans g = spans_of(at, extents);
     bool apart = true;
     for (size_t i = 0, j = 0; apart && i < g.size(); ++i) {
         while (j < o.size() && o[j].second <= g[i].first) ++j;
@@ -373,11 +383,11 @@ void check_outputs(const std::vector<const void*>& at, const std::vector<const v
 void check_outputs_py(const py::object& grad_list, const py::object& out_list) {
     const std::vector<Tensor> grads = tensors_of(grad_list, "gradients"), outs = tensors_of(out_list, "outputs");
     std::vector<const void*> at, out;
-    std::vector<int64_t> bytes;
-    for (const Tensor& t : grads) at.push_back(t.const_data_ptr()), bytes.push_back(t.nbytes());
-    for (const Tensor& t : outs) out.push_back(t.const_data_ptr());
-    if (at == out) check_outputs(at, at, bytes);
-    else check_outputs(at, out, bytes);
+    std::vector<int64_t> extents, bytes;
+    for (const Tensor& t : grads) at.push_back(t.const_data_ptr()), extents.push_back(extent_of(t));
+    for (const Tensor& t : outs) out.push_back(t.const_data_ptr()), bytes.push_back(t.nbytes());
+    if (at == out) check_outputs(at, extents, at, bytes);
+    else check_outputs(at, extents, out, bytes);
 }
 
 Tensor clip_grad_norm(const py::object& list, double max_norm, const py::object& out_list, double grad_scale) {
@@ -400,11 +410,15 @@ Tensor clip_grad_norm(const py::object& list, double max_norm, const py::object&
     TORCH_CHECK_VALUE(all_contiguous(outs), out ? "out tensors must be contiguous" : "gradients that are clipped in place must be contiguous");
     std::vector<int64_t> bytes;
     for (size_t i = 0; i < grads.size(); ++i) bytes.push_back(g.counts[i] * (g.types[i] == LQ_F32 ? 4 : 2));
-    check_outputs(g.at, out ? to : g.at, bytes);
+    const bool strided = out && !all_contiguous(grads);
+    std::vector<int64_t> extents;
+    if (strided)
+        for (const Tensor& t : grads) extents.push_back(extent_of(t));
+    check_outputs(g.at, strided ? extents : bytes, out ? to : g.at, bytes);
     c10::cuda::OptionalCUDAGuard guard(grads[0].device());
     std::vector<Tensor> copies;
     std::vector<const void*> at = g.at;
-    if (out && !all_contiguous(grads)) {
+    if (strided) {
         copies = contiguous(grads);
         for (size_t i = 0; i < copies.size(); ++i) at[i] = copies[i].const_data_ptr();
     }

@@ -161,7 +161,8 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
     """Scales every gradient by `grad_scale * min(1, max_norm / (norm + 1e-6))`, where `norm` is their
     `global_grad_norm` (with `grad_scale`), and returns that norm: two launches for up to 1024 tensors, no host
     synchronisation.  `grads` are scaled in place (they must be contiguous and must not overlap), or written to `out`:
-    contiguous tensors of the same shapes and types that overlap nothing but their own gradient.  A norm that is not
+    contiguous tensors of the same shapes and types that overlap nothing but their own gradient (a strided one from its first
+    element to its last).  A norm that is not
     finite gives what the formula gives: zeros and NaN for Inf, NaN for NaN."""
     return L.ext().clip_grad_norm(_tensors(grads), max_norm, None if out is None else _tensors(out), grad_scale)
 
