@@ -615,6 +615,8 @@ Tensor mx4_lora_linear(const Tensor& x_, const Tensor& wc, const Tensor& ws, int
     TORCH_CHECK_TYPE(x_.scalar_type() == at::kBFloat16, "the fused adapter takes bf16 activations, got ", x_.scalar_type());
     const std::pair<const char*, const Tensor*> named[] = {{"w", &wc}, {"lora_a", &a}, {"lora_b", &b}, {"the mirror", &mirror}};
     for (const auto& [name, v] : named) TORCH_CHECK(v->device() == x_.device(), name, " is on ", v->device(), ", x on ", x_.device());
+    TORCH_CHECK_TYPE(a.scalar_type() == at::kFloat && b.scalar_type() == at::kFloat, "LoRA factors must be f32, got ", a.scalar_type(), " and ",
+                     b.scalar_type());
     const int64_t rank = a.dim() == 2 ? a.size(1) : 0;
     TORCH_CHECK_VALUE(rank > 0 && a.size(0) == k && b.dim() == 2 && b.size(0) == rank && b.size(1) == m, "lora_a must be [", k,
                       ", rank], lora_b [rank, ", m, "], got ", a.sizes(), " and ", b.sizes());

@@ -258,11 +258,22 @@ def _compute_code(t: torch.Tensor, fp8_compute: bool) -> int:
     return dt
 
 
+def _check_factors(a: torch.Tensor, b: torch.Tensor) -> None:
+    """The mirror kernels read `a` [d_in, r] and `b` [r, d_out] as contiguous f32 through raw addresses."""
+    if a.dtype != torch.float32 or b.dtype != torch.float32:
+        raise TypeError(f"LoRA factors must be f32, got {a.dtype} and {b.dtype}")
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[0] or not a.is_contiguous() or not b.is_contiguous():
+        raise ValueError(f"LoRA factors must be contiguous [d_in, rank] and [rank, d_out], got {list(a.shape)} and {list(b.shape)}")
+    _require_cuda(a, "lora_a")
+    if b.device != a.device:
+        raise RuntimeError(f"lora_a is on {a.device}, lora_b on {b.device}")
+
+
 def lora_mirror(a: torch.Tensor, b: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bf16 operand mirror of one site's factors (`lq_lora_mirror_update`): `a` is `[d_in, r]`, `b` is
     `[r, d_out]`, both f32 on the device.  Returns the (256-byte aligned) byte buffer to pass as
     `mirror=` to `linear_fwd_raw` / `linear_bwd_raw`; pass `out` to refresh an existing one in place."""
-    _require_cuda(a, "lora_a")
+    _check_factors(a, b)
     d_in, r = a.shape
     d_out = b.shape[1]
     need = int(L.lib().lq_lora_mirror_bytes(d_in, d_out, r))
@@ -295,7 +306,7 @@ def lora_mirror_batch(jobs) -> None:
 
     arr = (L.MirrorJob * len(jobs))()
     for i, (a, b, m) in enumerate(jobs):
-        _require_cuda(a, "lora_a")
+        _check_factors(a, b)
         arr[i] = L.MirrorJob(a.data_ptr(), b.data_ptr(), a.shape[0], b.shape[1], a.shape[1], m.data_ptr())
     dev = jobs[0][0].device
     with torch.cuda.device(dev):
