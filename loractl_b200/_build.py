@@ -5,11 +5,12 @@ cross-compiles without a GPU; the resulting `lib/libloractl_b200.so` is what
 `loractl_b200._lib` loads.  Every translation unit is compiled to its own object
 (in parallel, and only when it or a header changed), then linked; internal C++
 symbols are hidden, only the C ABI of include/loractl_b200.h is exported.  The PyTorch binding of the
-short calls (`lib/_lq_torch.so`, csrc/lq_torch.cpp) is built with g++ against the installed torch.
+short calls (`lib/_lq_torch.*.so`, csrc/lq_torch.cpp) is built with g++ against the installed torch.
 """
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.metadata
 import pathlib
 import shutil
 import subprocess
@@ -24,7 +25,6 @@ SOURCES = ["lq_api.cu", "lq_quant.cu", "lq_simt.cu", "lq_tc.cu", "lq_w4.cu", "lq
            "lq_block.cu", "lq_resnorm.cu", "lq_gradnorm.cu", "lq_mx4.cu"]
 # the PyTorch binding of the short calls: a Python module that links the library and torch
 TORCH_SRC = CSRC / "lq_torch.cpp"
-TORCH_MODULE = PKG / "lib" / "_lq_torch.so"
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -39,16 +39,26 @@ def _stale(out: pathlib.Path, deps_mtime: float) -> bool:
     return not out.exists() or out.stat().st_mtime < deps_mtime
 
 
+def torch_module() -> pathlib.Path:
+    """The binding for this Python and the installed torch, whose C++ internals it is compiled against: they stand in its name,
+    so that another torch asks for a build of its own.  (torch itself is not imported.)"""
+    return PKG / "lib" / f"_lq_torch.{sys.implementation.cache_tag}-torch{importlib.metadata.version('torch')}.so"
+
+
+def _torch_module_stale() -> bool:
+    return _stale(torch_module(), max(HEADER.stat().st_mtime, TORCH_SRC.stat().st_mtime))
+
+
 def needs_build() -> bool:
     hdr = _headers_mtime()
-    if _stale(LIB, hdr) or _stale(TORCH_MODULE, max(HEADER.stat().st_mtime, TORCH_SRC.stat().st_mtime)):
+    if _stale(LIB, hdr) or _torch_module_stale():
         return True
     return any((CSRC / s).stat().st_mtime > LIB.stat().st_mtime for s in SOURCES)
 
 
 def _build_torch_module(force: bool) -> None:
     """g++ on csrc/lq_torch.cpp against the installed torch; finds the library beside itself."""
-    if not force and not _stale(TORCH_MODULE, max(HEADER.stat().st_mtime, TORCH_SRC.stat().st_mtime)):
+    if not force and not _torch_module_stale():
         return
     import sysconfig
 
@@ -60,7 +70,7 @@ def _build_torch_module(force: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_lq_torch",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{p}" for p in [*include_paths(), sysconfig.get_paths()["include"], cuda / "include"]],
-           "-o", str(TORCH_MODULE), str(TORCH_SRC), f"-L{LIB.parent}", f"-l:{LIB.name}", f"-L{libs}", "-lc10", "-lc10_cuda",
+           "-o", str(torch_module()), str(TORCH_SRC), f"-L{LIB.parent}", f"-l:{LIB.name}", f"-L{libs}", "-lc10", "-lc10_cuda",
            "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:

@@ -139,9 +139,12 @@ def ext():
     """The PyTorch binding of the short calls (csrc/lq_torch.cpp); raises if it has not been built."""
     global _ext
     if _ext is None:
-        path = LIB_PATH.parent / "_lq_torch.so"
+        from . import _build
+
+        path = _build.torch_module()
         if not path.exists():
-            raise RuntimeError(f"{path} is missing: build it with `python -m loractl_b200._build`. There is no fallback for it.")
+            raise RuntimeError(f"{path} is missing: build it with `python -m loractl_b200._build` (each torch needs its own). "
+                               "There is no fallback for it.")
         import importlib.util
 
         import torch  # noqa: F401  (its libraries come first)
