@@ -27,10 +27,13 @@
 
 #include "lq_internal.cuh"
 #include "lq_prof.cuh"
+#include "lq_resnorm_plan.cuh"
 #include "lq_tc.cuh"
 #include "lq_umma.cuh"
 
 namespace {
+
+using namespace resnorm_plan;
 
 typedef lq_residual_norm_args Args;
 
@@ -115,7 +118,6 @@ struct Rows {
 // backward on 1536 rows of 6144 bf16 columns, where this takes 17 and 25; the modulation read again from L1 for every row
 // was part of that.  At 4096 rows 34 us and 63 us: 89 % and 73 % of the measured HBM rate; 8 x 4096 x 2048 with the layer
 // norm 93 us and 150 us: 88 % and 82 %.
-constexpr int kMaxStages = 8;
 
 // Eight elements as they are stored (four registers in bf16): what is needed again behind a barrier waits like this.
 template <typename T>
@@ -810,7 +812,7 @@ __global__ void __launch_bounds__(512) resnorm_final_kernel(const Args a, const 
 // ---- host ---------------------------------------------------------------------------------------
 
 constexpr int64_t kMaxH = 16384;  // 1024 threads x 16 elements
-constexpr size_t kRingBytes = 216 * 1024;  // shared memory of an SM for the rings of its blocks
+static_assert(sizeof(float[2][2][kMaxWarps]) + sizeof(uint64_t[kMaxStages]) + 16 <= kRingStatic, "a ring block's own shared memory");
 
 inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -828,42 +830,6 @@ bool vectors_ok(const Args& a, const lq_residual_norm_grads* g) {
         if (g->dr) ok = ok && al16(g->dr) && g->dr_sample % v == 0 && g->dr_token % v == 0;
     }
     return ok;
-}
-
-int threads_of(int64_t h) { return (int)((h + 255) / 256 * 32); }  // 8 columns each
-
-// Blocks of an SM: 1024 threads with the forward's 64 registers, 768 with the backward's 80 (the launch bounds below).
-int blocks_per_sm(int64_t h, bool backward) { return std::max(1, (backward ? 768 : 1024) / threads_of(h)); }
-
-// ... and of the kernels for any rows: 8 elements a thread in up to 512 threads (128 registers; 64 in the forward), then
-// up to 1024 threads, then 16 elements.
-int scalar_threads(int64_t h) {
-    const int64_t e = h <= 8192 ? 8 : 16;
-    return (int)(((h + e - 1) / e + 31) / 32 * 32);
-}
-int scalar_blocks_per_sm(int64_t h, bool backward) { return std::max(1, (backward ? 512 : 1024) / scalar_threads(h)); }
-
-// Chunks of one sample, one block each: such that all blocks fill the SMs' places once, or w times where one round
-// would leave too many empty (a round beyond the last full one costs as much as a whole one: 448 blocks on 444 places took
-// 292 us where 440 take 256, 8 x 4096 x 2048 forward and backward); in the backward four rows or more each where that still
-// gives every SM a block (a chunk leaves three partial rows, so a short one costs as much traffic as its rows).
-int chunks_of(int64_t samples, int64_t tokens, int64_t places, int sms, bool backward) {
-    const int64_t one = (sms + samples - 1) / samples;
-    const int64_t most = std::max<int64_t>(1, backward ? std::min(tokens, std::max(tokens / 4, one)) : tokens);
-    int64_t best = 1, cost = -1;
-    for (int64_t w = 1; w <= 4; ++w) {
-        const int64_t c = std::min(most, std::max<int64_t>(1, places * w / samples));
-        const int64_t t = (samples * c + places - 1) / places * ((tokens + c - 1) / c + 2);
-        if (cost < 0 || t < cost) best = c, cost = t;
-    }
-    return (int)best;
-}
-
-// Rows in the ring of a block, 0 when fewer than two fit.
-int stages_of(int64_t h, int dtype, int inputs, bool backward) {
-    const size_t stage = (size_t)inputs * h * (dtype == LQ_F32 ? 4 : 2);
-    const size_t n = kRingBytes / blocks_per_sm(h, backward) / stage;
-    return n < 2 ? 0 : (int)std::min<size_t>(n, kMaxStages);
 }
 
 // Three partial rows a chunk, then three totals a sample.
@@ -956,7 +922,7 @@ void launch_ring(int dev, unsigned grid, int threads, size_t smem, cudaStream_t 
 constexpr int64_t kRingMaxH = 8192;  // 1024 threads x 8 columns
 
 void forward(const Args& a, int dev, cudaStream_t st) {
-    const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype, inputs, false) : 0;
+    const int inputs = a.y ? 2 : 1, stages = a.h <= kRingMaxH && vectors_ok(a, nullptr) ? stages_of(a.h, a.dtype == LQ_F32 ? 4 : 2, inputs, false) : 0;
     const int sms = lq_tc_sm_count(dev);
     const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, false) : scalar_blocks_per_sm(a.h, false)), sms, false);
     const int64_t per = (a.tokens + chunks - 1) / chunks;
@@ -984,7 +950,7 @@ int most_chunks(int64_t samples, int64_t tokens, int64_t h, int sms) {
 // Returns the chunks that it used.
 int backward(const Args& a, const lq_residual_norm_grads& g, float* part, int dev, cudaStream_t st) {
     const int inputs = 1 + (a.y ? 1 : 0) + (g.dz ? 1 : 0) + (g.dr ? 1 : 0);
-    const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype, inputs, true) : 0;
+    const int stages = a.h <= kRingMaxH && vectors_ok(a, &g) ? stages_of(a.h, a.dtype == LQ_F32 ? 4 : 2, inputs, true) : 0;
     const int sms = lq_tc_sm_count(dev);
     const int chunks = chunks_of(a.samples, a.tokens, (int64_t)sms * (stages ? blocks_per_sm(a.h, true) : scalar_blocks_per_sm(a.h, true)), sms, true);
     const int64_t per = (a.tokens + chunks - 1) / chunks;
