@@ -307,7 +307,7 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
 /* A LoRA adapter on such a weight (crates/loractl-core/src/mmdit.rs:526-536), bf16 activations:
  *   H = X . A,   Y = quant(X) . W^T + bias + scaling * H . B,
  *   dX = dY . W + scaling * dY . B^T . A^T,   dA = scaling * X^T . dY . B^T,   dB = scaling * H^T . dY,
- * the adapter reading X itself.  `mirror`: lq_lora_mirror_update() of the factors (A [k, rank], B [rank, m]); m a multiple of
+ * the adapter reading X itself; Y is rounded once, s * H and dH once each as operands.  `mirror`: lq_lora_mirror_update() of the factors (A [k, rank], B [rank, m]); m a multiple of
  * 8, rank <= 256; x, dy, y and dx contiguous, 16-byte aligned.  `h_out` / `h`: f32 [n, rank], may be NULL (the backward then
  * computes it again).  dX, dA and dB may be NULL; `accumulate` adds to dA and dB.  `ws`: lq_mx4_lora_workspace_bytes() bytes,
  * 256-byte aligned, of the forward or the backward; calls that can overlap need one each. */

@@ -857,8 +857,9 @@ int splits_of(int64_t tiles, int64_t kb, int sms) {
 
 // Pairs of SMs where their 256 x 256 tiles occupy two thirds of them; below, 128 x 128 tiles split along k spread
 // wider.  At k = 6144 (pair | stream, us): 24 tiles 16.1 | 14.4, 48 tiles 16.4 | 16.1, 72 tiles 16.9 | 16.9, 128 tiles 28 | 35, 384 tiles 71 | 93.
-bool use_pair(int64_t n, int64_t m, int sms) {
-    return n > 128 && m > 128 && ((n + 255) / 256) * ((m + 255) / 256) * 3 > sms;
+bool use_pair(int64_t n, int64_t m) {
+    constexpr int64_t kSms = 148;  // workspaces are sized by this rule too, without a device
+    return n > 128 && m > 128 && ((n + 255) / 256) * ((m + 255) / 256) * 3 > kSms;
 }
 
 template <int BN>
@@ -980,7 +981,7 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
     p.y = y;
     p.y_f32 = y_dtype == LQ_F32;
     p.status = lq_tc_status_word(dev);
-    if (use_pair(n, m, sms)) launch_pair(p, w_codes, x_codes, k, lora, dev, sms, st);
+    if (use_pair(n, m)) launch_pair(p, w_codes, x_codes, k, lora, dev, sms, st);
     else if (bn == 16) launch_stream<16>(p, w_codes, x_codes, k, st);
     else if (bn == 32) launch_stream<32>(p, w_codes, x_codes, k, st);
     else if (bn == 64) launch_stream<64>(p, w_codes, x_codes, k, st);
@@ -988,20 +989,22 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
 }
 
 // ---- with an adapter ------------------------------------------------------------------------------
-// y += h . B for few tokens (or few outputs): h = s * H [n, ext] and B [r, m] in bf16, the sum in f32, y rounded once more.
-// A thread owns two columns of eight rows; launch and latency bound it: 77 x 6144, rank 16 (240 blocks of 128 threads, y
-// fetched ahead) 4.6 us, with 120 blocks of 256 and y last 6.9.
+// y = base + h . B for few tokens (or few outputs): base [n, m] the product in f32, h = s * H [n, ext] and B [r, m] in bf16, y
+// rounded once, as the pair kernel's is.  A thread owns two columns of eight rows, base fetched ahead of the sums (240 blocks of
+// 128 threads at 77 x 6144; with 120 blocks of 256 and y last it took 6.9 us instead of 4.6); launch and latency bound it: the whole
+// call, rank 16, takes 26.2 us as a graph, with a bf16 base that y rounded again 25.9.
 constexpr int kDeltaRows = 8;
 constexpr int kDeltaThreads = 128;
-__global__ void __launch_bounds__(kDeltaThreads) mx4_add_delta_kernel(__nv_bfloat16* __restrict__ y, const __nv_bfloat16* __restrict__ h,
-                                                            const __nv_bfloat16* __restrict__ b, int64_t n, int64_t m, int r, int ext) {
+__global__ void __launch_bounds__(kDeltaThreads) mx4_add_delta_kernel(const float* __restrict__ base, __nv_bfloat16* __restrict__ y,
+                                                            const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ b,
+                                                            int64_t n, int64_t m, int r, int ext) {
     extern __shared__ float hs[];  // [rank][row]
     const int64_t row0 = (int64_t)blockIdx.y * kDeltaRows, col = ((int64_t)blockIdx.x * kDeltaThreads + threadIdx.x) * 2;
-    __nv_bfloat162 base[kDeltaRows] = {};  // fetched ahead of the sums
+    float2 acc[kDeltaRows] = {};  // fetched ahead of the sums
     if (col < m) {  // m is even
 #pragma unroll
         for (int i = 0; i < kDeltaRows; ++i)
-            if (row0 + i < n) base[i] = *(const __nv_bfloat162*)(y + (row0 + i) * m + col);
+            if (row0 + i < n) acc[i] = *(const float2*)(base + (row0 + i) * m + col);
     }
     for (int i = threadIdx.x; i < r * kDeltaRows; i += kDeltaThreads) {
         const int row = i / r, j = i - row * r;
@@ -1009,7 +1012,6 @@ __global__ void __launch_bounds__(kDeltaThreads) mx4_add_delta_kernel(__nv_bfloa
     }
     __syncthreads();
     if (col >= m) return;
-    float2 acc[kDeltaRows] = {};
 #pragma unroll 8
     for (int j = 0; j < r; ++j) {
         const float2 w = __bfloat1622float2(*(const __nv_bfloat162*)(b + j * m + col));
@@ -1021,22 +1023,21 @@ __global__ void __launch_bounds__(kDeltaThreads) mx4_add_delta_kernel(__nv_bfloa
     }
 #pragma unroll
     for (int i = 0; i < kDeltaRows; ++i)
-        if (row0 + i < n) {
-            const float2 v = __bfloat1622float2(base[i]);
-            *(__nv_bfloat162*)(y + (row0 + i) * m + col) = __floats2bfloat162_rn(v.x + acc[i].x, v.y + acc[i].y);
-        }
+        if (row0 + i < n) *(__nv_bfloat162*)(y + (row0 + i) * m + col) = __floats2bfloat162_rn(acc[i].x, acc[i].y);
 }
 
-// The forward's workspace: the quantised x, s * H, H where the caller does not keep it, and the partial sums of H.
+// The forward's workspace: the quantised x, s * H, H where the caller does not keep it, the partial sums of H, and the product
+// in f32 where the delta is added by a kernel of its own.
 struct LoraSpace {
-    size_t ext, h, part, bytes;
+    size_t ext, h, part, base, bytes;
 };
-LoraSpace lora_space(int64_t n, int64_t k, int r) {
+LoraSpace lora_space(int64_t n, int64_t m, int64_t k, int r) {
     LoraSpace s;
     s.ext = al256(lq_mx4_linear_workspace_bytes(n, k));
     s.h = s.ext + al256((size_t)n * lq_tc_ext_width(r) * 2);
     s.part = s.h + al256((size_t)n * r * 4);
-    s.bytes = s.part + lq_tc_lora_down_bytes(n, r);
+    s.base = s.part + al256(lq_tc_lora_down_bytes(n, r));
+    s.bytes = s.base + (use_pair(n, m) ? 0 : (size_t)n * m * 4);
     return s;
 }
 lq_weight lora_weight(const void* codes, const void* scales, int64_t m, int64_t k, int dev) {
@@ -1196,7 +1197,7 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
 
 size_t lq_mx4_lora_workspace_bytes(int64_t n, int64_t m, int64_t k, int rank, int backward) {
     if (n < 1 || m < 1 || k < 32 || rank < 1 || rank > 256) return 0;
-    if (!backward) return lora_space(n, k, rank).bytes;
+    if (!backward) return lora_space(n, m, k, rank).bytes;
     const lq_weight w = lora_weight(nullptr, nullptr, m, k, 0);
     return lq_tc_workspace_bytes(&w, n, rank);
 }
@@ -1209,7 +1210,7 @@ int lq_mx4_lora_fwd(const void* x, int64_t n, const void* w_codes, const void* w
         check_tensor(w_codes, w_scales);
         LQ_CHECK_ARG(x && y && al16(x) && al16(y), "x and y must be 16-byte aligned");
         LQ_CHECK_ARG(ws && ((uintptr_t)ws & 255) == 0, "a 256-byte aligned workspace is needed");
-        const LoraSpace sp = lora_space(n, k, rank);
+        const LoraSpace sp = lora_space(n, m, k, rank);
         if (ws_bytes < sp.bytes) throw LqError(LQ_ERR_WORKSPACE, "workspace too small for the microscaled linear with an adapter");
         cudaStream_t st = (cudaStream_t)stream;
         const int dev = current_device(), sms = lq_tc_sm_count(dev), ext = lq_tc_ext_width(rank);
@@ -1218,18 +1219,21 @@ int lq_mx4_lora_fwd(const void* x, int64_t n, const void* w_codes, const void* w
         __nv_bfloat16* sh = (__nv_bfloat16*)(codes + sp.ext);
         lq_tc_lora_down(x, n, k, k, mv.At, rank, scaling, h_out ? h_out : (float*)(codes + sp.h), sh, codes + sp.part, sms, st);
         quantize(x, LQ_BF16, n, k, k, codes, scales, dev, st);
-        const LoraOperands lora{sh, mv.Bt, ext};
-        product(codes, scales, n, w_codes, w_scales, m, k, bias, y, LQ_BF16, true, dev, st, &lora);
-        if (!use_pair(n, m, sms)) {
-            LqProf prof(LQ_K_REDUCE, st);
-            const int64_t rows = (n + kDeltaRows - 1) / kDeltaRows;
-            for (int64_t first = 0; first < rows; first += 65535) {
-                const int64_t part = std::min<int64_t>(65535, rows - first), at = first * kDeltaRows;
-                const dim3 grid((unsigned)((m + 2 * kDeltaThreads - 1) / (2 * kDeltaThreads)), (unsigned)part);
-                mx4_add_delta_kernel<<<grid, kDeltaThreads, (size_t)rank * kDeltaRows * 4, st>>>(
-                    (__nv_bfloat16*)y + at * m, sh + at * ext, mv.Bb, n - at, m, rank, ext);
-                LQ_CUDA(cudaGetLastError());
-            }
+        if (use_pair(n, m)) {
+            const LoraOperands lora{sh, mv.Bt, ext};
+            product(codes, scales, n, w_codes, w_scales, m, k, bias, y, LQ_BF16, true, dev, st, &lora);
+            return;
+        }
+        float* base = (float*)(codes + sp.base);
+        product(codes, scales, n, w_codes, w_scales, m, k, bias, base, LQ_F32, true, dev, st);
+        LqProf prof(LQ_K_REDUCE, st);
+        const int64_t rows = (n + kDeltaRows - 1) / kDeltaRows;
+        for (int64_t first = 0; first < rows; first += 65535) {
+            const int64_t part = std::min<int64_t>(65535, rows - first), at = first * kDeltaRows;
+            const dim3 grid((unsigned)((m + 2 * kDeltaThreads - 1) / (2 * kDeltaThreads)), (unsigned)part);
+            mx4_add_delta_kernel<<<grid, kDeltaThreads, (size_t)rank * kDeltaRows * 4, st>>>(base + at * m, (__nv_bfloat16*)y + at * m,
+                                                                                             sh + at * ext, mv.Bb, n - at, m, rank, ext);
+            LQ_CUDA(cudaGetLastError());
         }
     });
 }
