@@ -391,10 +391,14 @@ void check_outputs_py(const py::object& grad_list, const py::object& out_list) {
 }
 
 Tensor clip_grad_norm(const py::object& list, double max_norm, const py::object& out_list, double grad_scale) {
-    at::NoGradGuard no_grad;
     const std::vector<Tensor> grads = tensors_of(list, "gradients");
     const bool out = !out_list.is_none();
     const std::vector<Tensor> given = out ? tensors_of(out_list, "outputs") : std::vector<Tensor>();
+    if (at::GradMode::is_enabled())  // what torch's in-place operators refuse: most likely parameters in place of their gradients
+        for (const Tensor& t : out ? given : grads)
+            TORCH_CHECK(!t.requires_grad() || !t.is_leaf(), "a leaf that requires grad would be scaled in place: clip_grad_norm takes gradients, "
+                                                            "not parameters");
+    at::NoGradGuard no_grad;
     Gradients g(grads);
     TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must be >= 0, got ", max_norm);
     const std::vector<Tensor>& outs = out ? given : grads;
