@@ -925,7 +925,7 @@ void launch_pair(ProductParams p, const void* w_codes, const void* x_codes, int6
     p.x_tiles = (p.n + 255) / 256;
     p.w_tiles = (p.m + 255) / 256;
     LQ_CHECK_ARG((int64_t)p.x_tiles * p.w_tiles < (int64_t)1 << 31, "too many tiles");
-    const int pairs = std::min(resident_pairs(dev, sms), p.x_tiles * p.w_tiles);
+    const int pairs = std::min({resident_pairs(dev, sms), lq_tc_usable_sms(sms) / 2, p.x_tiles * p.w_tiles});
     auto kern = lora ? mx4_pair_kernel<true, true> : (tma_store ? mx4_pair_kernel<true, false> : mx4_pair_kernel<false, false>);
     LQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg2::SMEM));
     LqProf prof(LQ_K_GEMM_MAIN, st);

@@ -1578,6 +1578,8 @@ int lq_tc_read_status(int device, cudaStream_t st) {
     return v != 0 ? v : v2;
 }
 
+int lq_tc_usable_sms(int sm_count) { return usable_sms(sm_count); }
+
 int lq_tc_ext_width(int r) { return ext_width(r); }
 
 LqMirrorView lq_tc_mirror_view(int64_t K, int64_t M, int r, const void* mirror) {

@@ -70,6 +70,8 @@ int* lq_tc_status_word(int device);
 cudaStream_t lq_tc_fork(int device, cudaStream_t st);
 void lq_tc_join(int device, cudaStream_t st);
 int lq_tc_sm_count(int device);
+// ... of which a persistent grid may use this many (the "reserve_sms" option).
+int lq_tc_usable_sms(int sm_count);
 
 // Small-batch forward (int4 weights at N <= 64 tokens, scaled-fp8 weights at N <= 16): the packed
 // weight is streamed from HBM exactly once and converted on chip (registers + mma.sync at N <= 16,
