@@ -299,7 +299,8 @@ int lq_mx4_linear(const void* x, int dtype, int64_t n, int64_t ldx, const void* 
 /* dX[n, k] = dY[n, m] . W[m, k]: the gradient through the frozen weight (that of crates/loractl-core/src/
  * quant.rs:221-235), with the quantisation of x taken as the identity.  dy, dx contiguous, 16-byte aligned, LQ_BF16
  * (W is exact in bf16) or LQ_F32 (dy as three bf16 terms whose sum it is, each multiplied with f32 accumulation: products
- * are exact, so this is an f32 product).  `ws`: lq_mx4_matmul_dx_workspace_bytes() bytes, 256-byte aligned. */
+ * are exact, so this is an f32 product; bf16 ends at 2^-133, and what an element of dy has below that is cut).  `ws`:
+ * lq_mx4_matmul_dx_workspace_bytes() bytes, 256-byte aligned. */
 size_t lq_mx4_matmul_dx_workspace_bytes(int64_t n, int64_t m, int64_t k, int dtype);
 int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, const void* w_scales, int64_t m,
                      int64_t k, void* dx, void* ws, size_t ws_bytes, void* stream);
@@ -307,8 +308,8 @@ int lq_mx4_matmul_dx(const void* dy, int dtype, int64_t n, const void* w_codes, 
 /* A LoRA adapter on such a weight (crates/loractl-core/src/mmdit.rs:526-536), bf16 activations:
  *   H = X . A,   Y = quant(X) . W^T + bias + scaling * H . B,
  *   dX = dY . W + scaling * dY . B^T . A^T,   dA = scaling * X^T . dY . B^T,   dB = scaling * H^T . dY,
- * the adapter reading X itself; Y is rounded once, s * H and dH once each as operands.  `mirror`: lq_lora_mirror_update() of the factors (A [k, rank], B [rank, m]); m a multiple of
- * 8, rank <= 256; x, dy, y and dx contiguous, 16-byte aligned.  `h_out` / `h`: f32 [n, rank], may be NULL (the backward then
+ * the adapter reading X itself; Y is rounded once, scaling * H and scaling * dY . B^T once each as bf16 operands.  `mirror`:
+ * lq_lora_mirror_update() of the factors (A [k, rank], B [rank, m]); m a multiple of 8, rank <= 256; x, dy, y and dx contiguous, 16-byte aligned.  `h_out` / `h`: f32 [n, rank], may be NULL (the backward then
  * computes it again).  dX, dA and dB may be NULL; `accumulate` adds to dA and dB.  `ws`: lq_mx4_lora_workspace_bytes() bytes,
  * 256-byte aligned, of the forward or the backward; calls that can overlap need one each. */
 size_t lq_mx4_lora_workspace_bytes(int64_t n, int64_t m, int64_t k, int rank, int backward);

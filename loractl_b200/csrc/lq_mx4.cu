@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const __nv_bfloat16* __re
 }
 
 // [n, m] f32 as three stacked bf16 matrices [3, n, ld] whose sum it is: each takes the eight leading bits of what the one
-// before left, cut and not rounded, so nothing overflows and the third is exact too.  An Inf or a NaN goes to the first.
+// before left, cut and not rounded, so nothing overflows and the third is exact too (down to bf16's last bit, 2^-133).  An Inf or a NaN goes to the first.
 __global__ void __launch_bounds__(256) split3_kernel(const float* __restrict__ in, int64_t n, int64_t m, int64_t ld,
                                                      __nv_bfloat16* __restrict__ out) {
     const int64_t total = n * ld;

@@ -74,7 +74,8 @@ def mx4_matmul_t(x: Mx4Tensor, w: Mx4Tensor, bias: Optional[torch.Tensor] = None
 
 
 def mx4_matmul_dx(dy: torch.Tensor, w: Mx4Tensor) -> torch.Tensor:
-    """`dy [n, w.rows] . dequant(w)` in `dy`'s type: bf16 on the tensor cores (the weight is exact in bf16) or f32."""
+    """`dy [n, w.rows] . dequant(w)` in `dy`'s type: bf16 on the tensor cores (the weight is exact in bf16) or f32 (as three bf16
+    terms of dy, exact but for what an element has below 2^-133)."""
     return L.ext().mx4_matmul_dx(dy, w.codes, w.scales, w.rows, w.k)
 
 
