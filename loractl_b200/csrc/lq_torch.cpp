@@ -156,7 +156,7 @@ struct ResidualNormBackward : public Node {
         c10::cuda::OptionalCUDAGuard guard(device);
         const int64_t b = args.samples, h = args.h;
         const auto type = args.dtype == LQ_F32 ? at::kFloat : at::kBFloat16, mod = args.mod_f32 ? at::kFloat : at::kBFloat16;
-        const std::vector<int64_t> rows = {b, args.tokens, h}, vectors = {b, h}, columns = {h};
+        const int64_t rows[] = {b, args.tokens, h}, vectors[] = {b, h}, columns[] = {h};
         const ResidualNormInputs in = {restored(tensors[0], rows, type, device, "x"), restored(tensors[1], rows, type, device, "y"),
                                        restored(tensors[2], vectors, mod, device, "gate"), restored(tensors[3], vectors, mod, device, "shift"),
                                        restored(tensors[4], vectors, mod, device, "scale"), restored(tensors[5], columns, at::kFloat, device, "weight"),
@@ -282,13 +282,18 @@ std::vector<Tensor> tensors_of(const py::object& list, const char* what) {
     return v;
 }
 
+// Leaves that require grad are refused where they would be scaled, as torch's in-place operators do: they are most likely parameters
+// in place of their gradients.
+inline void no_parameter(const Tensor& t) {
+    TORCH_CHECK(!t.requires_grad() || !t.is_leaf(), "a leaf that requires grad would be scaled in place: clip_grad_norm takes gradients, not parameters");
+}
+
 struct Gradients {
     std::vector<const void*> at;
     std::vector<int64_t> counts;
     std::vector<int32_t> types;
-    explicit Gradients(const std::vector<Tensor>& grads) {
+    explicit Gradients(const std::vector<Tensor>& grads, bool scaled = false) {
         TORCH_CHECK_VALUE(!grads.empty(), "no gradient tensors");
-        require_cuda(grads[0], "gradients");
         at.reserve(grads.size()), counts.reserve(grads.size()), types.reserve(grads.size());
         for (const Tensor& t : grads) {
             TORCH_CHECK(t.device() == grads[0].device(), "gradients must live on one CUDA device, got ", grads[0].device(), " and ", t.device());
@@ -297,7 +302,9 @@ struct Gradients {
             at.push_back(t.const_data_ptr());
             counts.push_back(t.numel());
             types.push_back(type == at::kFloat ? LQ_F32 : LQ_BF16);
+            if (scaled) no_parameter(t);
         }
+        require_cuda(grads[0], "gradients");
     }
 };
 
@@ -394,12 +401,11 @@ Tensor clip_grad_norm(const py::object& list, double max_norm, const py::object&
     const std::vector<Tensor> grads = tensors_of(list, "gradients");
     const bool out = !out_list.is_none();
     const std::vector<Tensor> given = out ? tensors_of(out_list, "outputs") : std::vector<Tensor>();
-    if (at::GradMode::is_enabled())  // what torch's in-place operators refuse: most likely parameters in place of their gradients
-        for (const Tensor& t : out ? given : grads)
-            TORCH_CHECK(!t.requires_grad() || !t.is_leaf(), "a leaf that requires grad would be scaled in place: clip_grad_norm takes gradients, "
-                                                            "not parameters");
+    const bool grad_mode = at::GradMode::is_enabled();
+    if (grad_mode)
+        for (const Tensor& t : given) no_parameter(t);
     at::NoGradGuard no_grad;
-    Gradients g(grads);
+    Gradients g(grads, grad_mode && !out);
     TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must be >= 0, got ", max_norm);
     const std::vector<Tensor>& outs = out ? given : grads;
     std::vector<const void*> to;
