@@ -210,8 +210,9 @@ def zrmsnorm(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 # ---- the seam between two sub-blocks --------------------------------------------------------------
 
 def modulated_zrmsnorm(x: torch.Tensor, weight: Optional[torch.Tensor], shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
-    """`zrmsnorm(x, weight) * (1 + scale) + shift` (mmdit.rs:857-862 before a sub-block), one kernel each way; `weight`
-    `[h]` or None.  Gradients flow to every argument that asks for one, the norm's weight among them."""
+    """`zrmsnorm(x, weight) * (1 + scale) + shift` (mmdit.rs:857-862 before a sub-block), one kernel forward and backward
+    that of `gated_residual_norm`; `weight` `[h]` or None.  Gradients flow to every argument that asks for one, the norm's
+    weight among them."""
     return L.ext().residual_norm(x, None, None, shift, scale, weight, None, False, 1.0, ZRMS_EPS)[0]
 
 
@@ -227,8 +228,9 @@ def gated_residual_norm(x: torch.Tensor, gate: torch.Tensor, y: torch.Tensor, sh
     `x`, `y`: `[b, tokens, h]`, f32 or bf16 alike, rows contiguous, samples and tokens at any stride; `gate`, `shift`,
     `scale`: `[b, 1, h]` or `[b, h]` (slices of one modulation tensor are read in place; expand over `b` to share a
     vector); `weight`, `post_weight`: `[h]` or None; h <= 16384.  `norm`: "zrms" (mmdit.rs:282-330) or "layer".
-    Arithmetic is f32, `z` comes from the unrounded `r`, each output is rounded once; one kernel forward, one plus a
-    fixed-order sum over tokens backward, gradients to every tensor argument that asks for one."""
+    Arithmetic is f32, `z` comes from the unrounded `r`, each output is rounded once; one kernel forward; backward
+    one, and for the vectors a fixed-order sum over tokens (in two launches with norm weights over many samples).  Gradients go
+    to every tensor argument that asks for one."""
     if gate is None or y is None:
         raise ValueError("gate and y are needed: modulated_zrmsnorm is the norm alone")
     if norm not in ("zrms", "layer"):

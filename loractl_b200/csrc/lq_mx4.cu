@@ -295,7 +295,8 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {
 // reduction is cut into `splits` ranges, one block each, and the blocks of a tile are a cluster that adds its f32
 // tiles up through distributed shared memory, in rank order, each rank a share of the tokens.  (Partial tiles in HBM and
 // a second launch took 5.8 us of 14.6 at 77 x 2592 -> 6151, where this takes 9.6.)  One token through 6144 -> 16384 takes
-// 12.9 us, 4.1 TB/s of weight; the launch, its ramp and the loads alone take 11.3.  D's lane is a weight row, so a store of one
+// 13.4 us from HBM (captured, eight weights in turn), 4.0 TB/s of weight, and 10.4 with the weight in the L2; the launch, its ramp and
+// the loads alone take 11.3.  D's lane is a weight row, so a store of one
 // token writes 32 consecutive outputs.
 template <int BN>
 __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_constant__ CUtensorMap tmW,
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 2) mx4_stream_kernel(const __grid_co
 // the stage they came with, so that a stage's release covers them.  The accumulator has one buffer (256 columns; two
 // would leave no room for scales): the epilogue empties it into registers at once and converts and stores
 // while the next tile's products run.  4096 x 6144 -> 16384: 167 us, 4.9 PFLOP/s (single CTAs with 128 x 128 tiles: 343 us);
-// for seconds on end 4.3 PFLOP/s, at the card's power cap.  An adapter's product is one more k-block of bf16 for each 64 of
+// for seconds on end 4.3 PFLOP/s, at the card's power cap.  Its 128 registers a thread (448 threads) spill 44-56 bytes.  An adapter's product is one more k-block of bf16 for each 64 of
 // rank (the ring's stages fit: 64 bf16 are 128 bytes a row too): 180 us with rank 16.
 struct Cfg2 {
     static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = 128 * 128, SA_BYTES = 2 * kTile, SB_BYTES = 4 * kTile;
@@ -991,8 +992,8 @@ void product(const void* x_codes, const void* x_scales, int64_t n, const void* w
 // ---- with an adapter ------------------------------------------------------------------------------
 // y = base + h . B for few tokens (or few outputs): base [n, m] the product in f32, h = s * H [n, ext] and B [r, m] in bf16, y
 // rounded once, as the pair kernel's is.  A thread owns two columns of eight rows, base fetched ahead of the sums (240 blocks of
-// 128 threads at 77 x 6144; with 120 blocks of 256 and y last it took 6.9 us instead of 4.6); launch and latency bound it: the whole
-// call, rank 16, takes 26.2 us as a graph, with a bf16 base that y rounded again 25.9.
+// 128 threads at 77 x 6144: 4.6 us; with 120 blocks of 256 and y last 6.9); launch and latency bound it.  The whole call, rank 16,
+// takes 26.2 us as a graph, with a bf16 base that y rounded again 25.9.
 constexpr int kDeltaRows = 8;
 constexpr int kDeltaThreads = 128;
 __global__ void __launch_bounds__(kDeltaThreads) mx4_add_delta_kernel(const float* __restrict__ base, __nv_bfloat16* __restrict__ y,

@@ -117,7 +117,8 @@ struct Rows {
 // Register rows instead of the ring (one row per block, loads straight to registers) took 29 us forward and 95 us
 // backward on 1536 rows of 6144 bf16 columns, where this takes 17 and 25; the modulation read again from L1 for every row
 // was part of that.  At 4096 rows 34 us and 63 us: 89 % and 73 % of the measured HBM rate; 8 x 4096 x 2048 with the layer
-// norm 93 us and 150 us: 88 % and 82 %.
+// norm 93 us and 150 us: 88 % and 82 %.  The backward's column sums and modulation spill 16-140 bytes a thread at 80 registers, 144-296
+// at the 64 of 1024 threads.
 
 // Eight elements as they are stored (four registers in bf16): what is needed again behind a barrier waits like this.
 template <typename T>
@@ -518,7 +519,8 @@ __global__ void __launch_bounds__(MAXT, MINB) resnorm_bwd_ring_kernel(const Args
 // used, whatever columns the thread has (a place behind the row reads column 0 and counts as zero).  Up to 4096 columns
 // (512 threads) the modulation stays in registers over the rows of a chunk and the next row is fetched into registers behind
 // the current one's arithmetic; wider rows have no registers for either and take 1024 threads (4000 rows of 7777 bf16 columns:
-// 145 us forward, 295 us backward; the backward with 512 threads 424 us).  Bound by instructions, two accesses and a dozen
+// 145 us forward, 295 us backward; the backward with 512 threads 424 us), whose 64 registers spill 392-468 bytes a thread in the
+// backward up to 8192 columns and 1372-1464 above (272-328 there in the forward).  Bound by instructions, two accesses and a dozen
 // of arithmetic an element: 8000 rows of 4001 f32 columns 152 us forward and 166 us backward (51 % and 71 % of HBM),
 // 24000 rows of 1155 bf16 columns 110 us and 153 us (31 % and 33 %; 1152 columns by the ring: 41 us and 69 us).
 template <typename T, int VPT>
