@@ -230,9 +230,12 @@ class SingleStreamBlock(nn.Module):
     def forward(self, x: torch.Tensor, tvec: torch.Tensor, rope, mask4: Optional[torch.Tensor],
                 adapters: Optional[LoraAdapters] = None, prefix: str = "blocks.0") -> torch.Tensor:
         f = self.config.features
-        mod = tvec + self.mod_lin.to(tvec.dtype)  # [b, 1, 6f]
+        mod = tvec + self.mod_lin.to(tvec.dtype)  # [b, 1, 6f], or [1, 1, 6f] for the whole batch
+        fused = self.fused_norms and x.is_cuda
+        if fused:
+            mod = mod.expand(x.shape[0], -1, -1)
         prescale, preshift, pregate, postscale, postshift, postgate = (mod[..., i * f:(i + 1) * f] for i in range(6))
-        if self.fused_norms and x.is_cuda:
+        if fused:
             from .block_ops import gated_residual, gated_residual_norm, modulated_zrmsnorm
 
             att = self.attn(modulated_zrmsnorm(x, self.prenorm.scale, preshift, prescale), rope, mask4, adapters, f"{prefix}.attn")
